@@ -8,6 +8,10 @@ HERE = os.path.dirname(os.path.abspath(__file__))
 CSRC = os.path.join(HERE, "csrc")
 SOURCES = ["gemm.hip", "gemm_wres.hip", "gemm_dw.hip", "gemm_dw4.hip", "attention.hip", "attention_mfma.hip", "attention_qkv.hip", "gru.hip", "mixer.hip", "replay.hip", "collective.hip", "learner.hip", "profile.hip"]
 LIB = os.path.join(HERE, "librefil_hip.so")
+# Packed fp32 arithmetic (v_pk_add / mul / fma_f32) stays off: the compiler forms it from ordinary float code, and some of its forms have
+# given wrong results on this hardware now and then. Same IEEE operations, one lane at a time. (hipcc's host pass does not know the
+# feature and says so: harmless.)
+NO_PACKED_FP32 = ["-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops"]
 
 
 def _stale():
@@ -24,12 +28,20 @@ def build(force=False, verbose=True):
     hipcc = os.environ.get("HIPCC", "/opt/rocm/bin/hipcc")
     objs = []
     procs = []
-    os.makedirs(os.path.join(HERE, "build"), exist_ok=True)
+    extra = os.environ.get("REFIL_EXTRA_FLAGS", "").split()
+    obj_dir = os.path.join(HERE, "build", "extra") if extra else os.path.join(HERE, "build")     # (a variant's objects never mix with the library's)
+    os.makedirs(obj_dir, exist_ok=True)
+    headers = [os.path.join(CSRC, f) for f in os.listdir(CSRC) if f.endswith(".h")]
+    headers += [os.path.join(HERE, "..", "include", "refil_hip.h"), os.path.abspath(__file__)]
     for src in SOURCES:
-        obj = os.path.join(HERE, "build", src.replace(".hip", ".o"))
-        cmd = [hipcc, "--offload-arch=gfx950", "-O3", "-std=c++17", "-fPIC"] + os.environ.get("REFIL_EXTRA_FLAGS", "").split() + ["-c", os.path.join(CSRC, src), "-o", obj]
-        procs.append((src, subprocess.Popen(cmd, stdout=subprocess.PIPE, stderr=subprocess.STDOUT)))
+        obj = os.path.join(obj_dir, src.replace(".hip", ".o"))
+        cmd = [hipcc, "--offload-arch=gfx950", "-O3", "-std=c++17", "-fPIC"] + NO_PACKED_FP32 + extra + ["-c", os.path.join(CSRC, src), "-o", obj]
         objs.append(obj)
+        # one source changed: one compile (an object newer than its source and every header is kept unless the build is forced)
+        if not force and not extra and os.path.exists(obj) and \
+                all(os.path.getmtime(d) <= os.path.getmtime(obj) for d in headers + [os.path.join(CSRC, src)]):
+            continue
+        procs.append((src, subprocess.Popen(cmd, stdout=subprocess.PIPE, stderr=subprocess.STDOUT)))
     for src, p in procs:
         out, _ = p.communicate()
         if p.returncode != 0:
