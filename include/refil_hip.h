@@ -464,6 +464,111 @@ typedef struct refil_gru_desc {
 int refil_gru_forward(const refil_gru_desc* desc, void* stream);
 int refil_gru_backward(const refil_gru_desc* desc, void* stream);
 
+/* ---- the residual temporal block: an alternative to the GRU cell for long episodes ---------------------------------------
+ * Three operators around one residual stream: norm -> gated LINEAR recurrence -> norm, gate, residual -> gated feed-forward -> norm,
+ * gate, residual. No counterpart in the reference (its one recurrence is the GRUCell of entity_rnn_agent.py:49-55). Element types of
+ * the activations and the feed-forward weights: fp32, bf16 or fp16 (`dtype`); parameters of the recurrence and the norms, hidden
+ * states and their gradients are fp32. All strides count ELEMENTS, the innermost dimension is contiguous, no alignment beyond the
+ * element's is needed. Workspaces are scratch of one call: no content is kept, two calls in flight need two of them. Inputs and outputs
+ * of one call must not overlap (except state / state_out of refil_linrec_step, which may be the same buffer). */
+enum { REFIL_F32 = 0, REFIL_BF16 = 1, REFIL_F16 = 2 };
+
+/* Gated linear recurrence over [B, T, C], channel c with decay[c % D] (agents: C = n_agents * D):
+ *   L_t = scale softplus(decay) sigmoid(ga_t),  a_t = exp(-L_t)
+ *   h_t = a_t h_{t-1} + sqrt(1 - a_t^2) sigmoid(gi_t) x_t,   y_t = h_t
+ *   h0 [B,C] fp32 or NULL (zero); reset [B,T] uint8 or NULL: != 0 drops h_{t-1} (and h0) at that step, whatever it holds;
+ *   lengths [B] int32 or NULL: episode b has min(max(lengths[b],0),T) steps -- later steps are not read, their y is written as 0 and so
+ *   are their gradients, the state stays; h_last [B,C] fp32 or NULL: the state after the last step.
+ *   saved: NULL, or refil_linrec_saved_floats floats that the backward needs (the state at every 64th step).
+ * Backward (x, ga, gi, decay, h0, reset, lengths as in the forward, saved from it): dy [B,T,C], dh_last [B,C] or NULL ->
+ *   dx, dga, dgi (strides d_sB, d_sT), ddecay [D] (sum over everything that shares it), dh0 [B,C] or NULL. Deterministic. */
+typedef struct refil_linrec_desc {
+    const void* x;  int64_t x_sB, x_sT;
+    const void* ga; int64_t ga_sB, ga_sT;
+    const void* gi; int64_t gi_sB, gi_sT;
+    const float* decay; const float* h0;
+    const uint8_t* reset; int64_t rs_sB, rs_sT;
+    const int32_t* lengths;
+    void* y; int64_t y_sB, y_sT;
+    float* h_last; float* saved;
+    const void* dy; int64_t dy_sB, dy_sT;
+    const float* dh_last;
+    void* dx; void* dga; void* dgi; int64_t d_sB, d_sT;
+    float* ddecay; float* dh0;
+    int32_t B, T, C, D, dtype;
+    float scale;
+    void* workspace; size_t workspace_bytes;
+} refil_linrec_desc;
+size_t refil_linrec_workspace_bytes(const refil_linrec_desc* desc, int32_t backward);
+int64_t refil_linrec_saved_floats(const refil_linrec_desc* desc);
+int refil_linrec_forward(const refil_linrec_desc* desc, void* stream);
+int refil_linrec_backward(const refil_linrec_desc* desc, void* stream);
+
+/* One step of it for B rows (acting): x, ga, gi [B,C]; row b advances state[slots[b]] (slots NULL: state[b]) of [n_slots, C] fp32 into
+ * state_out (the same buffer, or another one of that shape: slots that no row names are not written there) and writes y[b]. A slot
+ * outside [0, n_slots) marks a padded row: y is 0, no state is touched. Rows that name one slot are consecutive steps of it, in row order. */
+typedef struct refil_linrec_step_desc {
+    const void* x;  int64_t x_sB;
+    const void* ga; int64_t ga_sB;
+    const void* gi; int64_t gi_sB;
+    const float* decay; const float* state; float* state_out; const int32_t* slots;
+    void* y; int64_t y_sB;
+    int32_t B, C, D, n_slots, dtype;
+    float scale;
+} refil_linrec_step_desc;
+int refil_linrec_step(const refil_linrec_step_desc* desc, void* stream);
+
+/* Norms before and after a block, fused with its gate and residual scale, on N rows of D <= 16384:
+ *   N(v; w) = v w / sqrt(mean(v^2) + eps);   y = alpha x + res_scale sigmoid(gate) N(o; post_weight);   n = N(y; pre_weight)
+ *   o / gate NULL: the term / the factor is left out; weights NULL: ones; row_mask [N] uint8 or NULL: rows with != 0 (inactive agents) are not
+ *   read, their outputs and gradients are 0. y / n NULL: not written (one of them is).
+ * Backward: dy / dn (one may be NULL) -> dx, d_o (with o), dgate (with gate), and dpost_weight / dres_scale / dpre_weight [D] (any may be
+ *   NULL), summed in a fixed order. */
+typedef struct refil_norm_gate_desc {
+    const void* x; int64_t x_stride;
+    const void* o; int64_t o_stride;
+    const void* gate; int64_t gate_stride;
+    const float* post_weight; const float* res_scale; const float* pre_weight;
+    const uint8_t* row_mask;
+    void* y; int64_t y_stride;
+    void* n; int64_t n_stride;
+    const void* dy; int64_t dy_stride;
+    const void* dn; int64_t dn_stride;
+    void* dx; int64_t dx_stride;
+    void* d_o; int64_t do_stride;
+    void* dgate; int64_t dgate_stride;
+    float* dpost_weight; float* dres_scale; float* dpre_weight;
+    int64_t N;
+    int32_t D, dtype;
+    float alpha, eps;
+    void* workspace; size_t workspace_bytes;      /* backward only */
+} refil_norm_gate_desc;
+size_t refil_norm_gate_workspace_bytes(const refil_norm_gate_desc* desc);
+int refil_norm_gate_forward(const refil_norm_gate_desc* desc, void* stream);
+int refil_norm_gate_backward(const refil_norm_gate_desc* desc, void* stream);
+
+/* Gated feed-forward block: h[N,F] = act(x w_gate^T + b_gate) * (x w_up^T + b_up), x [N,D], w_* [F,D] (both with w_stride), b_* [F] or NULL,
+ * all of `dtype`; act: REFIL_ACT_SILU v sigmoid(v), REFIL_ACT_GELU the tanh form. saved: NULL, or 2 N F elements of dtype that the
+ * backward needs (the two pre-activations). Backward: dh -> dx, dw_gate, dw_up [F,D] contiguous, db_* [F] or NULL; sums in fp32, rounded
+ * once. fp32 products run as six bf16 matrix products of an exact three-way split (refil_set_tuning's "wres_split" = 6 arithmetic). */
+enum { REFIL_ACT_SILU = 0, REFIL_ACT_GELU = 1 };
+typedef struct refil_gated_ff_desc {
+    const void* x; int64_t x_stride;
+    const void* w_gate; const void* w_up; int64_t w_stride;
+    const void* b_gate; const void* b_up;
+    void* h; int64_t h_stride;
+    void* saved;
+    const void* dh; int64_t dh_stride;
+    void* dx; int64_t dx_stride;
+    void* dw_gate; void* dw_up; void* db_gate; void* db_up;
+    int64_t N;
+    int32_t D, F, act, dtype;
+    void* workspace; size_t workspace_bytes;
+} refil_gated_ff_desc;
+size_t refil_gated_ff_workspace_bytes(const refil_gated_ff_desc* desc, int32_t backward);
+int refil_gated_ff_forward(const refil_gated_ff_desc* desc, void* stream);
+int refil_gated_ff_backward(const refil_gated_ff_desc* desc, void* stream);
+
 /* Optional per-kernel timing (HIP events recorded on the launch stream around every kernel the
  * library launches, aggregated per kernel symbol). bench.py uses it for the roofline fraction.
  * refil_profile_collect synchronises the device and returns MINUS the number of entries written

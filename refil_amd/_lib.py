@@ -115,6 +115,63 @@ class GruDesc(C.Structure):
     ]
 
 
+F32, BF16, F16 = 0, 1, 2
+ACT_SILU, ACT_GELU = 0, 1
+
+
+class LinrecDesc(C.Structure):
+    _fields_ = [
+        ("x", C.c_void_p), ("x_sB", C.c_int64), ("x_sT", C.c_int64),
+        ("ga", C.c_void_p), ("ga_sB", C.c_int64), ("ga_sT", C.c_int64),
+        ("gi", C.c_void_p), ("gi_sB", C.c_int64), ("gi_sT", C.c_int64),
+        ("decay", C.c_void_p), ("h0", C.c_void_p),
+        ("reset", C.c_void_p), ("rs_sB", C.c_int64), ("rs_sT", C.c_int64),
+        ("lengths", C.c_void_p),
+        ("y", C.c_void_p), ("y_sB", C.c_int64), ("y_sT", C.c_int64),
+        ("h_last", C.c_void_p), ("saved", C.c_void_p),
+        ("dy", C.c_void_p), ("dy_sB", C.c_int64), ("dy_sT", C.c_int64),
+        ("dh_last", C.c_void_p),
+        ("dx", C.c_void_p), ("dga", C.c_void_p), ("dgi", C.c_void_p), ("d_sB", C.c_int64), ("d_sT", C.c_int64),
+        ("ddecay", C.c_void_p), ("dh0", C.c_void_p),
+        ("B", C.c_int32), ("T", C.c_int32), ("C", C.c_int32), ("D", C.c_int32), ("dtype", C.c_int32),
+        ("scale", C.c_float),
+        ("workspace", C.c_void_p), ("workspace_bytes", C.c_size_t),
+    ]
+
+
+class LinrecStepDesc(C.Structure):
+    _fields_ = [
+        ("x", C.c_void_p), ("x_sB", C.c_int64), ("ga", C.c_void_p), ("ga_sB", C.c_int64), ("gi", C.c_void_p), ("gi_sB", C.c_int64),
+        ("decay", C.c_void_p), ("state", C.c_void_p), ("state_out", C.c_void_p), ("slots", C.c_void_p),
+        ("y", C.c_void_p), ("y_sB", C.c_int64),
+        ("B", C.c_int32), ("C", C.c_int32), ("D", C.c_int32), ("n_slots", C.c_int32), ("dtype", C.c_int32), ("scale", C.c_float),
+    ]
+
+
+class NormGateDesc(C.Structure):
+    _fields_ = [
+        ("x", C.c_void_p), ("x_stride", C.c_int64), ("o", C.c_void_p), ("o_stride", C.c_int64), ("gate", C.c_void_p), ("gate_stride", C.c_int64),
+        ("post_weight", C.c_void_p), ("res_scale", C.c_void_p), ("pre_weight", C.c_void_p), ("row_mask", C.c_void_p),
+        ("y", C.c_void_p), ("y_stride", C.c_int64), ("n", C.c_void_p), ("n_stride", C.c_int64),
+        ("dy", C.c_void_p), ("dy_stride", C.c_int64), ("dn", C.c_void_p), ("dn_stride", C.c_int64),
+        ("dx", C.c_void_p), ("dx_stride", C.c_int64), ("d_o", C.c_void_p), ("do_stride", C.c_int64), ("dgate", C.c_void_p), ("dgate_stride", C.c_int64),
+        ("dpost_weight", C.c_void_p), ("dres_scale", C.c_void_p), ("dpre_weight", C.c_void_p),
+        ("N", C.c_int64), ("D", C.c_int32), ("dtype", C.c_int32), ("alpha", C.c_float), ("eps", C.c_float),
+        ("workspace", C.c_void_p), ("workspace_bytes", C.c_size_t),
+    ]
+
+
+class GatedFfDesc(C.Structure):
+    _fields_ = [
+        ("x", C.c_void_p), ("x_stride", C.c_int64), ("w_gate", C.c_void_p), ("w_up", C.c_void_p), ("w_stride", C.c_int64),
+        ("b_gate", C.c_void_p), ("b_up", C.c_void_p), ("h", C.c_void_p), ("h_stride", C.c_int64), ("saved", C.c_void_p),
+        ("dh", C.c_void_p), ("dh_stride", C.c_int64), ("dx", C.c_void_p), ("dx_stride", C.c_int64),
+        ("dw_gate", C.c_void_p), ("dw_up", C.c_void_p), ("db_gate", C.c_void_p), ("db_up", C.c_void_p),
+        ("N", C.c_int64), ("D", C.c_int32), ("F", C.c_int32), ("act", C.c_int32), ("dtype", C.c_int32),
+        ("workspace", C.c_void_p), ("workspace_bytes", C.c_size_t),
+    ]
+
+
 class GatherField(C.Structure):
     _fields_ = [("src", C.c_void_p), ("dst", C.c_void_p), ("src_episode_bytes", C.c_int64), ("dst_episode_bytes", C.c_int64),
                 ("copy_bytes", C.c_int64), ("unpack_width", C.c_int32), ("reserved", C.c_int32)]
@@ -142,6 +199,9 @@ EXPORTS = [
     "refil_oneshot_create", "refil_oneshot_connect", "refil_oneshot_allreduce", "refil_oneshot_status", "refil_oneshot_destroy",
     "refil_allreduce_flat", "refil_pack_mask_bits", "refil_side_stream", "refil_set_tuning", "refil_get_stat",
     "refil_attn_qkv_forward",
+    "refil_linrec_workspace_bytes", "refil_linrec_saved_floats", "refil_linrec_forward", "refil_linrec_backward", "refil_linrec_step",
+    "refil_norm_gate_workspace_bytes", "refil_norm_gate_forward", "refil_norm_gate_backward",
+    "refil_gated_ff_workspace_bytes", "refil_gated_ff_forward", "refil_gated_ff_backward",
 ]
 IPC_HANDLE_BYTES = 64
 
@@ -192,6 +252,21 @@ def lib():
     L.refil_pool_backward.argtypes = [C.POINTER(AttnDesc), C.c_int32, C.c_void_p]
     L.refil_gru_forward.argtypes = [C.POINTER(GruDesc), C.c_void_p]
     L.refil_gru_backward.argtypes = [C.POINTER(GruDesc), C.c_void_p]
+    L.refil_linrec_workspace_bytes.argtypes = [C.POINTER(LinrecDesc), C.c_int32]
+    L.refil_linrec_workspace_bytes.restype = C.c_size_t
+    L.refil_linrec_saved_floats.argtypes = [C.POINTER(LinrecDesc)]
+    L.refil_linrec_saved_floats.restype = C.c_int64
+    L.refil_linrec_forward.argtypes = [C.POINTER(LinrecDesc), C.c_void_p]
+    L.refil_linrec_backward.argtypes = [C.POINTER(LinrecDesc), C.c_void_p]
+    L.refil_linrec_step.argtypes = [C.POINTER(LinrecStepDesc), C.c_void_p]
+    L.refil_norm_gate_workspace_bytes.argtypes = [C.POINTER(NormGateDesc)]
+    L.refil_norm_gate_workspace_bytes.restype = C.c_size_t
+    L.refil_norm_gate_forward.argtypes = [C.POINTER(NormGateDesc), C.c_void_p]
+    L.refil_norm_gate_backward.argtypes = [C.POINTER(NormGateDesc), C.c_void_p]
+    L.refil_gated_ff_workspace_bytes.argtypes = [C.POINTER(GatedFfDesc), C.c_int32]
+    L.refil_gated_ff_workspace_bytes.restype = C.c_size_t
+    L.refil_gated_ff_forward.argtypes = [C.POINTER(GatedFfDesc), C.c_void_p]
+    L.refil_gated_ff_backward.argtypes = [C.POINTER(GatedFfDesc), C.c_void_p]
     L.refil_set_overlap.argtypes = [C.c_int]
     L.refil_side_stream.argtypes = [C.POINTER(C.c_void_p)]
     L.refil_set_tuning.argtypes = [C.c_char_p, C.c_int64]

@@ -6,7 +6,7 @@ import sys
 
 HERE = os.path.dirname(os.path.abspath(__file__))
 CSRC = os.path.join(HERE, "csrc")
-SOURCES = ["gemm.hip", "gemm_wres.hip", "gemm_dw.hip", "gemm_dw4.hip", "attention.hip", "attention_mfma.hip", "attention_qkv.hip", "gru.hip", "mixer.hip", "replay.hip", "collective.hip", "learner.hip", "profile.hip"]
+SOURCES = ["gemm.hip", "gemm_wres.hip", "gemm_dw.hip", "gemm_dw4.hip", "attention.hip", "attention_mfma.hip", "attention_qkv.hip", "gru.hip", "linrec.hip", "norm_gate.hip", "gated_ff.hip", "mixer.hip", "replay.hip", "collective.hip", "learner.hip", "profile.hip"]
 LIB = os.path.join(HERE, "librefil_hip.so")
 # Packed fp32 arithmetic (v_pk_add / mul / fma_f32) stays off: the compiler forms it from ordinary float code, and some of its forms have
 # given wrong results on this hardware now and then. Same IEEE operations, one lane at a time. (hipcc's host pass does not know the

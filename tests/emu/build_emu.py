@@ -1,12 +1,13 @@
 """TEST INFRASTRUCTURE: builds tests/emu/_build/librefil_emu.so -- the kernel SOURCES of refil_amd/csrc compiled as x86 C++ against the
 CPU wavefront emulator (include/hip/hip_runtime.h, emu_rt.cpp). Used by the `-m "not gpu"` emulator tests only; the product never loads it.
 
-The sources are compiled as they are except for four mechanical rewrites done on a scratch copy (the files under refil_amd/csrc are
+The sources are compiled as they are except for five mechanical rewrites done on a scratch copy (the files under refil_amd/csrc are
 not touched):
   * `extern __shared__ <attrs> T name[];`   -> `T* const name = static_cast<T*>(emu::dyn_smem());`   (dynamic LDS)
   * the gfx950 inline-asm statements, by template: empty / s_nop -> nothing (they are register-allocation and hazard hints),
     v_add_f32 / v_sub_f32 -> the C expression, `s_waitcnt lgkmcnt(0); s_barrier` -> the workgroup barrier. An unknown template is an error.
   * `#include "../../include/refil_hip.h"`  -> the absolute path (the scratch copy lives elsewhere).
+  * `__attribute__((address_space(n)))` is dropped (one address space on the host)
   * `#pragma unroll` lines are dropped (host compile time; no semantic content).
 """
 import os
@@ -142,6 +143,7 @@ def transform(text, name):
     text = out + text[i:]
     # forced unrolling only costs host compile time (minutes for the heavily instantiated GEMM files): the loops stay loops here
     text = re.sub(r"^[ \t]*#pragma unroll.*$", "", text, flags=re.M)
+    text = re.sub(r"__attribute__\(\(address_space\(\d\)\)\)", "", text)
     text = text.replace('#include "../../include/refil_hip.h"', f'#include "{os.path.join(ROOT, "include", "refil_hip.h")}"')
     return text
 

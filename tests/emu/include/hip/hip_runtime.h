@@ -252,6 +252,30 @@ __attribute__((always_inline)) static inline v4f mfma_4x4x1f32(float a, float b,
     }
     return c;
 }
+typedef _Float16 v8h __attribute__((ext_vector_type(8)));
+// v_mfma_f32_16x16x32_f16: the lane layout of the bf16 form
+__attribute__((always_inline)) static inline v4f mfma_16x16x32_f16(v8h a, v8h b, v4f c, int, int, int) {
+    unsigned char ab[32];
+    memcpy(ab, &a, 16); memcpy(ab + 16, &b, 16);
+    const Xchg e = xchg(ab, 32);
+    const int l = lane_ids().lane, j = l & 15;
+    for (int r = 0; r < 4; ++r) {
+        const int i = 4 * (l >> 4) + r;
+        double acc = 0.0;
+        for (int g = 0; g < 4; ++g)
+            for (int x = 0; x < 8; ++x) {
+                _Float16 p, q;
+                memcpy(&p, e.tab + XS * (16 * g + i) + 2 * x, 2); memcpy(&q, e.tab + XS * (16 * g + j) + 16 + 2 * x, 2);
+                acc += (double)p * (double)q;
+            }
+        c[r] = (float)((double)c[r] + acc);
+    }
+    return c;
+}
+// global_load_lds_dwordx4: lane l's 16 bytes land at (wave-uniform base) + 16 l. (Immediate here: the wait in front of the read is not modelled.)
+static inline void global_load_lds(const void* g, void* lds, int bytes, int off, int) {
+    memcpy(static_cast<char*>(lds) + off + bytes * lane_ids().lane, g, bytes);
+}
 static inline float bf(const unsigned char* p, int e) {
     unsigned short h; memcpy(&h, p + 2 * e, 2);
     return __uint_as_float((unsigned)h << 16);
@@ -330,6 +354,8 @@ static inline void raw_buffer_store_b128(V v, rsrc rs, int voff, int soff, int) 
 #define __builtin_amdgcn_mfma_f32_4x4x1f32 emu::mfma_4x4x1f32
 #define __builtin_amdgcn_mfma_f32_16x16x32_bf16 emu::mfma_16x16x32_bf16
 #define __builtin_amdgcn_mfma_f32_32x32x16_bf16 emu::mfma_32x32x16_bf16
+#define __builtin_amdgcn_mfma_f32_16x16x32_f16 emu::mfma_16x16x32_f16
+#define __builtin_amdgcn_global_load_lds emu::global_load_lds
 #define __builtin_amdgcn_readfirstlane emu::readfirstlane
 #define __builtin_amdgcn_readlane emu::readlane
 #define __builtin_amdgcn_update_dpp emu::update_dpp
