@@ -32,21 +32,19 @@ __host__ __device__ constexpr int gf_pair_b(int p) { return p == 0 ? 0 : p == 1 
 // ---- activation ----
 // gelu(v) = v/2 (1 + tanh(A (v + B v^3)))
 constexpr float GF_A = 0.797884560802865f, GF_B = 0.044715f;
-template <class T>
 __device__ __forceinline__ float gf_act(int act, float v) {
-    if (act == REFIL_ACT_SILU) return v * sigmoid_t<T>(v);
+    if (act == REFIL_ACT_SILU) return v * fast_sigmoid(v);
     // 1 + tanh(z) = 2 sigmoid(2 z): no cancellation on the negative side
-    return v * sigmoid_t<T>(2.f * GF_A * (v + GF_B * v * v * v));
+    return v * fast_sigmoid(2.f * GF_A * (v + GF_B * v * v * v));
 }
 // value and derivative
-template <class T>
 __device__ __forceinline__ void gf_act_grad(int act, float v, float& f, float& df) {
     if (act == REFIL_ACT_SILU) {
-        const float s = sigmoid_t<T>(v);
+        const float s = fast_sigmoid(v);
         f = v * s;
         df = s * (1.f + v * (1.f - s));
     } else {
-        const float s = sigmoid_t<T>(2.f * GF_A * (v + GF_B * v * v * v));
+        const float s = fast_sigmoid(2.f * GF_A * (v + GF_B * v * v * v));
         f = v * s;
         df = s + v * s * (1.f - s) * (2.f * GF_A) * (1.f + 3.f * GF_B * v * v);
     }
@@ -167,7 +165,7 @@ __global__ void __launch_bounds__(WM * WN * 64) gf_gemm(const GfGemm k) {
                     g[r] = acc[i][j][r]; u[r] = acc[i][j + NT / 2][r];
                     if (k.bias0 && n + r < k.N) g[r] += to_f32(((const T*)k.bias0)[n + r]);
                     if (k.bias1 && n + r < k.N) u[r] += to_f32(((const T*)k.bias1)[n + r]);
-                    h[r] = gf_act<T>(k.act, g[r]) * u[r];
+                    h[r] = gf_act(k.act, g[r]) * u[r];
                 }
                 T* c = (T*)k.C0 + (long)m * k.ldc + n;
 #pragma unroll
@@ -270,7 +268,7 @@ __global__ void __launch_bounds__(256) gf_grad(const GfGrad k) {
         if (r < k.N && c < k.F) {
             const float g = to_f32(((const T*)k.sg)[r * k.F + c]), u = to_f32(((const T*)k.su)[r * k.F + c]), d = to_f32(((const T*)k.dh)[r * k.dh_s + c]);
             float f, df;
-            gf_act_grad<T>(k.act, g, f, df);
+            gf_act_grad(k.act, g, f, df);
             dg = d * u * df; du = d * f;
         }
         t[0][i * 4 + q][l] = dg; t[1][i * 4 + q][l] = du;

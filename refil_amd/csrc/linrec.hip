@@ -14,6 +14,8 @@
 // The gate gradients come without a division by sqrt(1 - a^2):
 //   q_t = d loss / d log L_t = g_t (sigmoid(gi) x a^2 L / sqrt(1 - a^2) - a h_{t-1} L),   L / sqrt(1 - a^2) -> sqrt(L / 2) -> 0
 //   dga_t = q_t (1 - sigmoid(ga)),   ddecay = sum q_t sigmoid(decay) / softplus(decay)
+#include <type_traits>
+
 #include "kernels.h"
 #include "profile.h"
 #include "vecio.h"
@@ -31,34 +33,24 @@ struct LinrecK {
     float* sumA; float* sumH;          // [B][nchunk][C]: the maps of whole chunks (A = -1: the chunk holds a reset)
 };
 
-constexpr int LR_CH = 64;              // channels of a workgroup
-constexpr int LR_TT = 64;              // steps of a tile = 4 waves x TW time-threads x S steps
-constexpr int LR_WAVES = 4;
+constexpr int LR_CH = 64;              // channels of a workgroup: 16 lanes x 4
+constexpr int LR_V = 4, LR_TC = LR_CH / LR_V, LR_TW = 64 / LR_TC, LR_S = 4, LR_WAVES = 4;
+constexpr int LR_TT = LR_WAVES * LR_TW * LR_S;         // 64 steps of a tile
 
-template <class T> struct LrGeo {
-    static constexpr int VEC = VEC_OF<T>, TC = LR_CH / VEC, TW = 64 / TC, S = LR_TT / (LR_WAVES * TW);
-};
-
-// 1 - exp(-z), z >= 0, given e = exp(-z): the difference loses digits below z = 1/4, the series does not (next term z^8 / 40320)
-__device__ __forceinline__ float one_minus_exp(float z, float e) {
-    float p = fmaf(z, 1.98412698e-4f, -1.38888889e-3f);
-    p = fmaf(z, p, 8.33333333e-3f);
-    p = fmaf(z, p, -4.16666667e-2f);
-    p = fmaf(z, p, 1.66666667e-1f);
-    p = fmaf(z, p, -0.5f);
-    p = fmaf(z, p, 1.0f);
-    return z < 0.25f ? z * p : 1.0f - e;
-}
 __device__ __forceinline__ float softplus_(float v) { return fmaxf(v, 0.f) + log1pf(expf(-fabsf(v))); }
 
 struct LrGate { float sa, si, L, a, beta, lob; };      // lob = L / sqrt(1 - a^2)
-template <class T>
+// 1 - a^2 = 1 - exp(-2L) = 2 a sinh(L): below L = 0.35 by sinh's series (next term L^9 / 362880: 6e-10 of it), where the difference would
+// lose digits. WIDE = false: no channel's L reaches 0.35.
+template <bool WIDE>
 __device__ __forceinline__ LrGate lr_gate(float ga, float gi, float rate) {
     LrGate g;
-    g.sa = sigmoid_t<T>(ga); g.si = sigmoid_t<T>(gi);
+    g.sa = fast_sigmoid(ga); g.si = fast_sigmoid(gi);
     g.L = rate * g.sa;
-    g.a = exp_t<T>(-g.L);
-    const float om = one_minus_exp(2.f * g.L, g.a * g.a);
+    g.a = fast_exp(-g.L);
+    const float q = g.L * g.L;
+    float om = (g.a * (g.L + g.L)) * fmaf(q, fmaf(q, fmaf(q, 1.98412698e-4f, 8.33333333e-3f), 1.66666667e-1f), 1.0f);
+    if (WIDE) om = g.L < 0.35f ? om : fmaf(-g.a, g.a, 1.0f);
     const float rs = __builtin_amdgcn_rsqf(fmaxf(om, 1e-37f));
     g.beta = om * rs;
     g.lob = g.L * rs;
@@ -74,106 +66,133 @@ __device__ __forceinline__ void lr_rates(const LinrecK& k, int ch0, float* s_rat
     __syncthreads();
 }
 
-// BWD = false: the maps' H from x; true: R from dy. One workgroup per (episode, 64 channels, chunk): the chunk's whole map.
-// FINAL: also write the outputs, starting from the carry of the chunks in front (behind).
-template <class T, bool FINAL>
+// the reset flags of S steps
+template <bool RST>
+__device__ __forceinline__ int lr_cuts(const LinrecK& k, int b, int t0, int Tb) {
+    int cuts = 0;
+    if (RST) {
+        const uint8_t* r = k.reset + (long)b * k.rs_sB + (long)t0 * k.rs_sT;
+#pragma unroll
+        for (int s = 0; s < LR_S; ++s) {
+            if (t0 + s < Tb && *r) cuts |= 1 << s;
+            r += k.rs_sT;
+        }
+    }
+    return cuts;
+}
+template <class T>
+__device__ __forceinline__ void lr_load(Raw<T, LR_V> (&r)[LR_S], const T* base, long sT, int t0, int Tb, int nv, unsigned absent = 0u) {
+    const T* p = base + (long)t0 * sT;
+#pragma unroll
+    for (int s = 0; s < LR_S; ++s) { r[s] = ld_raw<T, LR_V>(p, t0 + s < Tb ? nv : 0, absent); p += sT; }
+}
+
+// One workgroup per (episode, 64 channels, chunk of the time axis). FINAL: the outputs, starting from the carry of the chunks in front;
+// else the chunk's whole map only. Steps past the episode's end are not loaded: their decay gate is -inf (a = 1, no input), the state
+// stays. A wave whose steps all lie there skips the arithmetic.
+template <class T, bool FINAL, bool RST>
 __global__ void __launch_bounds__(256) linrec_fwd(const LinrecK k) {
-    using G = LrGeo<T>;
-    constexpr int VEC = G::VEC, TC = G::TC, TW = G::TW, S = G::S;
+    constexpr int V = LR_V, TC = LR_TC, TW = LR_TW, S = LR_S;
     __shared__ float s_rate[LR_CH];
     __shared__ float sA[2][LR_WAVES][LR_CH], sH[2][LR_WAVES][LR_CH];
     __shared__ int sCut[2][LR_WAVES];
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
     const int b = (int)(blockIdx.x / k.ncol), ch0 = (int)(blockIdx.x % k.ncol) * LR_CH, chunk = blockIdx.y;
-    const int cl = (lane % TC) * VEC, c0 = ch0 + cl, nv = min(max(k.C - c0, 0), VEC);
+    const int cl = (lane % TC) * V, c0 = ch0 + cl, nv = min(max(k.C - c0, 0), V);
     const int tw = lane / TC;
     lr_rates(k, ch0, s_rate);
-    float rate[VEC];
+    float rate[V], top = 0.f;
 #pragma unroll
-    for (int i = 0; i < VEC; ++i) rate[i] = s_rate[cl + i];
+    for (int i = 0; i < V; ++i) { rate[i] = s_rate[cl + i]; top = fmaxf(top, rate[i]); }
+    const bool wide = __any(!(top < 0.35f));
     const int Tb = k.lengths ? min(max(k.lengths[b], 0), k.T) : k.T;
-    float carry[VEC];
+    float carry[V];
 #pragma unroll
-    for (int i = 0; i < VEC; ++i) carry[i] = FINAL && k.h0 && i < nv ? k.h0[(long)b * k.C + c0 + i] : 0.f;
+    for (int i = 0; i < V; ++i) carry[i] = FINAL && k.h0 && i < nv ? k.h0[(long)b * k.C + c0 + i] : 0.f;
     if (FINAL) {
         for (int j = 0; j < chunk; ++j) {
             const long o = ((long)b * k.nchunk + j) * k.C + c0;
 #pragma unroll
-            for (int i = 0; i < VEC; ++i)
+            for (int i = 0; i < V; ++i)
                 if (i < nv) { const float A = k.sumA[o + i], H = k.sumH[o + i]; carry[i] = A < 0.f ? H : fmaf(A, carry[i], H); }
         }
     }
-    float cA[VEC]; int ccut = 0;       // !FINAL: the chunk's map so far (its H is `carry`, started from zero)
+    float cA[V]; int ccut = 0;       // !FINAL: the chunk's map so far (its H is `carry`, started from zero)
 #pragma unroll
-    for (int i = 0; i < VEC; ++i) cA[i] = 1.f;
+    for (int i = 0; i < V; ++i) cA[i] = 1.f;
     const T* xb = (const T*)k.x + (long)b * k.x_sB + c0;
     const T* gab = (const T*)k.ga + (long)b * k.ga_sB + c0;
     const T* gib = (const T*)k.gi + (long)b * k.gi_sB + c0;
     const int tile0 = chunk * k.tiles_per_chunk, tile1 = min(tile0 + k.tiles_per_chunk, k.ntile);
     for (int tile = tile0; tile < tile1; ++tile) {
-        const int p = tile & 1, t0 = tile * LR_TT + (wave * TW + tw) * S;
-        float a[S][VEC], u[S][VEC], A[VEC], H[VEC];
-        bool cut[S]; int anycut = 0;
-        Raw rx[S], rga[S], rgi[S];
+        const int p = tile & 1, tw0 = tile * LR_TT + wave * (TW * S), t0 = tw0 + tw * S;
+        const bool any_live = tw0 < Tb;                                   // (wave-uniform)
+        float a[S][V], u[S][V], A[V], H[V], eA[V], eH[V];
+        int cuts = 0, cut = 0, ecut = 0;
 #pragma unroll
-        for (int s = 0; s < S; ++s) {
-            const long t = t0 + s;
-            const int n = t < Tb ? nv : 0;
-            rx[s] = ld_raw<T>(xb + t * k.x_sT, n); rga[s] = ld_raw<T>(gab + t * k.ga_sT, n); rgi[s] = ld_raw<T>(gib + t * k.gi_sT, n);
-            cut[s] = k.reset && t < Tb && k.reset[(long)b * k.rs_sB + t * k.rs_sT] != 0;
-            anycut |= (int)cut[s];
-        }
+        for (int i = 0; i < V; ++i) { A[i] = 1.f; H[i] = 0.f; eA[i] = 1.f; eH[i] = 0.f; }
+        if (any_live) {
+            Raw<T, V> rx[S], rga[S], rgi[S];
+            lr_load<T>(rga, gab, k.ga_sT, t0, Tb, nv, NEG_INF_WORD<T>);
+            lr_load<T>(rgi, gib, k.gi_sT, t0, Tb, nv);
+            lr_load<T>(rx, xb, k.x_sT, t0, Tb, nv);
+            cuts = lr_cuts<RST>(k, b, t0, Tb);
+            cut = cuts != 0;
+            auto gates = [&](auto w) {
 #pragma unroll
-        for (int i = 0; i < VEC; ++i) { A[i] = 1.f; H[i] = 0.f; }
+                for (int s = 0; s < S; ++s)
 #pragma unroll
-        for (int s = 0; s < S; ++s) {
-            const bool live = t0 + s < Tb;
+                    for (int i = 0; i < V; ++i) {
+                        const LrGate g = lr_gate<decltype(w)::value>(raw_get(rga[s], i), raw_get(rgi[s], i), rate[i]);
+                        a[s][i] = g.a;
+                        u[s][i] = g.beta * (g.si * raw_get(rx[s], i));
+                    }
+            };
+            if (wide) gates(std::true_type{}); else gates(std::false_type{});
 #pragma unroll
-            for (int i = 0; i < VEC; ++i) {
-                const LrGate g = lr_gate<T>(raw_get<T>(rga[s], i), raw_get<T>(rgi[s], i), rate[i]);
-                a[s][i] = live ? g.a : 1.f;                       // past the end the state stays as it is
-                u[s][i] = live ? g.beta * g.si * raw_get<T>(rx[s], i) : 0.f;
-                H[i] = cut[s] ? u[s][i] : fmaf(a[s][i], H[i], u[s][i]);
-                A[i] *= a[s][i];
+            for (int s = 0; s < S; ++s)
+#pragma unroll
+                for (int i = 0; i < V; ++i) {
+                    H[i] = RST && (cuts >> s & 1) ? u[s][i] : fmaf(a[s][i], H[i], u[s][i]);
+                    A[i] *= a[s][i];
+                }
+            // inclusive over the wave's time-threads, then exclusive
+#pragma unroll
+            for (int d = 1; d < TW; d *= 2) {
+                const int pc = RST ? __shfl_up(cut, d * TC) : 0;
+#pragma unroll
+                for (int i = 0; i < V; ++i) {
+                    const float pA = __shfl_up(A[i], d * TC), pH = __shfl_up(H[i], d * TC);
+                    if (tw >= d) { H[i] = RST && cut ? H[i] : fmaf(A[i], pH, H[i]); A[i] *= pA; }
+                }
+                if (tw >= d) cut |= pc;
             }
-        }
-        // inclusive over the wave's time-threads, then exclusive
+            if (RST) ecut = __shfl_up(cut, TC);
 #pragma unroll
-        for (int d = 1; d < TW; d *= 2) {
-            const int pc = __shfl_up(anycut, d * TC);
-#pragma unroll
-            for (int i = 0; i < VEC; ++i) {
-                const float pA = __shfl_up(A[i], d * TC), pH = __shfl_up(H[i], d * TC);
-                if (tw >= d) { H[i] = anycut ? H[i] : fmaf(A[i], pH, H[i]); A[i] *= pA; }
+            for (int i = 0; i < V; ++i) {
+                const float pA = __shfl_up(A[i], TC), pH = __shfl_up(H[i], TC);
+                eA[i] = tw ? pA : 1.f; eH[i] = tw ? pH : 0.f;
             }
-            if (tw >= d) anycut |= pc;
+            if (tw == 0) ecut = 0;
         }
         if (tw == TW - 1) {
 #pragma unroll
-            for (int i = 0; i < VEC; ++i) { sA[p][wave][cl + i] = A[i]; sH[p][wave][cl + i] = H[i]; }
-            if (lane % TC == 0) sCut[p][wave] = anycut;
-        }
-        float eA[VEC], eH[VEC]; int ecut = __shfl_up(anycut, TC);
-#pragma unroll
-        for (int i = 0; i < VEC; ++i) { eA[i] = __shfl_up(A[i], TC); eH[i] = __shfl_up(H[i], TC); }
-        if (tw == 0) {
-            ecut = 0;
-#pragma unroll
-            for (int i = 0; i < VEC; ++i) { eA[i] = 1.f; eH[i] = 0.f; }
+            for (int i = 0; i < V; ++i) { sA[p][wave][cl + i] = A[i]; sH[p][wave][cl + i] = H[i]; }
+            if (RST && lane % TC == 0) sCut[p][wave] = cut;
         }
         lds_barrier();
-        float h[VEC];
+        float h[V];
         if (FINAL && k.saved && wave == 0 && tw == 0) {
             float* o = k.saved + ((long)b * k.ntile + tile) * k.C + c0;
 #pragma unroll
-            for (int i = 0; i < VEC; ++i)
+            for (int i = 0; i < V; ++i)
                 if (i < nv) o[i] = carry[i];
         }
 #pragma unroll
         for (int w = 0; w < LR_WAVES; ++w) {
-            const int wc = sCut[p][w];
+            const int wc = RST ? sCut[p][w] : 0;
 #pragma unroll
-            for (int i = 0; i < VEC; ++i) {
+            for (int i = 0; i < V; ++i) {
                 if (w == wave) h[i] = carry[i];
                 const float wA = sA[p][w][cl + i], wH = sH[p][w][cl + i];
                 carry[i] = wc ? wH : fmaf(wA, carry[i], wH);
@@ -181,19 +200,23 @@ __global__ void __launch_bounds__(256) linrec_fwd(const LinrecK k) {
             }
             ccut |= wc;
         }
-        if (FINAL) {
+        if (FINAL && tw0 < k.T) {
+            T* yp = (T*)k.y + (long)b * k.y_sB + (long)t0 * k.y_sT + c0;
+            if (any_live) {
 #pragma unroll
-            for (int i = 0; i < VEC; ++i) h[i] = ecut ? eH[i] : fmaf(eA[i], h[i], eH[i]);
+                for (int i = 0; i < V; ++i) h[i] = ecut ? eH[i] : fmaf(eA[i], h[i], eH[i]);
+            }
 #pragma unroll
             for (int s = 0; s < S; ++s) {
-                const long t = t0 + s;
-                float o[VEC];
+                const int t = t0 + s;
+                float o[V];
 #pragma unroll
-                for (int i = 0; i < VEC; ++i) {
-                    h[i] = cut[s] ? u[s][i] : fmaf(a[s][i], h[i], u[s][i]);
+                for (int i = 0; i < V; ++i) {
+                    if (any_live) h[i] = RST && (cuts >> s & 1) ? u[s][i] : fmaf(a[s][i], h[i], u[s][i]);
                     o[i] = t < Tb ? h[i] : 0.f;
                 }
-                if (t < k.T) st_raw<T>((T*)k.y + (long)b * k.y_sB + t * k.y_sT + c0, raw_pack<T>(o), nv);
+                if (t < k.T) st_raw<T, V>(yp, raw_pack<T, V>(o), nv);
+                yp += k.y_sT;
             }
         }
     }
@@ -201,35 +224,36 @@ __global__ void __launch_bounds__(256) linrec_fwd(const LinrecK k) {
         if (!FINAL) {
             const long o = ((long)b * k.nchunk + chunk) * k.C + c0;
 #pragma unroll
-            for (int i = 0; i < VEC; ++i)
+            for (int i = 0; i < V; ++i)
                 if (i < nv) { k.sumA[o + i] = ccut ? -1.f : cA[i]; k.sumH[o + i] = carry[i]; }
         } else if (k.h_last && chunk == k.nchunk - 1) {
 #pragma unroll
-            for (int i = 0; i < VEC; ++i)
+            for (int i = 0; i < V; ++i)
                 if (i < nv) k.h_last[(long)b * k.C + c0 + i] = carry[i];
         }
     }
 }
 
-template <class T, bool FINAL>
+// the same cut of the time axis in reverse order
+template <class T, bool FINAL, bool RST>
 __global__ void __launch_bounds__(256) linrec_bwd(const LinrecK k) {
-    using G = LrGeo<T>;
-    constexpr int VEC = G::VEC, TC = G::TC, TW = G::TW, S = G::S;
+    constexpr int V = LR_V, TC = LR_TC, TW = LR_TW, S = LR_S;
     __shared__ float s_rate[LR_CH];
     __shared__ float sA[2][LR_WAVES][LR_CH], sH[2][LR_WAVES][LR_CH], sR[2][LR_WAVES][LR_CH];
     __shared__ int sCut[2][LR_WAVES];
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
     const int b = (int)(blockIdx.x / k.ncol), ch0 = (int)(blockIdx.x % k.ncol) * LR_CH, chunk = blockIdx.y;
-    const int cl = (lane % TC) * VEC, c0 = ch0 + cl, nv = min(max(k.C - c0, 0), VEC);
+    const int cl = (lane % TC) * V, c0 = ch0 + cl, nv = min(max(k.C - c0, 0), V);
     const int tw = lane / TC;
     lr_rates(k, ch0, s_rate);
-    float rate[VEC];
+    float rate[V], top = 0.f;
 #pragma unroll
-    for (int i = 0; i < VEC; ++i) rate[i] = s_rate[cl + i];
+    for (int i = 0; i < V; ++i) { rate[i] = s_rate[cl + i]; top = fmaxf(top, rate[i]); }
+    const bool wide = __any(!(top < 0.35f));
     const int Tb = k.lengths ? min(max(k.lengths[b], 0), k.T) : k.T;
-    float carry[VEC], cA[VEC], dl[VEC]; int ccut = 0;
+    float carry[V], cA[V], dl[V]; int ccut = 0;
 #pragma unroll
-    for (int i = 0; i < VEC; ++i) {
+    for (int i = 0; i < V; ++i) {
         carry[i] = FINAL && k.dh_last && i < nv ? k.dh_last[(long)b * k.C + c0 + i] : 0.f;
         cA[i] = 1.f; dl[i] = 0.f;
     }
@@ -237,7 +261,7 @@ __global__ void __launch_bounds__(256) linrec_bwd(const LinrecK k) {
         for (int j = k.nchunk - 1; j > chunk; --j) {
             const long o = ((long)b * k.nchunk + j) * k.C + c0;
 #pragma unroll
-            for (int i = 0; i < VEC; ++i)
+            for (int i = 0; i < V; ++i)
                 if (i < nv) { const float A = k.sumA[o + i], R = k.sumH[o + i]; carry[i] = A < 0.f ? R : fmaf(A, carry[i], R); }
         }
     }
@@ -247,100 +271,98 @@ __global__ void __launch_bounds__(256) linrec_bwd(const LinrecK k) {
     const T* dyb = (const T*)k.dy + (long)b * k.dy_sB + c0;
     const int tile0 = chunk * k.tiles_per_chunk, tile1 = min(tile0 + k.tiles_per_chunk, k.ntile);
     for (int tile = tile1 - 1; tile >= tile0; --tile) {
-        const int p = tile & 1, t0 = tile * LR_TT + (wave * TW + tw) * S;
-        Raw rx[S], rga[S], rgi[S], rdy[S];
-        bool cut[S]; int anycut = 0;
+        const int p = tile & 1, tw0 = tile * LR_TT + wave * (TW * S), t0 = tw0 + tw * S;
+        const bool any_live = tw0 < Tb;
+        Raw<T, V> rx[S], rdy[S];
+        float a[S][V], sa[S][V], si[S][V], beta[S][V], lob[S][V];
+        float A[V], H[V], R[V], B[V], eA[V], eH[V], xA[V], xR[V], hin[V];
+        int cuts = 0, fcut = 0, rcut = 0, ecut = 0, xcut = 0;
 #pragma unroll
-        for (int s = 0; s < S; ++s) {
-            const long t = t0 + s;
-            const int n = t < Tb ? nv : 0;
-            rga[s] = ld_raw<T>(gab + t * k.ga_sT, n); rdy[s] = ld_raw<T>(dyb + t * k.dy_sT, n);
-            if (FINAL) { rx[s] = ld_raw<T>(xb + t * k.x_sT, n); rgi[s] = ld_raw<T>(gib + t * k.gi_sT, n); }
-            cut[s] = k.reset && t < Tb && k.reset[(long)b * k.rs_sB + t * k.rs_sT] != 0;
-            anycut |= (int)cut[s];
-        }
-        float hin[VEC];
-        if (FINAL) {
-            const float* o = k.saved + ((long)b * k.ntile + tile) * k.C + c0;
+        for (int i = 0; i < V; ++i) { A[i] = B[i] = 1.f; H[i] = R[i] = 0.f; eA[i] = xA[i] = 1.f; eH[i] = xR[i] = 0.f; hin[i] = 0.f; }
+        if (any_live) {
+            Raw<T, V> rga[S], rgi[S];
+            lr_load<T>(rga, gab, k.ga_sT, t0, Tb, nv, NEG_INF_WORD<T>);
+            lr_load<T>(rdy, dyb, k.dy_sT, t0, Tb, nv);
+            if (FINAL) { lr_load<T>(rgi, gib, k.gi_sT, t0, Tb, nv); lr_load<T>(rx, xb, k.x_sT, t0, Tb, nv); }
+            cuts = lr_cuts<RST>(k, b, t0, Tb);
+            fcut = rcut = cuts != 0;
+            if (FINAL) {
+                const float* o = k.saved + ((long)b * k.ntile + tile) * k.C + c0;
 #pragma unroll
-            for (int i = 0; i < VEC; ++i) hin[i] = i < nv ? o[i] : 0.f;
-        }
-        LrGate g[S][VEC];
-        float A[VEC], H[VEC], R[VEC];
-#pragma unroll
-        for (int i = 0; i < VEC; ++i) { A[i] = 1.f; H[i] = 0.f; R[i] = 0.f; }
-#pragma unroll
-        for (int s = 0; s < S; ++s) {
-            const bool live = t0 + s < Tb;
-#pragma unroll
-            for (int i = 0; i < VEC; ++i) {
-                g[s][i] = lr_gate<T>(raw_get<T>(rga[s], i), FINAL ? raw_get<T>(rgi[s], i) : 0.f, rate[i]);
-                if (!live) { g[s][i].a = 1.f; g[s][i].beta = 0.f; }
-                if (FINAL) {
-                    const float u = g[s][i].beta * g[s][i].si * raw_get<T>(rx[s], i);
-                    H[i] = cut[s] ? u : fmaf(g[s][i].a, H[i], u);
-                }
-                A[i] *= g[s][i].a;
+                for (int i = 0; i < V; ++i) hin[i] = i < nv ? o[i] : 0.f;
             }
-        }
+            auto gates = [&](auto w) {
 #pragma unroll
-        for (int s = S - 1; s >= 0; --s)
+                for (int s = 0; s < S; ++s)
 #pragma unroll
-            for (int i = 0; i < VEC; ++i) R[i] = cut[s] ? 0.f : g[s][i].a * (raw_get<T>(rdy[s], i) + R[i]);
-        // forward: inclusive prefix of (A, H); backward: inclusive suffix of (B, R)
-        float Bq[VEC]; int fcut = anycut, rcut = anycut;
+                    for (int i = 0; i < V; ++i) {
+                        if (FINAL) {
+                            const LrGate g = lr_gate<decltype(w)::value>(raw_get(rga[s], i), raw_get(rgi[s], i), rate[i]);
+                            a[s][i] = g.a; sa[s][i] = g.sa; si[s][i] = g.si; beta[s][i] = g.beta; lob[s][i] = g.lob;
+                        } else a[s][i] = fast_exp(-rate[i] * fast_sigmoid(raw_get(rga[s], i)));
+                    }
+            };
+            if (FINAL && wide) gates(std::true_type{}); else gates(std::false_type{});
 #pragma unroll
-        for (int i = 0; i < VEC; ++i) Bq[i] = A[i];
+            for (int s = 0; s < S; ++s)
 #pragma unroll
-        for (int d = 1; d < TW; d *= 2) {
-            const int pc = __shfl_up(fcut, d * TC), nc = __shfl_down(rcut, d * TC);
-#pragma unroll
-            for (int i = 0; i < VEC; ++i) {
-                if (FINAL) {
-                    const float pA = __shfl_up(A[i], d * TC), pH = __shfl_up(H[i], d * TC);
-                    if (tw >= d) { H[i] = fcut ? H[i] : fmaf(A[i], pH, H[i]); A[i] *= pA; }
+                for (int i = 0; i < V; ++i) {
+                    if (FINAL) {
+                        const float u = beta[s][i] * (si[s][i] * raw_get(rx[s], i));
+                        H[i] = RST && (cuts >> s & 1) ? u : fmaf(a[s][i], H[i], u);
+                    }
+                    A[i] *= a[s][i];
                 }
-                const float nA = __shfl_down(Bq[i], d * TC), nR = __shfl_down(R[i], d * TC);
-                if (tw + d < TW) { R[i] = rcut ? R[i] : fmaf(Bq[i], nR, R[i]); Bq[i] *= nA; }
+#pragma unroll
+            for (int s = S - 1; s >= 0; --s)
+#pragma unroll
+                for (int i = 0; i < V; ++i) R[i] = RST && (cuts >> s & 1) ? 0.f : a[s][i] * (raw_get(rdy[s], i) + R[i]);
+            // forward: inclusive prefix of (A, H); backward: inclusive suffix of (B, R)
+#pragma unroll
+            for (int i = 0; i < V; ++i) B[i] = A[i];
+#pragma unroll
+            for (int d = 1; d < TW; d *= 2) {
+                const int pc = RST ? __shfl_up(fcut, d * TC) : 0, nc = RST ? __shfl_down(rcut, d * TC) : 0;
+#pragma unroll
+                for (int i = 0; i < V; ++i) {
+                    if (FINAL) {
+                        const float pA = __shfl_up(A[i], d * TC), pH = __shfl_up(H[i], d * TC);
+                        if (tw >= d) { H[i] = RST && fcut ? H[i] : fmaf(A[i], pH, H[i]); A[i] *= pA; }
+                    }
+                    const float nA = __shfl_down(B[i], d * TC), nR = __shfl_down(R[i], d * TC);
+                    if (tw + d < TW) { R[i] = RST && rcut ? R[i] : fmaf(B[i], nR, R[i]); B[i] *= nA; }
+                }
+                if (tw >= d) fcut |= pc;
+                if (tw + d < TW) rcut |= nc;
             }
-            if (tw >= d) fcut |= pc;
-            if (tw + d < TW) rcut |= nc;
+            if (FINAL) {
+                if (RST) { ecut = __shfl_up(fcut, TC); xcut = __shfl_down(rcut, TC); }
+#pragma unroll
+                for (int i = 0; i < V; ++i) {
+                    const float pA = __shfl_up(A[i], TC), pH = __shfl_up(H[i], TC), nA = __shfl_down(B[i], TC), nR = __shfl_down(R[i], TC);
+                    eA[i] = tw ? pA : 1.f; eH[i] = tw ? pH : 0.f;
+                    xA[i] = tw < TW - 1 ? nA : 1.f; xR[i] = tw < TW - 1 ? nR : 0.f;
+                }
+                if (tw == 0) ecut = 0;
+                if (tw == TW - 1) xcut = 0;
+            }
         }
         if (tw == 0) {
 #pragma unroll
-            for (int i = 0; i < VEC; ++i) { sA[p][wave][cl + i] = Bq[i]; sR[p][wave][cl + i] = R[i]; }
-            if (lane % TC == 0) sCut[p][wave] = rcut;
+            for (int i = 0; i < V; ++i) { sA[p][wave][cl + i] = B[i]; sR[p][wave][cl + i] = R[i]; }
+            if (RST && lane % TC == 0) sCut[p][wave] = rcut;
         }
         if (FINAL && tw == TW - 1) {
 #pragma unroll
-            for (int i = 0; i < VEC; ++i) sH[p][wave][cl + i] = H[i];
-        }
-        float eA[VEC], eH[VEC], xA[VEC], xR[VEC]; int ecut, xcut;
-        if (FINAL) {
-            ecut = __shfl_up(fcut, TC); xcut = __shfl_down(rcut, TC);
-#pragma unroll
-            for (int i = 0; i < VEC; ++i) {
-                eA[i] = __shfl_up(A[i], TC); eH[i] = __shfl_up(H[i], TC);
-                xA[i] = __shfl_down(Bq[i], TC); xR[i] = __shfl_down(R[i], TC);
-            }
-            if (tw == 0) {
-                ecut = 0;
-#pragma unroll
-                for (int i = 0; i < VEC; ++i) { eA[i] = 1.f; eH[i] = 0.f; }
-            }
-            if (tw == TW - 1) {
-                xcut = 0;
-#pragma unroll
-                for (int i = 0; i < VEC; ++i) { xA[i] = 1.f; xR[i] = 0.f; }
-            }
+            for (int i = 0; i < V; ++i) sH[p][wave][cl + i] = H[i];
         }
         lds_barrier();
-        float c[VEC];
+        float c[V];
 #pragma unroll
         for (int w = LR_WAVES - 1; w >= 0; --w) {
-            const int wc = sCut[p][w];
+            const int wc = RST ? sCut[p][w] : 0;
 #pragma unroll
-            for (int i = 0; i < VEC; ++i) {
+            for (int i = 0; i < V; ++i) {
                 if (w == wave) c[i] = carry[i];
                 const float wA = sA[p][w][cl + i], wR = sR[p][w][cl + i];
                 carry[i] = wc ? wR : fmaf(wA, carry[i], wR);
@@ -348,52 +370,67 @@ __global__ void __launch_bounds__(256) linrec_bwd(const LinrecK k) {
             }
             ccut |= wc;
         }
-        if (FINAL) {
+        if (FINAL && tw0 < k.T) {
+            const long o = (long)b * k.d_sB + (long)t0 * k.d_sT + c0;
+            T* xp = (T*)k.dx + o; T* ap = (T*)k.dga + o; T* ip = (T*)k.dgi + o;
+            if (any_live) {
 #pragma unroll
-            for (int w = 0; w < LR_WAVES - 1; ++w) {
-                if (w < wave) {
-                    const int wc = sCut[p][w];
+                for (int w = 0; w < LR_WAVES - 1; ++w) {
+                    if (w < wave) {
+                        const int wc = RST ? sCut[p][w] : 0;
 #pragma unroll
-                    for (int i = 0; i < VEC; ++i) hin[i] = wc ? sH[p][w][cl + i] : fmaf(sA[p][w][cl + i], hin[i], sH[p][w][cl + i]);
+                        for (int i = 0; i < V; ++i) hin[i] = wc ? sH[p][w][cl + i] : fmaf(sA[p][w][cl + i], hin[i], sH[p][w][cl + i]);
+                    }
                 }
-            }
-            float hp[S][VEC];
+                float hp[S][V];
 #pragma unroll
-            for (int i = 0; i < VEC; ++i) {
-                hin[i] = ecut ? eH[i] : fmaf(eA[i], hin[i], eH[i]);
-                c[i] = xcut ? xR[i] : fmaf(xA[i], c[i], xR[i]);
-            }
-#pragma unroll
-            for (int s = 0; s < S; ++s)
-#pragma unroll
-                for (int i = 0; i < VEC; ++i) {
-                    hp[s][i] = hin[i];
-                    const float u = g[s][i].beta * g[s][i].si * raw_get<T>(rx[s], i);
-                    hin[i] = cut[s] ? u : fmaf(g[s][i].a, hin[i], u);
+                for (int i = 0; i < V; ++i) {
+                    hin[i] = ecut ? eH[i] : fmaf(eA[i], hin[i], eH[i]);
+                    c[i] = xcut ? xR[i] : fmaf(xA[i], c[i], xR[i]);
                 }
 #pragma unroll
-            for (int s = S - 1; s >= 0; --s) {
-                const long t = t0 + s;
-                const bool live = t < Tb;
-                float ox[VEC], oa[VEC], oi[VEC];
+                for (int s = 0; s < S; ++s)
 #pragma unroll
-                for (int i = 0; i < VEC; ++i) {
-                    const LrGate& e = g[s][i];
-                    const float gt = raw_get<T>(rdy[s], i) + c[i];
-                    const float sx = e.si * raw_get<T>(rx[s], i);
-                    const float through = cut[s] ? 0.f : e.a * hp[s][i] * e.L;
-                    const float q = gt * (sx * e.a * e.a * e.lob - through);
-                    ox[i] = live ? gt * e.beta * e.si : 0.f;
-                    oi[i] = live ? gt * e.beta * sx * (1.f - e.si) : 0.f;
-                    oa[i] = live ? q * (1.f - e.sa) : 0.f;
-                    dl[i] += live ? q : 0.f;
-                    c[i] = cut[s] ? 0.f : e.a * gt;
+                    for (int i = 0; i < V; ++i) {
+                        hp[s][i] = hin[i];
+                        const float u = beta[s][i] * (si[s][i] * raw_get(rx[s], i));
+                        hin[i] = RST && (cuts >> s & 1) ? u : fmaf(a[s][i], hin[i], u);
+                    }
+                xp += (S - 1) * k.d_sT; ap += (S - 1) * k.d_sT; ip += (S - 1) * k.d_sT;
+#pragma unroll
+                for (int s = S - 1; s >= 0; --s) {
+                    const int t = t0 + s;
+                    const bool live = t < Tb;
+                    float ox[V], oa[V], oi[V];
+#pragma unroll
+                    for (int i = 0; i < V; ++i) {
+                        const float x = raw_get(rx[s], i), gt = raw_get(rdy[s], i) + c[i];
+                        const float sx = si[s][i] * x, L = rate[i] * sa[s][i];
+                        const float through = RST && (cuts >> s & 1) ? 0.f : hp[s][i] * L;
+                        const float q = live ? (gt * a[s][i]) * (sx * (a[s][i] * lob[s][i]) - through) : 0.f;
+                        ox[i] = live ? gt * (beta[s][i] * si[s][i]) : 0.f;
+                        oi[i] = ox[i] * (x - sx);
+                        oa[i] = fmaf(-q, sa[s][i], q);
+                        dl[i] += q;
+                        c[i] = RST && (cuts >> s & 1) ? 0.f : a[s][i] * gt;
+                    }
+                    if (t < k.T) {
+                        st_raw<T, V>(xp, raw_pack<T, V>(ox), nv);
+                        st_raw<T, V>(ap, raw_pack<T, V>(oa), nv);
+                        st_raw<T, V>(ip, raw_pack<T, V>(oi), nv);
+                    }
+                    xp -= k.d_sT; ap -= k.d_sT; ip -= k.d_sT;
                 }
-                if (t < k.T) {
-                    const long o = (long)b * k.d_sB + t * k.d_sT + c0;
-                    st_raw<T>((T*)k.dx + o, raw_pack<T>(ox), nv);
-                    st_raw<T>((T*)k.dga + o, raw_pack<T>(oa), nv);
-                    st_raw<T>((T*)k.dgi + o, raw_pack<T>(oi), nv);
+            } else {
+                const float zero[V] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+                for (int s = 0; s < S; ++s) {
+                    if (t0 + s < k.T) {
+                        st_raw<T, V>(xp, raw_pack<T, V>(zero), nv);
+                        st_raw<T, V>(ap, raw_pack<T, V>(zero), nv);
+                        st_raw<T, V>(ip, raw_pack<T, V>(zero), nv);
+                    }
+                    xp += k.d_sT; ap += k.d_sT; ip += k.d_sT;
                 }
             }
         }
@@ -402,25 +439,25 @@ __global__ void __launch_bounds__(256) linrec_bwd(const LinrecK k) {
         if (wave == 0 && tw == 0) {
             const long o = ((long)b * k.nchunk + chunk) * k.C + c0;
 #pragma unroll
-            for (int i = 0; i < VEC; ++i)
+            for (int i = 0; i < V; ++i)
                 if (i < nv) { k.sumA[o + i] = ccut ? -1.f : cA[i]; k.sumH[o + i] = carry[i]; }
         }
         return;
     }
     if (k.dh0 && chunk == 0 && wave == 0 && tw == 0) {
 #pragma unroll
-        for (int i = 0; i < VEC; ++i)
+        for (int i = 0; i < V; ++i)
             if (i < nv) k.dh0[(long)b * k.C + c0 + i] = carry[i];
     }
     // the decay gradient's partial sum of this workgroup: time-threads, then waves, in a fixed order
 #pragma unroll
-    for (int i = 0; i < VEC; ++i)
+    for (int i = 0; i < V; ++i)
 #pragma unroll
         for (int d = TC; d < 64; d *= 2) dl[i] += __shfl_xor(dl[i], d);
     __syncthreads();
     if (tw == 0) {
 #pragma unroll
-        for (int i = 0; i < VEC; ++i) sA[0][wave][cl + i] = dl[i];
+        for (int i = 0; i < V; ++i) sA[0][wave][cl + i] = dl[i];
     }
     __syncthreads();
     if (wave == 0 && ch0 + lane < k.C)
@@ -461,13 +498,13 @@ __global__ void __launch_bounds__(64) linrec_step(const LinrecStepK k) {
     }
     int r = row;
     for (;;) {
-        const Raw rx = ld_raw<T>((const T*)k.x + (long)r * k.x_sB + c0, nv);
-        const Raw ra = ld_raw<T>((const T*)k.ga + (long)r * k.ga_sB + c0, nv);
-        const Raw ri = ld_raw<T>((const T*)k.gi + (long)r * k.gi_sB + c0, nv);
+        const auto rx = ld_raw<T>((const T*)k.x + (long)r * k.x_sB + c0, nv);
+        const auto ra = ld_raw<T>((const T*)k.ga + (long)r * k.ga_sB + c0, nv);
+        const auto ri = ld_raw<T>((const T*)k.gi + (long)r * k.gi_sB + c0, nv);
 #pragma unroll
         for (int i = 0; i < VEC; ++i) {
-            const LrGate g = lr_gate<T>(raw_get<T>(ra, i), raw_get<T>(ri, i), rate[i]);
-            h[i] = fmaf(g.a, h[i], g.beta * g.si * raw_get<T>(rx, i));
+            const LrGate g = lr_gate<true>(raw_get(ra, i), raw_get(ri, i), rate[i]);
+            h[i] = fmaf(g.a, h[i], g.beta * (g.si * raw_get(rx, i)));
         }
         st_raw<T>(y + (long)r * k.y_sB + c0, raw_pack<T>(h), nv);
         if (!k.slots) break;
@@ -535,8 +572,14 @@ static LrPlan lr_plan(const refil_linrec_desc& d) {
     LrPlan p;
     p.ncol = cdiv(d.C, LR_CH);
     p.ntile = cdiv(d.T, LR_TT);
-    p.nchunk = 1;
-    p.tiles_per_chunk = p.ntile;
+    // Too few (episode, column) pairs to fill the card: the time axis is cut into chunks of whole tiles, at the price of reading the
+    // inputs once more for the chunks' maps.
+    const long wgs = (long)d.B * p.ncol, want = 1024;
+    long n = wgs > 0 && wgs < want / 2 ? cdivl(want, wgs) : 1;
+    if (n > p.ntile) n = p.ntile;
+    if (n > 256) n = 256;
+    p.tiles_per_chunk = n > 1 ? (int)cdivl(p.ntile, n) : p.ntile;
+    p.nchunk = n > 1 ? cdiv(p.ntile, p.tiles_per_chunk) : 1;
     return p;
 }
 static int lr_check(const refil_linrec_desc& d, const char* who) {
@@ -578,11 +621,13 @@ static int lr_forward(const refil_linrec_desc& d, hipStream_t st) {
     const double n = (double)d.B * d.T * d.C;
     if (p.nchunk > 1) {
         ProfScope ps("linrec_fwd<summary>", 20 * n, 3 * n * sizeof(T), st);
-        hipLaunchKernelGGL((linrec_fwd<T, false>), grid, dim3(256), 0, st, k);
+        if (k.reset) hipLaunchKernelGGL((linrec_fwd<T, false, true>), grid, dim3(256), 0, st, k);
+        else hipLaunchKernelGGL((linrec_fwd<T, false, false>), grid, dim3(256), 0, st, k);
         REFIL_LAUNCH_CHECK();
     }
     ProfScope ps("linrec_fwd", 25 * n, 4 * n * sizeof(T), st);
-    hipLaunchKernelGGL((linrec_fwd<T, true>), grid, dim3(256), 0, st, k);
+    if (k.reset) hipLaunchKernelGGL((linrec_fwd<T, true, true>), grid, dim3(256), 0, st, k);
+    else hipLaunchKernelGGL((linrec_fwd<T, true, false>), grid, dim3(256), 0, st, k);
     REFIL_LAUNCH_CHECK();
     return 0;
 }
@@ -598,12 +643,14 @@ static int lr_backward(const refil_linrec_desc& d, hipStream_t st) {
     const double n = (double)d.B * d.T * d.C;
     if (p.nchunk > 1) {
         ProfScope ps("linrec_bwd<summary>", 20 * n, 2 * n * sizeof(T), st);
-        hipLaunchKernelGGL((linrec_bwd<T, false>), grid, dim3(256), 0, st, k);
+        if (k.reset) hipLaunchKernelGGL((linrec_bwd<T, false, true>), grid, dim3(256), 0, st, k);
+        else hipLaunchKernelGGL((linrec_bwd<T, false, false>), grid, dim3(256), 0, st, k);
         REFIL_LAUNCH_CHECK();
     }
     {
         ProfScope ps("linrec_bwd", 55 * n, 7 * n * sizeof(T), st);
-        hipLaunchKernelGGL((linrec_bwd<T, true>), grid, dim3(256), 0, st, k);
+        if (k.reset) hipLaunchKernelGGL((linrec_bwd<T, true, true>), grid, dim3(256), 0, st, k);
+        else hipLaunchKernelGGL((linrec_bwd<T, true, false>), grid, dim3(256), 0, st, k);
         REFIL_LAUNCH_CHECK();
     }
     return colsum_launch(k.part, rows, d.D, k.part + rows * d.D, d.decay, d.ddecay, st);

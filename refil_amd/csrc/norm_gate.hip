@@ -80,7 +80,7 @@ __global__ void __launch_bounds__(TPR > 256 ? TPR : 256) norm_gate_kernel(const 
         // (every thread takes every round: the reductions hold workgroup barriers)
         const long r = (it * gridDim.x + blockIdx.x) * GROUPS + grp;
         const bool in = r < k.N, live = in && !(k.mask && k.mask[r]);
-        Raw rx[K], ro[K], rg[K], rdy[K], rdn[K];
+        Raw<T> rx[K], ro[K], rg[K], rdy[K], rdn[K];
 #pragma unroll
         for (int j = 0; j < K; ++j) {
             const int c0 = (j * TPR + col) * VEC, n = live ? nv[j] : 0;
@@ -98,7 +98,7 @@ __global__ void __launch_bounds__(TPR > 256 ? TPR : 256) norm_gate_kernel(const 
 #pragma unroll
             for (int j = 0; j < K; ++j)
 #pragma unroll
-                for (int i = 0; i < VEC; ++i) { const float v = raw_get<T>(ro[j], i); q = fmaf(v, v, q); }
+                for (int i = 0; i < VEC; ++i) { const float v = raw_get(ro[j], i); q = fmaf(v, v, q); }
             irms_o = __builtin_amdgcn_rsqf(fmaf(row_sum<TPR>(q, s_red), inv_d, k.eps));
         }
         float y[K][VEC], sg[K][VEC], q = 0.f, ey = 0.f;
@@ -106,11 +106,11 @@ __global__ void __launch_bounds__(TPR > 256 ? TPR : 256) norm_gate_kernel(const 
         for (int j = 0; j < K; ++j)
 #pragma unroll
             for (int i = 0; i < VEC; ++i) {
-                sg[j][i] = k.g ? sigmoid_t<T>(raw_get<T>(rg[j], i)) : 1.f;
-                const float v = sc[j][i] * sg[j][i] * (raw_get<T>(ro[j], i) * irms_o * wp[j][i]);
-                y[j][i] = fmaf(k.alpha, raw_get<T>(rx[j], i), v);
+                sg[j][i] = k.g ? fast_sigmoid(raw_get(rg[j], i)) : 1.f;
+                const float v = sc[j][i] * sg[j][i] * (raw_get(ro[j], i) * irms_o * wp[j][i]);
+                y[j][i] = fmaf(k.alpha, raw_get(rx[j], i), v);
                 q = fmaf(y[j][i], y[j][i], q);
-                if (BWD) ey = fmaf(raw_get<T>(rdn[j], i) * wq[j][i], y[j][i], ey);
+                if (BWD) ey = fmaf(raw_get(rdn[j], i) * wq[j][i], y[j][i], ey);
             }
         float irms_y = 0.f;
         if (BWD ? k.dn != nullptr : k.n != nullptr) irms_y = __builtin_amdgcn_rsqf(fmaf(row_sum<TPR>(q, s_red), inv_d, k.eps));
@@ -139,10 +139,10 @@ __global__ void __launch_bounds__(TPR > 256 ? TPR : 256) norm_gate_kernel(const 
             for (int j = 0; j < K; ++j)
 #pragma unroll
                 for (int i = 0; i < VEC; ++i) {
-                    const float yh = y[j][i] * irms_y, dn = raw_get<T>(rdn[j], i);
-                    const float d = raw_get<T>(rdy[j], i) + irms_y * (dn * wq[j][i] - yh * m);
+                    const float yh = y[j][i] * irms_y, dn = raw_get(rdn[j], i);
+                    const float d = raw_get(rdy[j], i) + irms_y * (dn * wq[j][i] - yh * m);
                     awq[j][i] = live ? fmaf(dn, yh, awq[j][i]) : awq[j][i];
-                    const float oh = raw_get<T>(ro[j], i) * irms_o, f = d * sc[j][i] * sg[j][i];
+                    const float oh = raw_get(ro[j], i) * irms_o, f = d * sc[j][i] * sg[j][i];
                     awp[j][i] = live ? fmaf(f, oh, awp[j][i]) : awp[j][i];
                     asc[j][i] = live ? fmaf(d * sg[j][i], oh * wp[j][i], asc[j][i]) : asc[j][i];
                     e2o = fmaf(f * wp[j][i], oh, e2o);
@@ -156,7 +156,7 @@ __global__ void __launch_bounds__(TPR > 256 ? TPR : 256) norm_gate_kernel(const 
                 float ox[VEC], oo[VEC], og[VEC];
 #pragma unroll
                 for (int i = 0; i < VEC; ++i) {
-                    const float d = y[j][i], oh = raw_get<T>(ro[j], i) * irms_o, f = d * sc[j][i] * sg[j][i];
+                    const float d = y[j][i], oh = raw_get(ro[j], i) * irms_o, f = d * sc[j][i] * sg[j][i];
                     ox[i] = live ? k.alpha * d : 0.f;
                     oo[i] = live ? irms_o * (f * wp[j][i] - oh * m2) : 0.f;
                     og[i] = live ? f * oh * wp[j][i] * (1.f - sg[j][i]) : 0.f;
