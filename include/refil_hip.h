@@ -479,7 +479,7 @@ enum { REFIL_F32 = 0, REFIL_BF16 = 1, REFIL_F16 = 2 };
  *   h0 [B,C] fp32 or NULL (zero); reset [B,T] uint8 or NULL: != 0 drops h_{t-1} (and h0) at that step, whatever it holds;
  *   lengths [B] int32 or NULL: episode b has min(max(lengths[b],0),T) steps -- later steps are not read, their y is written as 0 and so
  *   are their gradients, the state stays; h_last [B,C] fp32 or NULL: the state after the last step.
- *   saved: NULL, or refil_linrec_saved_floats floats that the backward needs (the state at every 64th step).
+ *   saved: NULL, or refil_linrec_saved_floats floats that the backward needs (the state at every tile's start).
  * Backward (x, ga, gi, decay, h0, reset, lengths as in the forward, saved from it): dy [B,T,C], dh_last [B,C] or NULL ->
  *   dx, dga, dgi (strides d_sB, d_sT), ddecay [D] (sum over everything that shares it), dh0 [B,C] or NULL. Deterministic. */
 typedef struct refil_linrec_desc {

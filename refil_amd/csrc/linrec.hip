@@ -10,10 +10,12 @@
 //
 // Backward: with g_t the whole gradient of h_t, g_t = dy_t + c_t and c_{t-1} = a_t g_t [no reset at t] -- the same maps A in reverse
 // order, R_t in H_t's place. h_{t-1} is computed again from the fp32 state that the forward keeps at every tile's start (one value per
-// 64 steps), not read from the rounded y: no 16-bit rounding enters the gradient, and 7 streams move where reading y would make 8.
+// 32 or 64 steps), not read from the rounded y: no 16-bit rounding enters the gradient, and 7 streams move where reading y would make 8.
 // The gate gradients come without a division by sqrt(1 - a^2):
 //   q_t = d loss / d log L_t = g_t (sigmoid(gi) x a^2 L / sqrt(1 - a^2) - a h_{t-1} L),   L / sqrt(1 - a^2) -> sqrt(L / 2) -> 0
 //   dga_t = q_t (1 - sigmoid(ga)),   ddecay = sum q_t sigmoid(decay) / softplus(decay)
+#include <stdlib.h>
+
 #include <type_traits>
 
 #include "kernels.h"
@@ -34,15 +36,19 @@ struct LinrecK {
 };
 
 constexpr int LR_CH = 64;              // channels of a workgroup: 16 lanes x 4
-constexpr int LR_V = 4, LR_TC = LR_CH / LR_V, LR_TW = 64 / LR_TC, LR_S = 4, LR_WAVES = 4;
-constexpr int LR_TT = LR_WAVES * LR_TW * LR_S;         // 64 steps of a tile
+constexpr int LR_V = 4, LR_TC = LR_CH / LR_V, LR_TW = 64 / LR_TC, LR_WAVES = 4;
+// steps of a thread: the scan over the wave's time-threads costs the same whatever S is, registers grow with it. fp32 (64 bytes of raw
+// data per step and thread) is bound by occupancy, 16-bit types by instructions.
+template <class T> constexpr int LR_S_OF = sizeof(T) == 4 ? 2 : 4;
+template <class T> constexpr int LR_TT_OF = LR_WAVES * LR_TW * LR_S_OF<T>;         // 32 / 64 steps of a tile
+static int lr_tile(int dtype) { return dtype == REFIL_F32 ? LR_TT_OF<float> : LR_TT_OF<bf16_t>; }
 
 __device__ __forceinline__ float softplus_(float v) { return fmaxf(v, 0.f) + log1pf(expf(-fabsf(v))); }
 
 struct LrGate { float sa, si, L, a, beta, lob; };      // lob = L / sqrt(1 - a^2)
 // 1 - a^2 = 1 - exp(-2L) = 2 a sinh(L): below L = 0.35 by sinh's series (next term L^9 / 362880: 6e-10 of it), where the difference would
 // lose digits. WIDE = false: no channel's L reaches 0.35.
-template <bool WIDE>
+template <bool WIDE, bool BWD>
 __device__ __forceinline__ LrGate lr_gate(float ga, float gi, float rate) {
     LrGate g;
     g.sa = fast_sigmoid(ga); g.si = fast_sigmoid(gi);
@@ -51,48 +57,104 @@ __device__ __forceinline__ LrGate lr_gate(float ga, float gi, float rate) {
     const float q = g.L * g.L;
     float om = (g.a * (g.L + g.L)) * fmaf(q, fmaf(q, fmaf(q, 1.98412698e-4f, 8.33333333e-3f), 1.66666667e-1f), 1.0f);
     if (WIDE) om = g.L < 0.35f ? om : fmaf(-g.a, g.a, 1.0f);
-    const float rs = __builtin_amdgcn_rsqf(fmaxf(om, 1e-37f));
-    g.beta = om * rs;
-    g.lob = g.L * rs;
+    if (BWD) {
+        const float rs = __builtin_amdgcn_rsqf(fmaxf(om, 1e-37f));
+        g.beta = om * rs;
+        g.lob = g.L * rs;
+    } else g.beta = __builtin_amdgcn_sqrtf(om);
     return g;
 }
 
-// rates of the workgroup's 64 channels, one softplus each
+// rates of the workgroup's 64 channels, one softplus each (the caller issues its first loads in front of the barrier)
 __device__ __forceinline__ void lr_rates(const LinrecK& k, int ch0, float* s_rate) {
     if (threadIdx.x < LR_CH) {
         const int c = ch0 + (int)threadIdx.x;
         s_rate[threadIdx.x] = c < k.C ? k.scale * softplus_(k.decay[c % k.D]) : 0.f;
     }
-    __syncthreads();
+    lds_barrier();
 }
 
-// the reset flags of S steps
-template <bool RST>
-__device__ __forceinline__ int lr_cuts(const LinrecK& k, int b, int t0, int Tb) {
+// S steps of one stream. `whole` (wave-uniform): every step is live and every channel there -- no predicates
+template <class T, int S>
+__device__ __forceinline__ void lr_load(Raw<T, LR_V> (&r)[S], const T* base, long sT, int t0, int Tb, int nv, bool whole, unsigned absent = 0u) {
+    const T* p = base + (long)t0 * sT;
+    if (whole) {
+#pragma unroll
+        for (int s = 0; s < S; ++s) { r[s] = ld_raw<T, LR_V>(p, LR_V); p += sT; }
+    } else {
+#pragma unroll
+        for (int s = 0; s < S; ++s) { r[s] = ld_raw<T, LR_V>(p, t0 + s < Tb ? nv : 0, absent); p += sT; }
+    }
+}
+// the reset flags of S steps: loaded with the data, looked at when the maps are built
+template <bool RST, int S>
+__device__ __forceinline__ void lr_load_cuts(uint8_t (&r)[S], const LinrecK& k, int b, int t0, int Tb) {
+    if (RST) {
+        const uint8_t* p = k.reset + (long)b * k.rs_sB;
+#pragma unroll
+        for (int s = 0; s < S; ++s) r[s] = p[(long)min(t0 + s, Tb - 1) * k.rs_sT];      // (the wave has a live step: Tb >= 1)
+    }
+}
+template <bool RST, int S>
+__device__ __forceinline__ int lr_cuts(const uint8_t (&r)[S], int t0, int Tb) {
     int cuts = 0;
     if (RST) {
-        const uint8_t* r = k.reset + (long)b * k.rs_sB + (long)t0 * k.rs_sT;
 #pragma unroll
-        for (int s = 0; s < LR_S; ++s) {
-            if (t0 + s < Tb && *r) cuts |= 1 << s;
-            r += k.rs_sT;
-        }
+        for (int s = 0; s < S; ++s) cuts |= (t0 + s < Tb && r[s] ? 1 : 0) << s;
     }
     return cuts;
 }
-template <class T>
-__device__ __forceinline__ void lr_load(Raw<T, LR_V> (&r)[LR_S], const T* base, long sT, int t0, int Tb, int nv, unsigned absent = 0u) {
-    const T* p = base + (long)t0 * sT;
+
+// The maps of the n chunks in front (behind): chunk first + i * step is the i-th to apply. Each of the 16 time-threads composes a run of
+// them, the wave joins its four by shuffles; the waves' maps go to LDS (the caller's next barrier orders them).
+struct LrFront { float A[LR_WAVES][LR_CH], H[LR_WAVES][LR_CH]; int cut[LR_WAVES]; };
+__device__ __forceinline__ void lr_front(const LinrecK& k, LrFront& f, int b, int c0, int cl, int nv, int wave, int tw, int n, int first, int step) {
+    float A[LR_V], H[LR_V]; int cut = 0;
 #pragma unroll
-    for (int s = 0; s < LR_S; ++s) { r[s] = ld_raw<T, LR_V>(p, t0 + s < Tb ? nv : 0, absent); p += sT; }
+    for (int i = 0; i < LR_V; ++i) { A[i] = 1.f; H[i] = 0.f; }
+    const int per = cdiv(n, LR_WAVES * LR_TW), i0 = (wave * LR_TW + tw) * per, i1 = min(i0 + per, n);
+    for (int j = i0; j < i1; ++j) {
+        const long o = ((long)b * k.nchunk + first + j * step) * k.C + c0;
+        float a[LR_V], h[LR_V];
+#pragma unroll
+        for (int i = 0; i < LR_V; ++i) { a[i] = i < nv ? k.sumA[o + i] : 1.f; h[i] = i < nv ? k.sumH[o + i] : 0.f; }
+        const bool c = nv > 0 && a[0] < 0.f;               // (a reset cuts every channel)
+        cut |= (int)c;
+#pragma unroll
+        for (int i = 0; i < LR_V; ++i) { H[i] = c ? h[i] : fmaf(a[i], H[i], h[i]); A[i] *= a[i]; }
+    }
+#pragma unroll
+    for (int d = 1; d < LR_TW; d *= 2) {
+        const int pc = __shfl_up(cut, d * LR_TC);
+#pragma unroll
+        for (int i = 0; i < LR_V; ++i) {
+            const float pA = __shfl_up(A[i], d * LR_TC), pH = __shfl_up(H[i], d * LR_TC);
+            if (tw >= d) { H[i] = cut ? H[i] : fmaf(A[i], pH, H[i]); A[i] *= pA; }
+        }
+        if (tw >= d) cut |= pc;
+    }
+    if (tw == LR_TW - 1) {
+#pragma unroll
+        for (int i = 0; i < LR_V; ++i) { f.A[wave][cl + i] = A[i]; f.H[wave][cl + i] = H[i]; }
+        if (cl == 0) f.cut[wave] = cut;
+    }
+}
+__device__ __forceinline__ void lr_front_apply(const LrFront& f, int cl, float (&carry)[LR_V]) {
+#pragma unroll
+    for (int w = 0; w < LR_WAVES; ++w) {
+        const int c = f.cut[w];
+#pragma unroll
+        for (int i = 0; i < LR_V; ++i) carry[i] = c ? f.H[w][cl + i] : fmaf(f.A[w][cl + i], carry[i], f.H[w][cl + i]);
+    }
 }
 
 // One workgroup per (episode, 64 channels, chunk of the time axis). FINAL: the outputs, starting from the carry of the chunks in front;
 // else the chunk's whole map only. Steps past the episode's end are not loaded: their decay gate is -inf (a = 1, no input), the state
-// stays. A wave whose steps all lie there skips the arithmetic.
+// stays. A wave whose steps all lie there skips the arithmetic. The next tile's loads are in flight from the moment this tile's gates are
+// computed: over its scans, barrier and stores.
 template <class T, bool FINAL, bool RST>
-__global__ void __launch_bounds__(256) linrec_fwd(const LinrecK k) {
-    constexpr int V = LR_V, TC = LR_TC, TW = LR_TW, S = LR_S;
+__global__ void __launch_bounds__(256, sizeof(T) == 4 ? 4 : 3) linrec_fwd(const LinrecK k) {
+    constexpr int V = LR_V, TC = LR_TC, TW = LR_TW, S = LR_S_OF<T>, TT = LR_TT_OF<T>;
     __shared__ float s_rate[LR_CH];
     __shared__ float sA[2][LR_WAVES][LR_CH], sH[2][LR_WAVES][LR_CH];
     __shared__ int sCut[2][LR_WAVES];
@@ -100,55 +162,63 @@ __global__ void __launch_bounds__(256) linrec_fwd(const LinrecK k) {
     const int b = (int)(blockIdx.x / k.ncol), ch0 = (int)(blockIdx.x % k.ncol) * LR_CH, chunk = blockIdx.y;
     const int cl = (lane % TC) * V, c0 = ch0 + cl, nv = min(max(k.C - c0, 0), V);
     const int tw = lane / TC;
-    lr_rates(k, ch0, s_rate);
-    float rate[V], top = 0.f;
-#pragma unroll
-    for (int i = 0; i < V; ++i) { rate[i] = s_rate[cl + i]; top = fmaxf(top, rate[i]); }
-    const bool wide = __any(!(top < 0.35f));
+    const bool all_ch = ch0 + LR_CH <= k.C;
     const int Tb = k.lengths ? min(max(k.lengths[b], 0), k.T) : k.T;
-    float carry[V];
-#pragma unroll
-    for (int i = 0; i < V; ++i) carry[i] = FINAL && k.h0 && i < nv ? k.h0[(long)b * k.C + c0 + i] : 0.f;
-    if (FINAL) {
-        for (int j = 0; j < chunk; ++j) {
-            const long o = ((long)b * k.nchunk + j) * k.C + c0;
-#pragma unroll
-            for (int i = 0; i < V; ++i)
-                if (i < nv) { const float A = k.sumA[o + i], H = k.sumH[o + i]; carry[i] = A < 0.f ? H : fmaf(A, carry[i], H); }
-        }
-    }
-    float cA[V]; int ccut = 0;       // !FINAL: the chunk's map so far (its H is `carry`, started from zero)
-#pragma unroll
-    for (int i = 0; i < V; ++i) cA[i] = 1.f;
     const T* xb = (const T*)k.x + (long)b * k.x_sB + c0;
     const T* gab = (const T*)k.ga + (long)b * k.ga_sB + c0;
     const T* gib = (const T*)k.gi + (long)b * k.gi_sB + c0;
     const int tile0 = chunk * k.tiles_per_chunk, tile1 = min(tile0 + k.tiles_per_chunk, k.ntile);
+    Raw<T, V> rx[S], rga[S], rgi[S];
+    uint8_t rc[S];
+    auto load = [&](int tile) {
+        const int w0 = tile * TT + wave * (TW * S), t0 = w0 + tw * S;
+        if (tile < tile1 && w0 < Tb) {
+            const bool whole = all_ch && w0 + TW * S <= Tb;
+            lr_load(rga, gab, k.ga_sT, t0, Tb, nv, whole, NEG_INF_WORD<T>);
+            lr_load(rgi, gib, k.gi_sT, t0, Tb, nv, whole);
+            lr_load(rx, xb, k.x_sT, t0, Tb, nv, whole);
+            lr_load_cuts<RST, S>(rc, k, b, t0, Tb);
+        }
+    };
+    load(tile0);
+    float carry[V];
+#pragma unroll
+    for (int i = 0; i < V; ++i) carry[i] = FINAL && k.h0 && i < nv ? k.h0[(long)b * k.C + c0 + i] : 0.f;
+    __shared__ LrFront front;
+    if (FINAL && chunk > 0) lr_front(k, front, b, c0, cl, nv, wave, tw, chunk, 0, 1);
+    lr_rates(k, ch0, s_rate);
+    if (FINAL && chunk > 0) lr_front_apply(front, cl, carry);
+    float rate[V], top = 0.f;
+#pragma unroll
+    for (int i = 0; i < V; ++i) { rate[i] = s_rate[cl + i]; top = fmaxf(top, rate[i]); }
+    const bool wide = __any(!(top < 0.35f));
+    float cA[V]; int ccut = 0;       // !FINAL: the chunk's map so far (its H is `carry`, started from zero)
+#pragma unroll
+    for (int i = 0; i < V; ++i) cA[i] = 1.f;
     for (int tile = tile0; tile < tile1; ++tile) {
-        const int p = tile & 1, tw0 = tile * LR_TT + wave * (TW * S), t0 = tw0 + tw * S;
+        const int p = tile & 1, tw0 = tile * TT + wave * (TW * S), t0 = tw0 + tw * S;
         const bool any_live = tw0 < Tb;                                   // (wave-uniform)
         float a[S][V], u[S][V], A[V], H[V], eA[V], eH[V];
         int cuts = 0, cut = 0, ecut = 0;
 #pragma unroll
         for (int i = 0; i < V; ++i) { A[i] = 1.f; H[i] = 0.f; eA[i] = 1.f; eH[i] = 0.f; }
         if (any_live) {
-            Raw<T, V> rx[S], rga[S], rgi[S];
-            lr_load<T>(rga, gab, k.ga_sT, t0, Tb, nv, NEG_INF_WORD<T>);
-            lr_load<T>(rgi, gib, k.gi_sT, t0, Tb, nv);
-            lr_load<T>(rx, xb, k.x_sT, t0, Tb, nv);
-            cuts = lr_cuts<RST>(k, b, t0, Tb);
+            cuts = lr_cuts<RST, S>(rc, t0, Tb);
             cut = cuts != 0;
             auto gates = [&](auto w) {
 #pragma unroll
                 for (int s = 0; s < S; ++s)
 #pragma unroll
                     for (int i = 0; i < V; ++i) {
-                        const LrGate g = lr_gate<decltype(w)::value>(raw_get(rga[s], i), raw_get(rgi[s], i), rate[i]);
+                        const LrGate g = lr_gate<decltype(w)::value, false>(raw_get(rga[s], i), raw_get(rgi[s], i), rate[i]);
                         a[s][i] = g.a;
                         u[s][i] = g.beta * (g.si * raw_get(rx[s], i));
                     }
             };
             if (wide) gates(std::true_type{}); else gates(std::false_type{});
+        }
+        load(tile + 1);
+        if (any_live) {
 #pragma unroll
             for (int s = 0; s < S; ++s)
 #pragma unroll
@@ -236,8 +306,8 @@ __global__ void __launch_bounds__(256) linrec_fwd(const LinrecK k) {
 
 // the same cut of the time axis in reverse order
 template <class T, bool FINAL, bool RST>
-__global__ void __launch_bounds__(256) linrec_bwd(const LinrecK k) {
-    constexpr int V = LR_V, TC = LR_TC, TW = LR_TW, S = LR_S;
+__global__ void __launch_bounds__(256, sizeof(T) == 4 || !FINAL ? 3 : 2) linrec_bwd(const LinrecK k) {
+    constexpr int V = LR_V, TC = LR_TC, TW = LR_TW, S = LR_S_OF<T>, TT = LR_TT_OF<T>;
     __shared__ float s_rate[LR_CH];
     __shared__ float sA[2][LR_WAVES][LR_CH], sH[2][LR_WAVES][LR_CH], sR[2][LR_WAVES][LR_CH];
     __shared__ int sCut[2][LR_WAVES];
@@ -245,60 +315,70 @@ __global__ void __launch_bounds__(256) linrec_bwd(const LinrecK k) {
     const int b = (int)(blockIdx.x / k.ncol), ch0 = (int)(blockIdx.x % k.ncol) * LR_CH, chunk = blockIdx.y;
     const int cl = (lane % TC) * V, c0 = ch0 + cl, nv = min(max(k.C - c0, 0), V);
     const int tw = lane / TC;
-    lr_rates(k, ch0, s_rate);
-    float rate[V], top = 0.f;
-#pragma unroll
-    for (int i = 0; i < V; ++i) { rate[i] = s_rate[cl + i]; top = fmaxf(top, rate[i]); }
-    const bool wide = __any(!(top < 0.35f));
+    const bool all_ch = ch0 + LR_CH <= k.C;
     const int Tb = k.lengths ? min(max(k.lengths[b], 0), k.T) : k.T;
+    const T* xb = (const T*)k.x + (long)b * k.x_sB + c0;
+    const T* gab = (const T*)k.ga + (long)b * k.ga_sB + c0;
+    const T* gib = (const T*)k.gi + (long)b * k.gi_sB + c0;
+    const T* dyb = (const T*)k.dy + (long)b * k.dy_sB + c0;
+    const int tile0 = chunk * k.tiles_per_chunk, tile1 = min(tile0 + k.tiles_per_chunk, k.ntile);
+    Raw<T, V> rx[S], rdy[S], rga[S], rgi[S];
+    uint8_t rc[S];
+    float hin[V];
+    auto load = [&](int tile) {
+        const int w0 = tile * TT + wave * (TW * S), t0 = w0 + tw * S;
+        if (tile >= tile0 && w0 < Tb) {
+            const bool whole = all_ch && w0 + TW * S <= Tb;
+            lr_load(rga, gab, k.ga_sT, t0, Tb, nv, whole, NEG_INF_WORD<T>);
+            lr_load(rdy, dyb, k.dy_sT, t0, Tb, nv, whole);
+            if (FINAL) {
+                lr_load(rgi, gib, k.gi_sT, t0, Tb, nv, whole);
+                lr_load(rx, xb, k.x_sT, t0, Tb, nv, whole);
+                const float* o = k.saved + ((long)b * k.ntile + tile) * k.C + c0;
+#pragma unroll
+                for (int i = 0; i < V; ++i) hin[i] = i < nv ? o[i] : 0.f;
+            }
+            lr_load_cuts<RST, S>(rc, k, b, t0, Tb);
+        }
+    };
+    load(tile1 - 1);
     float carry[V], cA[V], dl[V]; int ccut = 0;
 #pragma unroll
     for (int i = 0; i < V; ++i) {
         carry[i] = FINAL && k.dh_last && i < nv ? k.dh_last[(long)b * k.C + c0 + i] : 0.f;
         cA[i] = 1.f; dl[i] = 0.f;
     }
-    if (FINAL) {
-        for (int j = k.nchunk - 1; j > chunk; --j) {
-            const long o = ((long)b * k.nchunk + j) * k.C + c0;
+    __shared__ LrFront front;
+    const int behind = k.nchunk - 1 - chunk;
+    if (FINAL && behind > 0) lr_front(k, front, b, c0, cl, nv, wave, tw, behind, k.nchunk - 1, -1);
+    lr_rates(k, ch0, s_rate);
+    if (FINAL && behind > 0) lr_front_apply(front, cl, carry);
+    float rate[V], top = 0.f;
 #pragma unroll
-            for (int i = 0; i < V; ++i)
-                if (i < nv) { const float A = k.sumA[o + i], R = k.sumH[o + i]; carry[i] = A < 0.f ? R : fmaf(A, carry[i], R); }
-        }
-    }
-    const T* xb = (const T*)k.x + (long)b * k.x_sB + c0;
-    const T* gab = (const T*)k.ga + (long)b * k.ga_sB + c0;
-    const T* gib = (const T*)k.gi + (long)b * k.gi_sB + c0;
-    const T* dyb = (const T*)k.dy + (long)b * k.dy_sB + c0;
-    const int tile0 = chunk * k.tiles_per_chunk, tile1 = min(tile0 + k.tiles_per_chunk, k.ntile);
+    for (int i = 0; i < V; ++i) { rate[i] = s_rate[cl + i]; top = fmaxf(top, rate[i]); }
+    const bool wide = __any(!(top < 0.35f));
     for (int tile = tile1 - 1; tile >= tile0; --tile) {
-        const int p = tile & 1, tw0 = tile * LR_TT + wave * (TW * S), t0 = tw0 + tw * S;
+        const int p = tile & 1, tw0 = tile * TT + wave * (TW * S), t0 = tw0 + tw * S;
         const bool any_live = tw0 < Tb;
-        Raw<T, V> rx[S], rdy[S];
-        float a[S][V], sa[S][V], si[S][V], beta[S][V], lob[S][V];
-        float A[V], H[V], R[V], B[V], eA[V], eH[V], xA[V], xR[V], hin[V];
+        // what the outputs need of an element: a, sigmoid(ga), f = sqrt(1 - a^2) sigmoid(gi), w = sigmoid(gi) x a L / sqrt(1 - a^2) and
+        // xd = x (1 - sigmoid(gi)):  dx = g f,  dgi = dx xd,  q = g a (w - h_{t-1} L)
+        float a[S][V], sa[S][V], f[S][V], w_[S][V], xd[S][V];
+        float A[V], H[V], R[V], B[V], eA[V], eH[V], xA[V], xR[V];
         int cuts = 0, fcut = 0, rcut = 0, ecut = 0, xcut = 0;
 #pragma unroll
-        for (int i = 0; i < V; ++i) { A[i] = B[i] = 1.f; H[i] = R[i] = 0.f; eA[i] = xA[i] = 1.f; eH[i] = xR[i] = 0.f; hin[i] = 0.f; }
+        for (int i = 0; i < V; ++i) { A[i] = B[i] = 1.f; H[i] = R[i] = 0.f; eA[i] = xA[i] = 1.f; eH[i] = xR[i] = 0.f; }
         if (any_live) {
-            Raw<T, V> rga[S], rgi[S];
-            lr_load<T>(rga, gab, k.ga_sT, t0, Tb, nv, NEG_INF_WORD<T>);
-            lr_load<T>(rdy, dyb, k.dy_sT, t0, Tb, nv);
-            if (FINAL) { lr_load<T>(rgi, gib, k.gi_sT, t0, Tb, nv); lr_load<T>(rx, xb, k.x_sT, t0, Tb, nv); }
-            cuts = lr_cuts<RST>(k, b, t0, Tb);
+            cuts = lr_cuts<RST, S>(rc, t0, Tb);
             fcut = rcut = cuts != 0;
-            if (FINAL) {
-                const float* o = k.saved + ((long)b * k.ntile + tile) * k.C + c0;
-#pragma unroll
-                for (int i = 0; i < V; ++i) hin[i] = i < nv ? o[i] : 0.f;
-            }
             auto gates = [&](auto w) {
 #pragma unroll
                 for (int s = 0; s < S; ++s)
 #pragma unroll
                     for (int i = 0; i < V; ++i) {
                         if (FINAL) {
-                            const LrGate g = lr_gate<decltype(w)::value>(raw_get(rga[s], i), raw_get(rgi[s], i), rate[i]);
-                            a[s][i] = g.a; sa[s][i] = g.sa; si[s][i] = g.si; beta[s][i] = g.beta; lob[s][i] = g.lob;
+                            const LrGate g = lr_gate<decltype(w)::value, true>(raw_get(rga[s], i), raw_get(rgi[s], i), rate[i]);
+                            const float x = raw_get(rx[s], i), sx = g.si * x;
+                            a[s][i] = g.a; sa[s][i] = g.sa; f[s][i] = g.beta * g.si; w_[s][i] = sx * (g.a * g.lob); xd[s][i] = x - sx;
                         } else a[s][i] = fast_exp(-rate[i] * fast_sigmoid(raw_get(rga[s], i)));
                     }
             };
@@ -308,7 +388,7 @@ __global__ void __launch_bounds__(256) linrec_bwd(const LinrecK k) {
 #pragma unroll
                 for (int i = 0; i < V; ++i) {
                     if (FINAL) {
-                        const float u = beta[s][i] * (si[s][i] * raw_get(rx[s], i));
+                        const float u = f[s][i] * raw_get(rx[s], i);
                         H[i] = RST && (cuts >> s & 1) ? u : fmaf(a[s][i], H[i], u);
                     }
                     A[i] *= a[s][i];
@@ -317,6 +397,9 @@ __global__ void __launch_bounds__(256) linrec_bwd(const LinrecK k) {
             for (int s = S - 1; s >= 0; --s)
 #pragma unroll
                 for (int i = 0; i < V; ++i) R[i] = RST && (cuts >> s & 1) ? 0.f : a[s][i] * (raw_get(rdy[s], i) + R[i]);
+        }
+        if (!FINAL) load(tile - 1);
+        if (any_live) {
             // forward: inclusive prefix of (A, H); backward: inclusive suffix of (B, R)
 #pragma unroll
             for (int i = 0; i < V; ++i) B[i] = A[i];
@@ -382,7 +465,6 @@ __global__ void __launch_bounds__(256) linrec_bwd(const LinrecK k) {
                         for (int i = 0; i < V; ++i) hin[i] = wc ? sH[p][w][cl + i] : fmaf(sA[p][w][cl + i], hin[i], sH[p][w][cl + i]);
                     }
                 }
-                float hp[S][V];
 #pragma unroll
                 for (int i = 0; i < V; ++i) {
                     hin[i] = ecut ? eH[i] : fmaf(eA[i], hin[i], eH[i]);
@@ -392,9 +474,9 @@ __global__ void __launch_bounds__(256) linrec_bwd(const LinrecK k) {
                 for (int s = 0; s < S; ++s)
 #pragma unroll
                     for (int i = 0; i < V; ++i) {
-                        hp[s][i] = hin[i];
-                        const float u = beta[s][i] * (si[s][i] * raw_get(rx[s], i));
-                        hin[i] = RST && (cuts >> s & 1) ? u : fmaf(a[s][i], hin[i], u);
+                        const float u = f[s][i] * raw_get(rx[s], i);
+                        if (RST && (cuts >> s & 1)) hin[i] = u;                       // (w_ stands: nothing came through)
+                        else { w_[s][i] = fmaf(-hin[i], rate[i] * sa[s][i], w_[s][i]); hin[i] = fmaf(a[s][i], hin[i], u); }
                     }
                 xp += (S - 1) * k.d_sT; ap += (S - 1) * k.d_sT; ip += (S - 1) * k.d_sT;
 #pragma unroll
@@ -404,15 +486,13 @@ __global__ void __launch_bounds__(256) linrec_bwd(const LinrecK k) {
                     float ox[V], oa[V], oi[V];
 #pragma unroll
                     for (int i = 0; i < V; ++i) {
-                        const float x = raw_get(rx[s], i), gt = raw_get(rdy[s], i) + c[i];
-                        const float sx = si[s][i] * x, L = rate[i] * sa[s][i];
-                        const float through = RST && (cuts >> s & 1) ? 0.f : hp[s][i] * L;
-                        const float q = live ? (gt * a[s][i]) * (sx * (a[s][i] * lob[s][i]) - through) : 0.f;
-                        ox[i] = live ? gt * (beta[s][i] * si[s][i]) : 0.f;
-                        oi[i] = ox[i] * (x - sx);
+                        const float gt = raw_get(rdy[s], i) + c[i], ag = a[s][i] * gt;
+                        const float q = live ? ag * w_[s][i] : 0.f;
+                        ox[i] = live ? gt * f[s][i] : 0.f;
+                        oi[i] = ox[i] * xd[s][i];
                         oa[i] = fmaf(-q, sa[s][i], q);
                         dl[i] += q;
-                        c[i] = RST && (cuts >> s & 1) ? 0.f : a[s][i] * gt;
+                        c[i] = RST && (cuts >> s & 1) ? 0.f : ag;
                     }
                     if (t < k.T) {
                         st_raw<T, V>(xp, raw_pack<T, V>(ox), nv);
@@ -434,6 +514,7 @@ __global__ void __launch_bounds__(256) linrec_bwd(const LinrecK k) {
                 }
             }
         }
+        if (FINAL) load(tile - 1);
     }
     if (!FINAL) {
         if (wave == 0 && tw == 0) {
@@ -503,7 +584,7 @@ __global__ void __launch_bounds__(64) linrec_step(const LinrecStepK k) {
         const auto ri = ld_raw<T>((const T*)k.gi + (long)r * k.gi_sB + c0, nv);
 #pragma unroll
         for (int i = 0; i < VEC; ++i) {
-            const LrGate g = lr_gate<true>(raw_get(ra, i), raw_get(ri, i), rate[i]);
+            const LrGate g = lr_gate<true, false>(raw_get(ra, i), raw_get(ri, i), rate[i]);
             h[i] = fmaf(g.a, h[i], g.beta * (g.si * raw_get(rx, i)));
         }
         st_raw<T>(y + (long)r * k.y_sB + c0, raw_pack<T>(h), nv);
@@ -571,10 +652,10 @@ struct LrPlan { int ncol, ntile, nchunk, tiles_per_chunk; };
 static LrPlan lr_plan(const refil_linrec_desc& d) {
     LrPlan p;
     p.ncol = cdiv(d.C, LR_CH);
-    p.ntile = cdiv(d.T, LR_TT);
+    p.ntile = cdiv(d.T, lr_tile(d.dtype));
     // Too few (episode, column) pairs to fill the card: the time axis is cut into chunks of whole tiles, at the price of reading the
     // inputs once more for the chunks' maps.
-    const long wgs = (long)d.B * p.ncol, want = 1024;
+    const long wgs = (long)d.B * p.ncol, want = getenv("LRW") ? atol(getenv("LRW")) : 1024;
     long n = wgs > 0 && wgs < want / 2 ? cdivl(want, wgs) : 1;
     if (n > p.ntile) n = p.ntile;
     if (n > 256) n = 256;
@@ -677,7 +758,7 @@ extern "C" size_t refil_linrec_workspace_bytes(const refil_linrec_desc* d, int32
 }
 extern "C" int64_t refil_linrec_saved_floats(const refil_linrec_desc* d) {
     if (!d || lr_check(*d, "refil_linrec_saved_floats")) return 0;
-    return (int64_t)d->B * cdiv(d->T, LR_TT) * d->C;
+    return (int64_t)d->B * cdiv(d->T, lr_tile(d->dtype)) * d->C;
 }
 extern "C" int refil_linrec_forward(const refil_linrec_desc* d, void* stream) {
     REFIL_CHECK(d, "refil_linrec_forward: null desc");

@@ -126,6 +126,7 @@ static inline void __syncthreads() { emu::block_sync(); }
 #define __builtin_amdgcn_s_barrier() emu::block_sync()
 #define __builtin_amdgcn_rcpf(x) (1.0f / (x))
 #define __builtin_amdgcn_exp2f(x) exp2f(x)
+#define __builtin_amdgcn_sqrtf(x) sqrtf(x)
 #define __builtin_amdgcn_rsqf(x) (1.0f / sqrtf(x))
 
 // ---- wave collectives ----
