@@ -14,8 +14,6 @@
 // The gate gradients come without a division by sqrt(1 - a^2):
 //   q_t = d loss / d log L_t = g_t (sigmoid(gi) x a^2 L / sqrt(1 - a^2) - a h_{t-1} L),   L / sqrt(1 - a^2) -> sqrt(L / 2) -> 0
 //   dga_t = q_t (1 - sigmoid(ga)),   ddecay = sum q_t sigmoid(decay) / softplus(decay)
-#include <stdlib.h>
-
 #include <type_traits>
 
 #include "kernels.h"
@@ -602,61 +600,43 @@ __global__ void __launch_bounds__(64) linrec_step(const LinrecStepK k) {
         if (i < nv) k.state_out[(long)slot * k.C + c0 + i] = h[i];
 }
 
-// out[d] = factor(d) * sum_r src[r][d], rows in a fixed order. decay != NULL: factor = sigmoid(decay) / softplus(decay).
-__global__ void __launch_bounds__(256) colsum_stage(const float* src, long R, int D, long rows_per, float* dst) {
-    __shared__ float s[4][64];
-    const int lane = threadIdx.x & 63, w = threadIdx.x >> 6, d = blockIdx.x * 64 + lane;
-    const long r0 = (long)blockIdx.y * rows_per, r1 = min(r0 + rows_per, R);
-    float acc = 0.f;
-    if (d < D)
-        for (long r = r0 + w; r < r1; r += 4) acc += src[r * D + d];
-    s[w][lane] = acc;
-    __syncthreads();
-    if (w == 0 && d < D) dst[(long)blockIdx.y * D + d] = (s[0][lane] + s[1][lane]) + (s[2][lane] + s[3][lane]);
-}
-__global__ void __launch_bounds__(1024) colsum_final(const float* src, long R, int D, const float* decay, float* dst) {
+// ddecay[d] = sigmoid(decay) / softplus(decay) * sum_r part[r][d], rows in a fixed order: a wave's rows eight at a time, then the waves
+__global__ void __launch_bounds__(1024) linrec_ddecay(const float* src, long R, int D, const float* decay, float* dst) {
     __shared__ float s[16][64];
     const int lane = threadIdx.x & 63, w = threadIdx.x >> 6, d = blockIdx.x * 64 + lane;
     float acc = 0.f;
-    if (d < D)
-        for (long r = w; r < R; r += 16) acc += src[r * D + d];
+    if (d < D) {
+        long r = w;
+        for (; r + 7 * 16 < R; r += 8 * 16) {
+            float v[8];
+#pragma unroll
+            for (int j = 0; j < 8; ++j) v[j] = src[(r + j * 16) * D + d];
+#pragma unroll
+            for (int j = 0; j < 8; ++j) acc += v[j];
+        }
+        for (; r < R; r += 16) acc += src[r * D + d];
+    }
     s[w][lane] = acc;
     __syncthreads();
     if (w == 0 && d < D) {
         float t = 0.f;
 #pragma unroll
         for (int j = 0; j < 16; ++j) t += s[j][lane];
-        if (decay) {
-            const float v = decay[d], sp = softplus_(v);
-            t *= sp > 0.f ? (1.f / (1.f + expf(-v))) / sp : 1.f;        // (both vanish alike as decay -> -inf)
-        }
-        dst[d] = t;
+        const float v = decay[d], sp = softplus_(v);
+        dst[d] = R ? t * (sp > 0.f ? (1.f / (1.f + expf(-v))) / sp : 1.f) : 0.f;        // (both vanish alike as decay -> -inf)
     }
-}
-long colsum_tmp_floats(long R, int D) { return R > 512 ? 256L * D : 0; }
-int colsum_launch(const float* src, long R, int D, float* tmp, const float* decay, float* dst, hipStream_t st) {
-    const dim3 cols(cdiv(D, 64));
-    if (R > 512) {
-        const long per = cdivl(R, 256);
-        const int n = (int)cdivl(R, per);
-        hipLaunchKernelGGL(colsum_stage, dim3(cdiv(D, 64), n), dim3(256), 0, st, src, R, D, per, tmp);
-        REFIL_LAUNCH_CHECK();
-        src = tmp; R = n;
-    }
-    hipLaunchKernelGGL(colsum_final, cols, dim3(1024), 0, st, src, R, D, decay, dst);
-    REFIL_LAUNCH_CHECK();
-    return 0;
 }
 
 struct LrPlan { int ncol, ntile, nchunk, tiles_per_chunk; };
-static LrPlan lr_plan(const refil_linrec_desc& d) {
+static LrPlan lr_plan(const refil_linrec_desc& d, bool bwd) {
     LrPlan p;
     p.ncol = cdiv(d.C, LR_CH);
     p.ntile = cdiv(d.T, lr_tile(d.dtype));
     // Too few (episode, column) pairs to fill the card: the time axis is cut into chunks of whole tiles, at the price of reading the
-    // inputs once more for the chunks' maps.
-    const long wgs = (long)d.B * p.ncol, want = getenv("LRW") ? atol(getenv("LRW")) : 1024;
-    long n = wgs > 0 && wgs < want / 2 ? cdivl(want, wgs) : 1;
+    // inputs once more for the chunks' maps. B 4, T 8192, C 1024 bf16: forward 125 us at 1024 workgroups, 121 at 2048 (three fit a CU:
+    // the last round is shorter); backward, two a CU, 148 and 163 us (each workgroup composes the maps in front of it).
+    const long pairs = (long)d.B * p.ncol, want = bwd ? 1024 : 2048;
+    long n = pairs > 0 && pairs < 512 ? cdivl(want, pairs) : 1;
     if (n > p.ntile) n = p.ntile;
     if (n > 256) n = 256;
     p.tiles_per_chunk = n > 1 ? (int)cdivl(p.ntile, n) : p.ntile;
@@ -681,20 +661,20 @@ static LinrecK lr_args(const refil_linrec_desc& d, const LrPlan& p) {
     k.B = d.B; k.T = d.T; k.C = d.C; k.D = d.D; k.ncol = p.ncol; k.nchunk = p.nchunk; k.tiles_per_chunk = p.tiles_per_chunk; k.ntile = p.ntile;
     return k;
 }
-// workspace: [sumA][sumH] (more than one chunk), backward: [part][column-sum scratch]
+// workspace: [sumA][sumH] (more than one chunk), backward: [part]
 static long lr_sum_floats(const refil_linrec_desc& d, const LrPlan& p) { return p.nchunk > 1 ? 2L * d.B * p.nchunk * d.C : 0; }
 static long lr_ws_floats(const refil_linrec_desc& d, const LrPlan& p, bool bwd) {
     long n = lr_sum_floats(d, p);
     if (bwd) {
         const long rows = (long)d.B * p.nchunk * (d.C / d.D);
-        n += rows * d.D + colsum_tmp_floats(rows, d.D);
+        n += rows * d.D;
     }
     return n;
 }
 
 template <class T>
 static int lr_forward(const refil_linrec_desc& d, hipStream_t st) {
-    const LrPlan p = lr_plan(d);
+    const LrPlan p = lr_plan(d, false);
     LinrecK k = lr_args(d, p);
     float* ws = (float*)d.workspace;
     k.sumA = ws; k.sumH = ws ? ws + (long)d.B * p.nchunk * d.C : nullptr;
@@ -712,9 +692,14 @@ static int lr_forward(const refil_linrec_desc& d, hipStream_t st) {
     REFIL_LAUNCH_CHECK();
     return 0;
 }
+static int lr_ddecay(const refil_linrec_desc& d, const float* part, long rows, hipStream_t st) {
+    hipLaunchKernelGGL(linrec_ddecay, dim3(cdiv(d.D, 64)), dim3(1024), 0, st, part, rows, d.D, d.decay, d.ddecay);
+    REFIL_LAUNCH_CHECK();
+    return 0;
+}
 template <class T>
 static int lr_backward(const refil_linrec_desc& d, hipStream_t st) {
-    const LrPlan p = lr_plan(d);
+    const LrPlan p = lr_plan(d, true);
     LinrecK k = lr_args(d, p);
     float* ws = (float*)d.workspace;
     k.sumA = ws; k.sumH = ws + (long)d.B * p.nchunk * d.C;
@@ -734,7 +719,7 @@ static int lr_backward(const refil_linrec_desc& d, hipStream_t st) {
         else hipLaunchKernelGGL((linrec_bwd<T, true, false>), grid, dim3(256), 0, st, k);
         REFIL_LAUNCH_CHECK();
     }
-    return colsum_launch(k.part, rows, d.D, k.part + rows * d.D, d.decay, d.ddecay, st);
+    return lr_ddecay(d, k.part, rows, st);
 }
 template <class T>
 static int lr_step(const refil_linrec_step_desc& d, hipStream_t st) {
@@ -754,7 +739,7 @@ using namespace refil;
 
 extern "C" size_t refil_linrec_workspace_bytes(const refil_linrec_desc* d, int32_t backward) {
     if (!d || lr_check(*d, "refil_linrec_workspace_bytes")) return 0;
-    return (size_t)lr_ws_floats(*d, lr_plan(*d), backward != 0) * sizeof(float);
+    return (size_t)lr_ws_floats(*d, lr_plan(*d, backward != 0), backward != 0) * sizeof(float);
 }
 extern "C" int64_t refil_linrec_saved_floats(const refil_linrec_desc* d) {
     if (!d || lr_check(*d, "refil_linrec_saved_floats")) return 0;
@@ -780,7 +765,7 @@ extern "C" int refil_linrec_backward(const refil_linrec_desc* d, void* stream) {
     const size_t need = refil_linrec_workspace_bytes(d, 1);
     REFIL_CHECK(!need || (d->workspace && d->workspace_bytes >= need), "refil_linrec_backward: workspace of %zu bytes, %zu needed", d->workspace_bytes, need);
     hipStream_t st = (hipStream_t)stream;
-    if (!d->B || !d->C) return colsum_launch(nullptr, 0, d->D, nullptr, nullptr, d->ddecay, st);
+    if (!d->B || !d->C) return lr_ddecay(*d, nullptr, 0, st);
     return d->dtype == REFIL_F32 ? lr_backward<float>(*d, st) : d->dtype == REFIL_BF16 ? lr_backward<bf16_t>(*d, st) : lr_backward<f16_t>(*d, st);
 }
 extern "C" int refil_linrec_step(const refil_linrec_step_desc* d, void* stream) {
