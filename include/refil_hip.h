@@ -548,7 +548,7 @@ int refil_norm_gate_forward(const refil_norm_gate_desc* desc, void* stream);
 int refil_norm_gate_backward(const refil_norm_gate_desc* desc, void* stream);
 
 /* Gated feed-forward block: h[N,F] = act(x w_gate^T + b_gate) * (x w_up^T + b_up), x [N,D], w_* [F,D] (both with w_stride), b_* [F] or NULL,
- * all of `dtype`; act: REFIL_ACT_SILU v sigmoid(v), REFIL_ACT_GELU the tanh form. saved: NULL, or 2 N F elements of dtype that the
+ * all of `dtype`; act: REFIL_ACT_SILU v sigmoid(v), REFIL_ACT_GELU the tanh form. saved: NULL, or 2 N F floats that the
  * backward needs (the two pre-activations). Backward: dh -> dx, dw_gate, dw_up [F,D] contiguous, db_* [F] or NULL; sums in fp32, rounded
  * once. fp32 products run as six bf16 matrix products of an exact three-way split (refil_set_tuning's "wres_split" = 6 arithmetic). */
 enum { REFIL_ACT_SILU = 0, REFIL_ACT_GELU = 1 };
@@ -557,7 +557,7 @@ typedef struct refil_gated_ff_desc {
     const void* w_gate; const void* w_up; int64_t w_stride;
     const void* b_gate; const void* b_up;
     void* h; int64_t h_stride;
-    void* saved;
+    float* saved;
     const void* dh; int64_t dh_stride;
     void* dx; int64_t dx_stride;
     void* dw_gate; void* dw_up; void* db_gate; void* db_up;

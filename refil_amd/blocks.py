@@ -393,7 +393,7 @@ def _ff_desc(who, x, w_gate, w_up, act):
 
 def gated_ff_forward(x, w_gate, w_up, b_gate=None, b_up=None, *, act="silu", save=False):
     """(h, saved): h = act(x w_gate^T + b_gate) * (x w_up^T + b_up). x [..., D], w_* [F, D], b_* [F], one dtype; act "silu" or "gelu" (tanh form);
-    saved (None unless `save`): the two pre-activations in that dtype, for the backward."""
+    saved (None unless `save`): the two pre-activations, fp32, for the backward."""
     who = "gated_ff_forward"
     d = _ff_desc(who, x, w_gate, w_up, act)
     L = _lib.lib()
@@ -404,7 +404,7 @@ def gated_ff_forward(x, w_gate, w_up, b_gate=None, b_up=None, *, act="silu", sav
             keep.append(t)
             setattr(d, name, t.data_ptr())
     h = torch.empty((*x.shape[:-1], d.F), dtype=x.dtype, device=x.device)
-    saved = torch.empty((2, d.N, d.F), dtype=x.dtype, device=x.device) if save else None
+    saved = torch.empty((2, d.N, d.F), dtype=torch.float32, device=x.device) if save else None
     ws = _workspace(L.refil_gated_ff_workspace_bytes(C.byref(d), 0), x)
     d.h, d.h_stride, d.saved = h.data_ptr(), d.F, _p(saved)
     d.workspace, d.workspace_bytes = _p(ws), 0 if ws is None else ws.numel()
@@ -418,9 +418,7 @@ def gated_ff_backward(dh, x, w_gate, w_up, saved, *, act="silu", bias=False):
     d = _ff_desc(who, x, w_gate, w_up, act)
     L, F, D = _lib.lib(), d.F, d.D
     _like(dh, x, "dh", who, (*x.shape[:-1], F))
-    _like(saved, x, "saved", who, (2, d.N, F))
-    if not saved.is_contiguous():
-        raise ValueError(f"{who}: saved must be the dense tensor that gated_ff_forward returned")
+    saved = _f32(saved, x, "saved", who, (2, d.N, F))
     new = torch.empty if d.N else torch.zeros
     dx = torch.empty(x.shape, dtype=x.dtype, device=x.device)
     dwg, dwu = (new((F, D), dtype=x.dtype, device=x.device) for _ in range(2))

@@ -1,12 +1,13 @@
 // Gated feed-forward block h = act(x Wg^T + bg) * (x Wu^T + bu), forward and backward (include/refil_hip.h: refil_gated_ff_*).
 //
-// All products are C[m][n] = sum_k A[m][k] B[n][k] with both operands k-contiguous in 16 bits, on v_mfma_f32_16x16x32 (fp32 accumulate):
-//   forward   A = x, B = [Wg | Wu] interleaved so that one wave holds both projections of a column: bias, activation and product happen
-//             in its registers; h (and for training the two pre-activations) is all that is written
-//   backward  [dg | du] from the saved pre-activations and dh (one elementwise pass that also leaves the transposed copy and the bias
-//             sums); dx = [dg | du] [Wg ; Wu] with the weights transposed once per call; [dWg ; dWu] = [dg | du]^T x
-// fp32 operands are split exactly into three bf16 pieces and a product runs as six bf16 products (hi hi, hi mid, mid hi, mid mid, hi lo,
-// lo hi), as the library's projection GEMMs do: the k loop walks the six pairs of planes.
+// Every product is C[m][n] = sum_k A(m, k) B(n, k) on v_mfma_f32_16x16x32 (fp32 accumulate), tiles staged through LDS:
+//   forward   A = x, B = rows of Wg and Wu interleaved so that one wave holds both projections of a column: bias, activation and product
+//             happen in its registers; h (and for training the two pre-activations, fp32) is all that is written
+//   backward  one elementwise pass turns the saved pre-activations and dh into [dg | du] (rounded to the type once) and the bias sums;
+//             dx = [dg | du] [Wg ; Wu] and [dWg ; dWu] = [dg | du]^T x read the operands as they lie in memory: where the reduction index
+//             is the row, the LDS tile keeps rows of k and ds_read_b64_tr_b16 hands the matrix core its columns -- nothing is transposed
+// fp32 operands are split exactly into three bf16 pieces on their way into LDS and a product runs as six bf16 products (lo hi, hi lo,
+// mid mid, mid hi, hi mid, hi hi), as the library's projection GEMMs do.
 // Up to 64 rows the weights' bytes are the cost and a second kernel reads them once, straight into matrix-core fragments.
 #include "kernels.h"
 #include "profile.h"
@@ -24,10 +25,6 @@ __device__ __forceinline__ f32x4 gf_mfma(gf_u32x4 a, gf_u32x4 b, f32x4 c) {
     if constexpr (__is_same(E, f16_t)) return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(gf_f16x8, a), __builtin_bit_cast(gf_f16x8, b), c, 0, 0, 0);
     else return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(gf_bf16x8, a), __builtin_bit_cast(gf_bf16x8, b), c, 0, 0, 0);
 }
-
-// the six products of two three-way splits that reach 2^-24 of the result, leading one last (smallest terms first)
-__host__ __device__ constexpr int gf_pair_a(int p) { return p == 0 ? 2 : p == 1 ? 0 : p == 2 ? 1 : p == 3 ? 1 : p == 4 ? 0 : 0; }
-__host__ __device__ constexpr int gf_pair_b(int p) { return p == 0 ? 0 : p == 1 ? 2 : p == 2 ? 1 : p == 3 ? 0 : p == 4 ? 1 : 0; }
 
 // ---- activation ----
 // gelu(v) = v/2 (1 + tanh(A (v + B v^3)))
@@ -50,35 +47,89 @@ __device__ __forceinline__ void gf_act_grad(int act, float v, float& f, float& d
     }
 }
 
+
 // ---- the tiled product ----
+enum { GF_K = 0, GF_M = 1 };       // an operand's contiguous index: k (rows are m / n) or m / n (rows are k)
+
 struct GfGemm {
-    const void* A; long lda, planeA;
-    const void* B0; const void* B1; long ldb, planeB;        // B1: the second half of the interleaved forward
-    int M, N, K, pairs;                                      // K a multiple of 64, zero-padded
-    int splits; float* partial;                              // splits > 1: fp32 partial sums [splits][M][N]
-    void* C0; void* C1; long ldc; int msplit;                // rows >= msplit go to C1 (dWg / dWu)
-    // gated epilogue
-    const void* bias0; const void* bias1; void* save0; void* save1; int act;
+    const void* A; long lda;
+    const void* B0; const void* B1; long ldb;      // gated: B1 = the up projection; else rows of k at and behind ksplit come from B1
+    int M, N, K;
+    int a_rows, b_rows;                            // rows that exist of A, of each B (GF_M operands; GF_K: M, N)
+    int ksplit;
+    int splits; float* partial;                    // splits > 1: fp32 partial sums [splits][M][N]
+    void* C0; void* C1; long ldc; int msplit, mlim;      // rows m < msplit: row m of C0; the others: row m - msplit of C1; rows at or behind mlim of either are padding
+    const void* bias0; const void* bias1; float* save0; float* save1; int act;      // gated epilogue
 };
 
-constexpr int GF_BK = 64;
+template <class T>
+__device__ __forceinline__ void gf_gated_out(const GfGemm& k, int m, int n, int c, f32x4 ga, f32x4 ua) {
+    float g[4], u[4], h[4];
+#pragma unroll
+    for (int r = 0; r < 4; ++r) {
+        g[r] = ga[r]; u[r] = ua[r];
+        if (k.bias0 && r < c) g[r] += to_f32(((const T*)k.bias0)[n + r]);
+        if (k.bias1 && r < c) u[r] += to_f32(((const T*)k.bias1)[n + r]);
+        h[r] = gf_act(k.act, g[r]) * u[r];
+    }
+    st_raw<T, 4>((T*)k.C0 + (long)m * k.ldc + n, raw_pack<T, 4>(h), c);
+    if (k.save0) {
+        st_raw<float, 4>(k.save0 + (long)m * k.N + n, raw_pack<float, 4>(g), c);
+        st_raw<float, 4>(k.save1 + (long)m * k.N + n, raw_pack<float, 4>(u), c);
+    }
+}
+
+template <class T> constexpr int GF_P = sizeof(T) == 4 ? 3 : 1;        // 16-bit planes of an operand
+template <class T> constexpr int GF_BK = sizeof(T) == 4 ? 32 : 64;
+template <class T> struct GfElem { typedef T type; };
+template <> struct GfElem<float> { typedef bf16_t type; };
 
 __device__ __forceinline__ void gf_copy16(const void* g, void* lds) {
     // 64 lanes x 16 bytes of global memory to 1 KB of LDS behind `lds` (wave-uniform), lane order
     __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)g, (__attribute__((address_space(3))) void*)lds, 16, 0, 0);
 }
+typedef short gf_s16x4 __attribute__((ext_vector_type(4)));
+// four rows of k, 16 columns: lane i of a 16-lane group supplies columns 4 (i & 3) .. of row i >> 2 and receives column i of the four rows
+__device__ __forceinline__ uint2 gf_read_tr(const char* p) {
+    return __builtin_bit_cast(uint2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) gf_s16x4*)p));
+}
 
-// WM x WN waves, each MT x NT tiles of 16 x 16. LDS rows hold 64 k values = 8 chunks of 16 bytes, chunk c of row r in slot c ^ (r & 7):
-// the fragment reads (16 rows, one chunk) hit all banks, and the swizzle costs nothing on the way in (it permutes the lanes' addresses).
-template <class T, class E, int WM, int WN, int MT, int NT, bool GATED>
-__global__ void __launch_bounds__(WM * WN * 64) gf_gemm(const GfGemm k) {
-    constexpr int WAVES = WM * WN, BM = WM * MT * 16, BN = WN * NT * 16, HALF = GATED ? BN / 2 : BN;
-    constexpr int A_IT = BM / 8 / WAVES, B_IT = BN / 8 / WAVES;
+// Geometry of one operand's LDS tile: ROWS rows of CH chunks of 16 bytes. Which chunk sits in which slot is permuted per row so that the
+// fragment reads meet no bank twice: GF_K rows (one chunk of 16 rows is read) slot = chunk ^ row bits; GF_M rows (32 bytes of eight rows
+// k, k + 1, .. k + 3, k + 8, .. are read) pairs of chunks ^ the row's bits 0, 1 and 3.
+template <int LAY, int DIM, int BK> struct GfTile {
+    static constexpr int ROWS = LAY == GF_K ? DIM : BK, CH = (LAY == GF_K ? BK : DIM) / 8, BYTES = ROWS * CH * 16;
+    __device__ static int swz(int r) { return LAY == GF_K ? (CH == 8 ? (r & 7) : ((r >> 2) & 3)) : 2 * ((r & 3) | ((r >> 1) & 4)); }
+    // fragment of the 16 m (n) behind 16 t, k = 32 kk + 8 (lane / 16) + 0..7
+    __device__ static gf_u32x4 frag(const char* tile, int t, int kk, int lane) {
+        const int g = lane >> 4, r = lane & 15;
+        if constexpr (LAY == GF_K) return *reinterpret_cast<const gf_u32x4*>(tile + ((t * 16 + r) * CH + ((kk * 4 + g) ^ swz(r))) * 16);
+        else {
+            const int k0 = kk * 32 + g * 8 + (r >> 2);
+            const uint2 lo = gf_read_tr(tile + (k0 * CH + ((2 * t) ^ swz(k0))) * 16 + (r & 3) * 8);
+            const uint2 hi = gf_read_tr(tile + ((k0 + 4) * CH + ((2 * t) ^ swz(k0 + 4))) * 16 + (r & 3) * 8);
+            return gf_u32x4{lo.x, lo.y, hi.x, hi.y};
+        }
+    }
+};
+
+// WM x WN waves, each MT x NT tiles of 16 x 16.
+// DIRECT (16-bit, 16-byte aligned rows): global memory goes straight to LDS, two tiles in turn, the next one in flight under the
+// products of this one. Otherwise (fp32; odd widths, strides or addresses) it goes through registers -- any alignment, ragged ends filled
+// with zeros, fp32 split into its planes -- into one LDS tile, the next one in flight in registers.
+template <class T, int LA, int LB, int WM, int WN, int MT, int NT, bool DIRECT, bool GATED>
+__global__ void __launch_bounds__(WM * WN * 64, DIRECT ? 1 : 2) gf_gemm(const GfGemm k) {
+    typedef typename GfElem<T>::type E;
+    constexpr int P = GF_P<T>, BK = GF_BK<T>, WAVES = WM * WN, THREADS = WAVES * 64, BM = WM * MT * 16, BN = WN * NT * 16, HALF = GATED ? BN / 2 : BN;
+    typedef GfTile<LA, BM, BK> TA;
+    typedef GfTile<LB, BN, BK> TB;
+    constexpr int A_IT = TA::ROWS * TA::CH / THREADS, B_IT = TB::ROWS * TB::CH / THREADS;
+    static_assert(!DIRECT || P == 1, "planes are made in registers");
     extern __shared__ __attribute__((aligned(16))) char gf_smem[];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
     const int wm = wave / WN, wn = wave % WN;
     const int mt = cdiv(k.M, BM), nt = cdiv(k.N, HALF);
-    // consecutive workgroups land on different XCDs (8 of them): give each XCD a contiguous run of tiles, in 8-row panels, so that its
+    // consecutive workgroups land on different XCDs (8 of them): give each XCD a contiguous run of tiles, in panels of 8 rows, so that its
     // L2 holds the panels it reads
     const int total = mt * nt;
     int id = blockIdx.x;
@@ -89,36 +140,15 @@ __global__ void __launch_bounds__(WM * WN * 64) gf_gemm(const GfGemm k) {
     const int panel = id / (8 * nt), prow = min(8, mt - panel * 8), in_panel = id - panel * 8 * nt;
     const int m0 = (panel * 8 + in_panel % prow) * BM, n0 = in_panel / prow * HALF;
     const int split = blockIdx.y;
+    const int iters = cdiv(k.K, BK), per = cdiv(iters, k.splits), it0 = min(split * per, iters), it1 = min(it0 + per, iters);
 
-    const E* pa[A_IT]; const E* pb[B_IT];
-#pragma unroll
-    for (int i = 0; i < A_IT; ++i) {
-        const int r = (i * WAVES + wave) * 8 + (lane >> 3), ch = (lane & 7) ^ (r & 7);
-        pa[i] = (const E*)k.A + (long)min(m0 + r, k.M - 1) * k.lda + ch * 8;
-    }
-#pragma unroll
-    for (int i = 0; i < B_IT; ++i) {
-        const int r = (i * WAVES + wave) * 8 + (lane >> 3), ch = (lane & 7) ^ (r & 7);
-        const E* src = (const E*)k.B0;
-        int n = n0 + r;
-        if (GATED) {      // rows of a wave's columns: NT/2 tiles of the gate, then the same columns of the up projection
-            const int w = r / (NT * 16), j = r % (NT * 16);
-            if (j >= NT * 8) src = (const E*)k.B1;
-            n = n0 + w * NT * 8 + j % (NT * 8);
-        }
-        pb[i] = src + (long)min(n, k.N - 1) * k.ldb + ch * 8;
-    }
-    const int kb = k.K / GF_BK, iters = kb * k.pairs;
-    const int per = cdiv(iters, k.splits), it0 = min(split * per, iters), it1 = min(it0 + per, iters);
-    char* const sa = gf_smem; char* const sb = gf_smem + 2 * BM * 128;
-
-    auto stage = [&](int it, int buf) {
-        const int p = it / kb, kk = it - p * kb;
-        const long oa = (k.pairs > 1 ? gf_pair_a(p) * k.planeA : 0) + (long)kk * GF_BK, ob = (k.pairs > 1 ? gf_pair_b(p) * k.planeB : 0) + (long)kk * GF_BK;
-#pragma unroll
-        for (int i = 0; i < A_IT; ++i) gf_copy16(pa[i] + oa, sa + buf * BM * 128 + (i * WAVES + wave) * 1024);
-#pragma unroll
-        for (int i = 0; i < B_IT; ++i) gf_copy16(pb[i] + ob, sb + buf * BN * 128 + (i * WAVES + wave) * 1024);
+    // row n of the (interleaved) B tile -> source and row: NT/2 tiles of the gate, then the same columns of the up projection, per wave
+    auto b_row = [&](int r, const T*& src) {
+        src = (const T*)k.B0;
+        if (!GATED) return n0 + r;
+        const int w = r / (NT * 16), j = r % (NT * 16);
+        if (j >= NT * 8) src = (const T*)k.B1;
+        return n0 + w * NT * 8 + j % (NT * 8);
     };
 
     f32x4 acc[MT][NT];
@@ -127,27 +157,132 @@ __global__ void __launch_bounds__(WM * WN * 64) gf_gemm(const GfGemm k) {
 #pragma unroll
         for (int j = 0; j < NT; ++j) acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
 
-    if (it0 < it1) stage(it0, 0);
-    __syncthreads();
-    for (int it = it0; it < it1; ++it) {
-        const int buf = (it - it0) & 1;
-        if (it + 1 < it1) stage(it + 1, buf ^ 1);
-        const char* a = sa + buf * BM * 128 + wm * MT * 16 * 128;
-        const char* b = sb + buf * BN * 128 + wn * NT * 16 * 128;
+    auto products = [&](const char* a, const char* b) {
 #pragma unroll
-        for (int kk = 0; kk < 2; ++kk) {
-            const int r = lane & 15, slot = ((kk * 4 + (lane >> 4)) ^ (r & 7)) * 16;
-            gf_u32x4 fa[MT], fb[NT];
+        for (int kk = 0; kk < BK / 32; ++kk) {
+            gf_u32x4 fa[P][MT], fb[P][NT];
 #pragma unroll
-            for (int i = 0; i < MT; ++i) fa[i] = *reinterpret_cast<const gf_u32x4*>(a + (i * 16 + r) * 128 + slot);
+            for (int p = 0; p < P; ++p) {
 #pragma unroll
-            for (int j = 0; j < NT; ++j) fb[j] = *reinterpret_cast<const gf_u32x4*>(b + (j * 16 + r) * 128 + slot);
+                for (int i = 0; i < MT; ++i) fa[p][i] = TA::frag(a + p * TA::BYTES, wm * MT + i, kk, lane);
+#pragma unroll
+                for (int j = 0; j < NT; ++j) fb[p][j] = TB::frag(b + p * TB::BYTES, wn * NT + j, kk, lane);
+            }
+            // D rows = n, columns = m: a lane holds 4 neighbouring n of one m
 #pragma unroll
             for (int i = 0; i < MT; ++i)
 #pragma unroll
-                for (int j = 0; j < NT; ++j) acc[i][j] = gf_mfma<E>(fb[j], fa[i], acc[i][j]);      // D rows = n, columns = m: a lane holds 4 neighbouring n
+                for (int j = 0; j < NT; ++j) {
+                    if constexpr (P == 3) {
+                        acc[i][j] = gf_mfma<E>(fb[0][j], fa[P - 1][i], acc[i][j]);
+                        acc[i][j] = gf_mfma<E>(fb[P - 1][j], fa[0][i], acc[i][j]);
+                        acc[i][j] = gf_mfma<E>(fb[P / 2][j], fa[P / 2][i], acc[i][j]);
+                        acc[i][j] = gf_mfma<E>(fb[0][j], fa[P / 2][i], acc[i][j]);
+                        acc[i][j] = gf_mfma<E>(fb[P / 2][j], fa[0][i], acc[i][j]);
+                    }
+                    acc[i][j] = gf_mfma<E>(fb[0][j], fa[0][i], acc[i][j]);
+                }
         }
-        __syncthreads();
+    };
+
+    if constexpr (DIRECT) {
+        char* const sa = gf_smem; char* const sb = gf_smem + 2 * TA::BYTES;
+        const T* pa[A_IT]; const T* pb[B_IT]; int ob[B_IT];      // (ob: a column of B, whose rows change hands at ksplit)
+#pragma unroll
+        for (int i = 0; i < A_IT; ++i) {
+            const int e = (i * WAVES + wave) * 64 + lane, r = e / TA::CH, ch = (e % TA::CH) ^ TA::swz(r);
+            if (LA == GF_K) pa[i] = (const T*)k.A + (long)min(m0 + r, k.M - 1) * k.lda + ch * 8;
+            else pa[i] = (const T*)k.A + min(m0 + ch * 8, k.M - 8);
+        }
+#pragma unroll
+        for (int i = 0; i < B_IT; ++i) {
+            const int e = (i * WAVES + wave) * 64 + lane, r = e / TB::CH, ch = (e % TB::CH) ^ TB::swz(r);
+            if (LB == GF_K) {
+                const T* src; const int n = b_row(r, src);
+                pb[i] = src + (long)min(n, k.N - 1) * k.ldb + ch * 8;
+            } else ob[i] = min(n0 + ch * 8, k.N - 8);
+        }
+        auto stage = [&](int it, int buf) {
+            const int k0 = it * BK;
+#pragma unroll
+            for (int i = 0; i < A_IT; ++i) {
+                const int r = ((i * WAVES + wave) * 64 + lane) / TA::CH;
+                const T* p = LA == GF_K ? pa[i] + k0 : pa[i] + (long)min(k0 + r, k.a_rows - 1) * k.lda;
+                gf_copy16(p, sa + buf * TA::BYTES + (i * WAVES + wave) * 1024);
+            }
+            const T* src = (const T*)k.B0; int kb = k0;
+            if (LB == GF_M && k0 >= k.ksplit) { src = (const T*)k.B1; kb -= k.ksplit; }
+#pragma unroll
+            for (int i = 0; i < B_IT; ++i) {
+                const int r = ((i * WAVES + wave) * 64 + lane) / TB::CH;
+                const T* p = LB == GF_K ? pb[i] + k0 : src + ob[i] + (long)min(kb + r, k.b_rows - 1) * k.ldb;
+                gf_copy16(p, sb + buf * TB::BYTES + (i * WAVES + wave) * 1024);
+            }
+        };
+        if (it0 < it1) stage(it0, 0);
+        __syncthreads();                    // (also waits for the copies)
+        for (int it = it0; it < it1; ++it) {
+            const int buf = (it - it0) & 1;
+            if (it + 1 < it1) stage(it + 1, buf ^ 1);
+            products(sa + buf * TA::BYTES, sb + buf * TB::BYTES);
+            __syncthreads();
+        }
+    } else {
+        char* const sa = gf_smem; char* const sb = gf_smem + P * TA::BYTES;
+        Raw<T> ra[A_IT][8 / VEC_OF<T>], rb[B_IT][8 / VEC_OF<T>];
+        constexpr int V = VEC_OF<T>;
+        auto fetch = [&](Raw<T> (&r)[8 / V], const T* p, int n) {
+#pragma unroll
+            for (int q = 0; q < 8 / V; ++q) r[q] = ld_raw<T, V>(p + q * V, min(max(n - q * V, 0), V));
+        };
+        auto load = [&](int it) {
+            const int k0 = it * BK;
+#pragma unroll
+            for (int i = 0; i < A_IT; ++i) {
+                const int e = i * THREADS + (int)threadIdx.x, r = e / TA::CH, c = (e % TA::CH) * 8;
+                const int row = LA == GF_K ? m0 + r : k0 + r, col = LA == GF_K ? k0 + c : m0 + c;
+                const bool in = row < (LA == GF_K ? k.M : min(k.a_rows, k.K));
+                fetch(ra[i], (const T*)k.A + (long)(in ? row : 0) * k.lda + col, in ? (LA == GF_K ? k.K : k.M) - col : 0);
+            }
+            const T* src = (const T*)k.B0; int kb = k0;
+            if (LB == GF_M && k0 >= k.ksplit) { src = (const T*)k.B1; kb -= k.ksplit; }
+#pragma unroll
+            for (int i = 0; i < B_IT; ++i) {
+                const int e = i * THREADS + (int)threadIdx.x, r = e / TB::CH, c = (e % TB::CH) * 8;
+                int row = kb + r; const int col = LB == GF_K ? k0 + c : n0 + c;
+                if (LB == GF_K) row = b_row(r, src);
+                const bool in = row < (LB == GF_K ? k.N : k.b_rows);
+                fetch(rb[i], src + (long)(in ? row : 0) * k.ldb + col, in ? (LB == GF_K ? k.K : k.N) - col : 0);
+            }
+        };
+        auto put = [&](char* tile, int bytes, int slot, const Raw<T> (&r)[8 / V]) {
+            if constexpr (P == 1) *reinterpret_cast<gf_u32x4*>(tile + slot * 16) = gf_u32x4{r[0].w[0], r[0].w[1], r[0].w[2], r[0].w[3]};
+            else {
+                unsigned h[4], m[4], l[4];
+#pragma unroll
+                for (int q = 0; q < 4; ++q) wr_split(raw_get(r[q / 2], 2 * (q & 1)), raw_get(r[q / 2], 2 * (q & 1) + 1), h[q], m[q], l[q]);
+                *reinterpret_cast<gf_u32x4*>(tile + slot * 16) = gf_u32x4{h[0], h[1], h[2], h[3]};
+                *reinterpret_cast<gf_u32x4*>(tile + bytes + slot * 16) = gf_u32x4{m[0], m[1], m[2], m[3]};
+                *reinterpret_cast<gf_u32x4*>(tile + 2 * bytes + slot * 16) = gf_u32x4{l[0], l[1], l[2], l[3]};
+            }
+        };
+        if (it0 < it1) load(it0);
+        for (int it = it0; it < it1; ++it) {
+            lds_barrier();                  // the products of the tile before have been read
+#pragma unroll
+            for (int i = 0; i < A_IT; ++i) {
+                const int e = i * THREADS + (int)threadIdx.x, r = e / TA::CH;
+                put(sa, TA::BYTES, r * TA::CH + ((e % TA::CH) ^ TA::swz(r)), ra[i]);
+            }
+#pragma unroll
+            for (int i = 0; i < B_IT; ++i) {
+                const int e = i * THREADS + (int)threadIdx.x, r = e / TB::CH;
+                put(sb, TB::BYTES, r * TB::CH + ((e % TB::CH) ^ TB::swz(r)), rb[i]);
+            }
+            lds_barrier();
+            if (it + 1 < it1) load(it + 1);
+            products(sa, sb);
+        }
     }
 
     // lane: m = lane & 15, n = 4 (lane >> 4) + 0..3 of every tile
@@ -158,40 +293,21 @@ __global__ void __launch_bounds__(WM * WN * 64) gf_gemm(const GfGemm k) {
         if constexpr (GATED) {
 #pragma unroll
             for (int j = 0; j < NT / 2; ++j) {
-                const int n = n0 + wn * NT * 8 + j * 16 + (lane >> 4) * 4;
-                float g[4], u[4], h[4];
-#pragma unroll
-                for (int r = 0; r < 4; ++r) {
-                    g[r] = acc[i][j][r]; u[r] = acc[i][j + NT / 2][r];
-                    if (k.bias0 && n + r < k.N) g[r] += to_f32(((const T*)k.bias0)[n + r]);
-                    if (k.bias1 && n + r < k.N) u[r] += to_f32(((const T*)k.bias1)[n + r]);
-                    h[r] = gf_act(k.act, g[r]) * u[r];
-                }
-                T* c = (T*)k.C0 + (long)m * k.ldc + n;
-#pragma unroll
-                for (int r = 0; r < 4; ++r)
-                    if (n + r < k.N) c[r] = from_f32<T>(h[r]);
-                if (k.save0) {
-                    T* s0 = (T*)k.save0 + (long)m * k.N + n; T* s1 = (T*)k.save1 + (long)m * k.N + n;
-#pragma unroll
-                    for (int r = 0; r < 4; ++r)
-                        if (n + r < k.N) { s0[r] = from_f32<T>(g[r]); s1[r] = from_f32<T>(u[r]); }
-                }
+                const int n = n0 + wn * NT * 8 + j * 16 + (lane >> 4) * 4, c = min(max(k.N - n, 0), 4);
+                gf_gated_out<T>(k, m, n, c, acc[i][j], acc[i][j + NT / 2]);
             }
         } else {
 #pragma unroll
             for (int j = 0; j < NT; ++j) {
-                const int n = n0 + (wn * NT + j) * 16 + (lane >> 4) * 4;
-                if (k.splits > 1) {
-                    float* c = k.partial + ((long)split * k.M + m) * k.N + n;
+                const int n = n0 + (wn * NT + j) * 16 + (lane >> 4) * 4, c = min(max(k.N - n, 0), 4);
+                float v[4];
 #pragma unroll
-                    for (int r = 0; r < 4; ++r)
-                        if (n + r < k.N) c[r] = acc[i][j][r];
-                } else {
-                    T* c = (m < k.msplit ? (T*)k.C0 + (long)m * k.ldc : (T*)k.C1 + (long)(m - k.msplit) * k.ldc) + n;
-#pragma unroll
-                    for (int r = 0; r < 4; ++r)
-                        if (n + r < k.N) c[r] = from_f32<T>(acc[i][j][r]);
+                for (int r = 0; r < 4; ++r) v[r] = acc[i][j][r];
+                if (k.splits > 1) st_raw<float, 4>(k.partial + ((long)split * k.M + m) * k.N + n, raw_pack<float, 4>(v), c);
+                else {
+                    const bool first = m < k.msplit;
+                    const int row = first ? m : m - k.msplit;
+                    if (row < k.mlim) st_raw<T, 4>((T*)(first ? k.C0 : k.C1) + (long)row * k.ldc + n, raw_pack<T, 4>(v), c);
                 }
             }
         }
@@ -200,125 +316,188 @@ __global__ void __launch_bounds__(WM * WN * 64) gf_gemm(const GfGemm k) {
 
 // sums of the split products, in split order
 template <class T>
-__global__ void __launch_bounds__(256) gf_reduce(const float* partial, int splits, int M, int N, void* C0, void* C1, long ldc, int msplit) {
-    const long n = (long)M * N;
+__global__ void __launch_bounds__(256) gf_reduce(const GfGemm k) {
+    const long n = (long)k.M * k.N;
     for (long e = (long)blockIdx.x * 256 + threadIdx.x; e < n; e += (long)gridDim.x * 256) {
+        const int m = (int)(e / k.N), c = (int)(e - (long)m * k.N);
+        const bool first = m < k.msplit;
+        const int row = first ? m : m - k.msplit;
+        if (row >= k.mlim) continue;
         float s = 0.f;
-        for (int p = 0; p < splits; ++p) s += partial[p * n + e];
-        const int m = (int)(e / N), c = (int)(e - (long)m * N);
-        T* o = m < msplit ? (T*)C0 + (long)m * ldc : (T*)C1 + (long)(m - msplit) * ldc;
-        o[c] = from_f32<T>(s);
+        int p = 0;
+        for (; p + 8 <= k.splits; p += 8) {
+            float v[8];
+#pragma unroll
+            for (int j = 0; j < 8; ++j) v[j] = k.partial[(p + j) * n + e];
+#pragma unroll
+            for (int j = 0; j < 8; ++j) s += v[j];
+        }
+        for (; p < k.splits; ++p) s += k.partial[p * n + e];
+        ((T*)(first ? k.C0 : k.C1))[(long)row * k.ldc + c] = from_f32<T>(s);
     }
 }
 
-// ---- operands into k-contiguous, zero-padded 16-bit form ----
-template <class T> struct GfElem { typedef T type; static constexpr int planes = 1; };
-template <> struct GfElem<float> { typedef bf16_t type; static constexpr int planes = 3; };
-
-template <class T>
-__device__ __forceinline__ void gf_emit(void* dst, long plane, long o, float v) {
+// ---- few rows: every weight is read once, straight into fragments ----
+// A workgroup owns 16 columns of h, its eight waves share the reduction; a lane reads 16 neighbouring k (two matrix steps) of one weight
+// row, so that a row's reads are whole cache lines -- the order of k inside a product is free as long as both operands share it.
+template <class T, int MT>
+__global__ void __launch_bounds__(512) gf_skinny(const GfGemm k) {
     typedef typename GfElem<T>::type E;
-    E* d = (E*)dst;
-    if constexpr (GfElem<T>::planes == 1) d[o] = from_f32<T>(v);
-    else {
-        const E h = (E)v; const float r1 = v - (float)h;
-        const E m = (E)r1; const float r2 = r1 - (float)m;
-        d[o] = h; d[o + plane] = m; d[o + 2 * plane] = (E)r2;
-    }
-}
-// dst[r][c] = src[r][c], c in [0, Kp)
-template <class T>
-__global__ void __launch_bounds__(256) gf_pack(const void* src, long ld, long rows, int K, int Kp, void* dst, long ldd, long plane) {
-    const long n = rows * Kp;
-    for (long e = (long)blockIdx.x * 256 + threadIdx.x; e < n; e += (long)gridDim.x * 256) {
-        const long r = e / Kp; const int c = (int)(e - r * Kp);
-        gf_emit<T>(dst, plane, r * ldd + c, c < K ? to_f32(((const T*)src)[r * ld + c]) : 0.f);
-    }
-}
-// dst[c][r] = src[r][c], r in [0, Rp): 64 x 64 tiles through LDS
-template <class T>
-__global__ void __launch_bounds__(256) gf_transpose(const void* src, long ld, long rows, int cols, long Rp, void* dst, long ldd, long plane) {
-    __shared__ float t[64][65];
-    const long r0 = (long)blockIdx.x * 64; const int c0 = blockIdx.y * 64, l = threadIdx.x & 63, q = threadIdx.x >> 6;
+    constexpr int P = GF_P<T>, V = VEC_OF<T>, Q = 16 / V;
+    __shared__ float s_acc[8][2][MT][64][4];
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6), r = lane & 15, g = lane >> 4;
+    const int n0 = blockIdx.x * 16;
+    const bool in_n = n0 + r < k.N;
+    const T* pg = (const T*)k.B0 + (long)(in_n ? n0 + r : 0) * k.ldb;
+    const T* pu = (const T*)k.B1 + (long)(in_n ? n0 + r : 0) * k.ldb;
+    f32x4 acc[2][MT];
 #pragma unroll
-    for (int i = 0; i < 16; ++i) {
-        const long r = r0 + i * 4 + q; const int c = c0 + l;
-        t[i * 4 + q][l] = r < rows && c < cols ? to_f32(((const T*)src)[r * ld + c]) : 0.f;
+    for (int z = 0; z < 2; ++z)
+#pragma unroll
+        for (int i = 0; i < MT; ++i) acc[z][i] = f32x4{0.f, 0.f, 0.f, 0.f};
+    auto fetch = [&](Raw<T> (&o)[Q], const T* p, int k0, bool in) {
+#pragma unroll
+        for (int q = 0; q < Q; ++q) o[q] = ld_raw<T, V>(p + k0 + q * V, in ? min(max(k.K - k0 - q * V, 0), V) : 0);
+    };
+    auto planes = [&](const Raw<T> (&o)[Q], int half, gf_u32x4 (&f)[P]) {
+        if constexpr (P == 1) f[0] = gf_u32x4{o[half].w[0], o[half].w[1], o[half].w[2], o[half].w[3]};
+        else {
+#pragma unroll
+            for (int q = 0; q < 4; ++q) {
+                unsigned h, m, l;
+                wr_split(raw_get(o[half * 2 + q / 2], 2 * (q & 1)), raw_get(o[half * 2 + q / 2], 2 * (q & 1) + 1), h, m, l);
+                f[0][q] = h; f[P / 2][q] = m; f[P - 1][q] = l;
+            }
+        }
+    };
+    for (int kb = wave * 64; kb < k.K; kb += 8 * 64) {
+        const int k0 = kb + g * 16;
+        Raw<T> wg[Q], wu[Q], x[MT][Q];
+        fetch(wg, pg, k0, in_n);
+        fetch(wu, pu, k0, in_n);
+#pragma unroll
+        for (int i = 0; i < MT; ++i) {
+            const int m = i * 16 + r;
+            fetch(x[i], (const T*)k.A + (long)min(m, k.M - 1) * k.lda, k0, m < k.M);
+        }
+#pragma unroll
+        for (int half = 0; half < 2; ++half) {
+            gf_u32x4 fg[P], fu[P];
+            planes(wg, half, fg);
+            planes(wu, half, fu);
+#pragma unroll
+            for (int i = 0; i < MT; ++i) {
+                gf_u32x4 fx[P];
+                planes(x[i], half, fx);
+                if constexpr (P == 3) {
+                    acc[0][i] = gf_mfma<E>(fg[0], fx[P - 1], acc[0][i]); acc[1][i] = gf_mfma<E>(fu[0], fx[P - 1], acc[1][i]);
+                    acc[0][i] = gf_mfma<E>(fg[P - 1], fx[0], acc[0][i]); acc[1][i] = gf_mfma<E>(fu[P - 1], fx[0], acc[1][i]);
+                    acc[0][i] = gf_mfma<E>(fg[P / 2], fx[P / 2], acc[0][i]); acc[1][i] = gf_mfma<E>(fu[P / 2], fx[P / 2], acc[1][i]);
+                    acc[0][i] = gf_mfma<E>(fg[0], fx[P / 2], acc[0][i]); acc[1][i] = gf_mfma<E>(fu[0], fx[P / 2], acc[1][i]);
+                    acc[0][i] = gf_mfma<E>(fg[P / 2], fx[0], acc[0][i]); acc[1][i] = gf_mfma<E>(fu[P / 2], fx[0], acc[1][i]);
+                }
+                acc[0][i] = gf_mfma<E>(fg[0], fx[0], acc[0][i]); acc[1][i] = gf_mfma<E>(fu[0], fx[0], acc[1][i]);
+            }
+        }
     }
+#pragma unroll
+    for (int z = 0; z < 2; ++z)
+#pragma unroll
+        for (int i = 0; i < MT; ++i)
+#pragma unroll
+            for (int q = 0; q < 4; ++q) s_acc[wave][z][i][lane][q] = acc[z][i][q];
     __syncthreads();
+    if (wave < MT) {
+        f32x4 a[2];
 #pragma unroll
-    for (int i = 0; i < 16; ++i) {
-        const int c = c0 + i * 4 + q; const long r = r0 + l;
-        if (c < cols && r < Rp) gf_emit<T>(dst, plane, (long)c * ldd + r, t[l][i * 4 + q]);
+        for (int z = 0; z < 2; ++z)
+#pragma unroll
+            for (int q = 0; q < 4; ++q) {
+                float t = 0.f;
+#pragma unroll
+                for (int w = 0; w < 8; ++w) t += s_acc[w][z][wave][lane][q];
+                a[z][q] = t;
+            }
+        const int m = wave * 16 + r, n = n0 + g * 4;
+        if (m < k.M) gf_gated_out<T>(k, m, n, min(max(k.N - n, 0), 4), a[0], a[1]);
     }
 }
-// [dg | du] of a 64 x 64 tile of (row, column): rows [N][2 Fp], transposed [2 F][Np], and the tile's column sums
+
+// ---- the elementwise part of the backward ----
+// [dg | du] of rows [0, rows_out) (rows behind N and columns behind F are zero: the products read whole 64-blocks of them), rounded to T:
+// in 16 bits half a step of each, which the products carry on as they carry x's and the weights'. A workgroup walks `per` rows of 32
+// vectors of columns and leaves one partial row of the bias sums, taken before the rounding.
 struct GfGrad {
-    const void* sg; const void* su; const void* dh; long dh_s; long N; int F, act;
-    void* rows; long ldr, plane_r; int Fp; void* cols; long ldc, plane_c; long Np; float* colsum;      // colsum [tiles of N][2 F] or NULL
+    const float* sg; const float* su; const void* dh; long dh_s; long N, rows_out; int F, Fp, act;
+    void* out; long ldo; float* colsum; int per;      // colsum [row blocks][2 Fp] or NULL
 };
 template <class T>
 __global__ void __launch_bounds__(256) gf_grad(const GfGrad k) {
-    __shared__ float t[2][64][65];
-    const long r0 = (long)blockIdx.x * 64; const int c0 = blockIdx.y * 64, l = threadIdx.x & 63, q = threadIdx.x >> 6;
+    constexpr int V = VEC_OF<T>, CT = 32, RT = 8;
+    __shared__ float s[RT][2][CT * V];
+    const int ct = threadIdx.x % CT, rt = threadIdx.x / CT;
+    const int c0 = (blockIdx.y * CT + ct) * V, nv = min(max(k.F - c0, 0), V), np = min(max(k.Fp - c0, 0), V);
+    const long r0 = (long)blockIdx.x * k.per, r1 = min(r0 + k.per, k.rows_out);
+    float bg[V], bu[V];
 #pragma unroll
-    for (int i = 0; i < 16; ++i) {
-        const long r = r0 + i * 4 + q; const int c = c0 + l;
-        float dg = 0.f, du = 0.f;
-        if (r < k.N && c < k.F) {
-            const float g = to_f32(((const T*)k.sg)[r * k.F + c]), u = to_f32(((const T*)k.su)[r * k.F + c]), d = to_f32(((const T*)k.dh)[r * k.dh_s + c]);
+    for (int i = 0; i < V; ++i) bg[i] = bu[i] = 0.f;
+    for (long r = r0 + rt; r < r1; r += RT) {
+        const int n = r < k.N ? nv : 0;
+        const long o = r * k.F + c0;
+        const auto rd = ld_raw<T, V>((const T*)k.dh + r * k.dh_s + c0, n);
+        Raw<float> rg[V / 4], ru[V / 4];
+#pragma unroll
+        for (int q = 0; q < V / 4; ++q) {
+            rg[q] = ld_raw<float, 4>(k.sg + o + q * 4, min(max(n - q * 4, 0), 4));
+            ru[q] = ld_raw<float, 4>(k.su + o + q * 4, min(max(n - q * 4, 0), 4));
+        }
+        float dg[V], du[V];
+#pragma unroll
+        for (int i = 0; i < V; ++i) {
             float f, df;
-            gf_act_grad(k.act, g, f, df);
-            dg = d * u * df; du = d * f;
+            gf_act_grad(k.act, raw_get(rg[i / 4], i % 4), f, df);
+            const float d = raw_get(rd, i);
+            dg[i] = i < n ? d * raw_get(ru[i / 4], i % 4) * df : 0.f;
+            du[i] = i < n ? d * f : 0.f;
+            bg[i] += dg[i]; bu[i] += du[i];
         }
-        t[0][i * 4 + q][l] = dg; t[1][i * 4 + q][l] = du;
-        if (r < k.N && c < k.Fp) {
-            gf_emit<T>(k.rows, k.plane_r, r * k.ldr + c, dg);
-            gf_emit<T>(k.rows, k.plane_r, r * k.ldr + k.Fp + c, du);
-        }
+        T* p = (T*)k.out + r * k.ldo + c0;
+        st_raw<T, V>(p, raw_pack<T, V>(dg), np);
+        st_raw<T, V>(p + k.Fp, raw_pack<T, V>(du), np);
     }
-    __syncthreads();
+    if (!k.colsum) return;
 #pragma unroll
-    for (int i = 0; i < 16; ++i) {
-        const int c = c0 + i * 4 + q; const long r = r0 + l;
-        if (c < k.F && r < k.Np) {
-            gf_emit<T>(k.cols, k.plane_c, (long)c * k.ldc + r, t[0][l][i * 4 + q]);
-            gf_emit<T>(k.cols, k.plane_c, (long)(k.F + c) * k.ldc + r, t[1][l][i * 4 + q]);
-        }
-    }
-    if (k.colsum && threadIdx.x < 128) {
-        const int z = threadIdx.x >> 6, c = c0 + l;
-        float s = 0.f;
-        for (int i = 0; i < 64; ++i) s += t[z][i][l];
-        if (c < k.F) k.colsum[(long)blockIdx.x * 2 * k.F + z * k.F + c] = s;
+    for (int i = 0; i < V; ++i) { s[rt][0][ct * V + i] = bg[i]; s[rt][1][ct * V + i] = bu[i]; }
+    __syncthreads();
+    for (int e = threadIdx.x; e < 2 * CT * V; e += 256) {
+        const int z = e / (CT * V), c = e % (CT * V), col = blockIdx.y * CT * V + c;
+        float t = 0.f;
+#pragma unroll
+        for (int q = 0; q < RT; ++q) t += s[q][z][c];
+        if (col < k.F) k.colsum[(long)blockIdx.x * 2 * k.F + z * k.F + col] = t;
     }
 }
-// bias gradients: column sums over the row tiles
+// bias gradients: the partial rows in order
 template <class T>
-__global__ void __launch_bounds__(256) gf_bias(const float* part, long R, int F, void* dbg, void* dbu) {
-    __shared__ float s[4][64];
+__global__ void __launch_bounds__(1024) gf_bias(const float* part, int R, int F, void* dbg, void* dbu) {
+    __shared__ float s[16][64];
     const int lane = threadIdx.x & 63, w = threadIdx.x >> 6, c = blockIdx.x * 64 + lane;
     float acc = 0.f;
     if (c < 2 * F)
-        for (long r = w; r < R; r += 4) acc += part[r * 2 * F + c];
+        for (int r = w; r < R; r += 16) acc += part[(long)r * 2 * F + c];
     s[w][lane] = acc;
     __syncthreads();
     if (w == 0 && c < 2 * F) {
-        const float v = (s[0][lane] + s[1][lane]) + (s[2][lane] + s[3][lane]);
+        float v = 0.f;
+#pragma unroll
+        for (int j = 0; j < 16; ++j) v += s[j][lane];
         T* o = (T*)(c < F ? dbg : dbu);
         if (o) o[c < F ? c : c - F] = from_f32<T>(v);
     }
 }
 
 // ---- host ----
-static int pad64(long n) { return (int)((n + 63) / 64 * 64); }
-static bool gf_direct(const refil_gated_ff_desc& d, const void* p, long ld) {
-    return d.dtype != REFIL_F32 && d.D % 64 == 0 && ld % 8 == 0 && (uintptr_t)p % 16 == 0;
-}
-static int gf_planes(int dtype) { return dtype == REFIL_F32 ? 3 : 1; }
-
-// the 256 x 256 tile once its grid covers most of the card, else the 128 x 128 tile, then splits of the reduction
-static bool gf_large(long M, long N, int cus) { return cdivl(M, 256) * cdivl(N, 256) >= cus / 2; }
+static long pad64(long n) { return (n + 63) / 64 * 64; }
 static int gf_cus() {
     static thread_local int cus = 0;
     if (!cus) {
@@ -327,99 +506,97 @@ static int gf_cus() {
     }
     return cus;
 }
-static int gf_splits(long M, long N, long iters, bool large) {
-    const long b = large ? 256 : 128, tiles = cdivl(M, b) * cdivl(N, b), want = 2L * gf_cus();
-    if (tiles >= gf_cus()) return 1;
-    long s = want / tiles;
+static bool gf_aligned(const refil_gated_ff_desc& d, const void* p, long ld) { return d.dtype != REFIL_F32 && ld % 8 == 0 && (uintptr_t)p % 16 == 0; }
+// global memory straight to LDS: 16-byte chunks that never leave their row (the forward's reduction also needs whole tiles of it)
+static bool gf_direct(const refil_gated_ff_desc& d, bool bwd) {
+    const bool a = gf_aligned(d, d.x, d.x_stride) && gf_aligned(d, d.w_gate, d.w_stride) && gf_aligned(d, d.w_up, d.w_stride);
+    return a && d.D % (bwd ? 8 : 64) == 0;
+}
+struct GfPlan { bool direct, large; int splits; };
+static GfPlan gf_plan(long M, long N, long K, int bk, bool direct) {
+    GfPlan p;
+    p.direct = direct;
+    p.large = direct && cdivl(M, 256) * cdivl(N, 256) >= gf_cus() / 2;
+    const long b = p.large ? 256 : 128, tiles = cdivl(M, b) * cdivl(N, b), iters = cdivl(K, bk);
+    long s = tiles >= gf_cus() ? 1 : 2L * gf_cus() / tiles;
     if (s > iters / 8) s = iters / 8;
     if (s > 64) s = 64;
-    return s < 1 ? 1 : (int)s;
+    p.splits = s < 1 ? 1 : (int)s;
+    return p;
 }
 
-template <class T, bool GATED>
-static int gf_launch(GfGemm k, bool large, hipStream_t st, const char* name, double flops, double bytes) {
-    typedef typename GfElem<T>::type E;
-    const int bm = large ? 256 : 128, half = (large ? 256 : 128) / (GATED ? 2 : 1);
-    const long tiles = cdivl(k.M, bm) * cdivl(k.N, half);
+template <class T, int LA, int LB, int WM, int WN, int MT, int NT, bool DIRECT, bool GATED>
+static int gf_go(const GfGemm& k, hipStream_t st) {
+    constexpr int BM = WM * MT * 16, BN = WN * NT * 16, HALF = GATED ? BN / 2 : BN;
+    constexpr size_t LDS = (size_t)(DIRECT ? 2 : GF_P<T>) * (GfTile<LA, BM, GF_BK<T>>::BYTES + GfTile<LB, BN, GF_BK<T>>::BYTES);
+    const long tiles = cdivl(k.M, BM) * cdivl(k.N, HALF);
     REFIL_CHECK(tiles < (1L << 31), "refil_gated_ff: too many tiles");
-    const size_t lds = (size_t)2 * (bm + bm) * 128;
-    ProfScope ps(name, flops, bytes, st, nullptr, 0.0, k.pairs > 1 ? flops : 0.0);
-    if (large) {
-        auto* f = gf_gemm<T, E, 2, 4, 8, 4, GATED>;
-        REFIL_HIP(hipFuncSetAttribute((const void*)f, (hipFuncAttribute)hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds));
-        hipLaunchKernelGGL(f, dim3(tiles, k.splits), dim3(512), lds, st, k);
-    } else {
-        auto* f = gf_gemm<T, E, 2, 2, 4, 4, GATED>;
-        REFIL_HIP(hipFuncSetAttribute((const void*)f, (hipFuncAttribute)hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds));
-        hipLaunchKernelGGL(f, dim3(tiles, k.splits), dim3(256), lds, st, k);
-    }
+    auto* f = gf_gemm<T, LA, LB, WM, WN, MT, NT, DIRECT, GATED>;
+    REFIL_HIP(hipFuncSetAttribute((const void*)f, (hipFuncAttribute)hipFuncAttributeMaxDynamicSharedMemorySize, (int)LDS));
+    hipLaunchKernelGGL(f, dim3((unsigned)tiles, k.splits), dim3(WM * WN * 64), LDS, st, k);
     REFIL_LAUNCH_CHECK();
     return 0;
 }
+template <class T, int LA, int LB, bool GATED>
+static int gf_launch(GfGemm k, const GfPlan& p, hipStream_t st, const char* name, double flops, double bytes) {
+    ProfScope ps(name, flops, bytes, st, nullptr, 0.0, sizeof(T) == 4 ? flops : 0.0);
+    k.splits = p.splits;
+    if constexpr (sizeof(T) == 2) {
+        if (p.large) return gf_go<T, LA, LB, 2, 4, 8, 4, true, GATED>(k, st);
+        if (p.direct) return gf_go<T, LA, LB, 2, 2, 4, 4, true, GATED>(k, st);
+    }
+    return gf_go<T, LA, LB, 2, 2, 4, 4, false, GATED>(k, st);
+}
 
-struct GfBump { char* p; size_t n; void* take(size_t b) { char* r = p ? p + n : nullptr; n += (b + 255) / 256 * 256; return r; } };
-struct GfFwdWs { void* x; void* wg; void* wu; size_t bytes; };
-static GfFwdWs gf_fwd_ws(const refil_gated_ff_desc& d, void* base) {
-    GfBump b{(char*)base, 0};
-    GfFwdWs w{};
-    const size_t es = 2 * gf_planes(d.dtype), Kp = pad64(d.D);
-    if (!gf_direct(d, d.x, d.x_stride)) w.x = b.take((size_t)d.N * Kp * es);
-    if (!gf_direct(d, d.w_gate, d.w_stride) || !gf_direct(d, d.w_up, d.w_stride)) { w.wg = b.take((size_t)d.F * Kp * es); w.wu = b.take((size_t)d.F * Kp * es); }
-    w.bytes = b.n;
-    return w;
-}
-struct GfBwdWs { void* rows; void* cols; void* wt; void* xt; float* colsum; float* part_w; float* part_x; int split_w, split_x; bool large_w, large_x; size_t bytes; };
-static GfBwdWs gf_bwd_ws(const refil_gated_ff_desc& d, void* base) {
-    GfBump b{(char*)base, 0};
-    GfBwdWs w{};
-    const size_t es = 2 * gf_planes(d.dtype), Fp = pad64(d.F), Np = pad64(d.N);
-    const int pairs = d.dtype == REFIL_F32 ? 6 : 1;
-    w.rows = b.take((size_t)d.N * 2 * Fp * es);
-    w.cols = b.take((size_t)2 * d.F * Np * es);
-    w.wt = b.take((size_t)d.D * 2 * Fp * es);
-    w.xt = b.take((size_t)d.D * Np * es);
-    w.colsum = (float*)b.take((size_t)cdivl(d.N, 64) * 2 * d.F * 4);
-    w.large_x = gf_large(d.N, d.D, gf_cus()); w.large_w = gf_large(2L * d.F, d.D, gf_cus());
-    w.split_x = gf_splits(d.N, d.D, (long)pairs * (2 * Fp / 64), w.large_x);
-    w.split_w = gf_splits(2L * d.F, d.D, (long)pairs * (Np / 64), w.large_w);
-    if (w.split_x > 1) w.part_x = (float*)b.take((size_t)w.split_x * d.N * d.D * 4);
-    if (w.split_w > 1) w.part_w = (float*)b.take((size_t)w.split_w * 2 * d.F * d.D * 4);
-    w.bytes = b.n;
-    return w;
-}
 static int gf_blocks(long n) { const long b = cdivl(n, 256 * 4); return (int)(b < 1 ? 1 : b > 8192 ? 8192 : b); }
+struct GfBwdWs { void* grad; float* colsum; float* part; long Fp, Np; GfPlan px, pw; int row_blocks, per; size_t bytes; };
+static GfBwdWs gf_bwd_ws(const refil_gated_ff_desc& d, void* base) {
+    char* const p = (char*)base; size_t n = 0;
+    auto take = [&](size_t b) { char* r = p ? p + n : nullptr; n += (b + 255) / 256 * 256; return (void*)r; };
+    GfBwdWs w{};
+    const int bk = d.dtype == REFIL_F32 ? 32 : 64;
+    const bool direct = gf_direct(d, true);
+    w.Fp = pad64(d.F); w.Np = pad64(d.N);
+    w.grad = take((size_t)w.Np * 2 * w.Fp * (d.dtype == REFIL_F32 ? 4 : 2));
+    w.per = (int)(w.Np / 256 > 64 ? pad64(cdivl(w.Np, 256)) : 64);
+    w.row_blocks = (int)cdivl(w.Np, w.per);
+    w.colsum = (float*)take((size_t)w.row_blocks * 2 * d.F * 4);
+    w.px = gf_plan(d.N, d.D, 2 * w.Fp, bk, direct);
+    w.pw = gf_plan(2 * w.Fp, d.D, w.Np, bk, direct);
+    const size_t a = w.px.splits > 1 ? (size_t)w.px.splits * d.N * d.D : 0, b = w.pw.splits > 1 ? (size_t)w.pw.splits * 2 * w.Fp * d.D : 0;
+    w.part = (float*)take(4 * (a > b ? a : b));
+    w.bytes = n;
+    return w;
+}
 
 template <class T>
 static int gf_forward(const refil_gated_ff_desc& d, hipStream_t st) {
-    const GfFwdWs w = gf_fwd_ws(d, d.workspace);
-    const int Kp = pad64(d.D);
     GfGemm k{};
-    k.pairs = GfElem<T>::planes == 3 ? 6 : 1;
-    k.M = (int)d.N; k.N = d.F; k.K = Kp; k.splits = 1;
-    k.A = d.x; k.lda = d.x_stride; k.B0 = d.w_gate; k.B1 = d.w_up; k.ldb = d.w_stride;
-    if (w.x) {
-        hipLaunchKernelGGL((gf_pack<T>), dim3(gf_blocks(d.N * Kp)), dim3(256), 0, st, d.x, (long)d.x_stride, (long)d.N, d.D, Kp, w.x, (long)Kp, (long)d.N * Kp);
+    k.A = d.x; k.lda = d.x_stride; k.B0 = d.w_gate; k.B1 = d.w_up; k.ldb = d.w_stride; k.M = (int)d.N; k.N = d.F; k.K = d.D; k.ksplit = 1 << 30; k.splits = 1;
+    k.a_rows = k.M; k.b_rows = k.N;
+    k.C0 = d.h; k.ldc = d.h_stride; k.bias0 = d.b_gate; k.bias1 = d.b_up; k.act = d.act;
+    k.save0 = d.saved; k.save1 = d.saved ? d.saved + d.N * d.F : nullptr;
+    const double nf = (double)d.N * d.F, fl = 4 * nf * d.D, by = sizeof(T) * ((double)d.N * d.D + 2.0 * d.F * d.D + nf) + (d.saved ? 8 * nf : 0);
+    if (d.N <= 64) {
+        ProfScope ps("gated_ff_few_rows", fl, by, st, nullptr, 0.0, sizeof(T) == 4 ? fl : 0.0);
+        const dim3 grid(cdiv(d.F, 16));
+        if (d.N <= 16) hipLaunchKernelGGL((gf_skinny<T, 1>), grid, dim3(512), 0, st, k);
+        else if (d.N <= 32) hipLaunchKernelGGL((gf_skinny<T, 2>), grid, dim3(512), 0, st, k);
+        else hipLaunchKernelGGL((gf_skinny<T, 4>), grid, dim3(512), 0, st, k);
         REFIL_LAUNCH_CHECK();
-        k.A = w.x; k.lda = Kp; k.planeA = (long)d.N * Kp;
+        return 0;
     }
-    if (w.wg) {
-        hipLaunchKernelGGL((gf_pack<T>), dim3(gf_blocks((long)d.F * Kp)), dim3(256), 0, st, d.w_gate, (long)d.w_stride, (long)d.F, d.D, Kp, w.wg, (long)Kp, (long)d.F * Kp);
-        REFIL_LAUNCH_CHECK();
-        hipLaunchKernelGGL((gf_pack<T>), dim3(gf_blocks((long)d.F * Kp)), dim3(256), 0, st, d.w_up, (long)d.w_stride, (long)d.F, d.D, Kp, w.wu, (long)Kp, (long)d.F * Kp);
-        REFIL_LAUNCH_CHECK();
-        k.B0 = w.wg; k.B1 = w.wu; k.ldb = Kp; k.planeB = (long)d.F * Kp;
-    }
-    k.C0 = d.h; k.ldc = d.h_stride; k.msplit = k.M; k.bias0 = d.b_gate; k.bias1 = d.b_up; k.act = d.act;
-    k.save0 = d.saved; k.save1 = d.saved ? (T*)d.saved + d.N * d.F : nullptr;
-    const double es = sizeof(T), fl = 4.0 * d.N * d.D * d.F;
-    return gf_launch<T, true>(k, gf_large(d.N, 2L * d.F, gf_cus()), st, "gated_ff_fwd", fl, es * ((double)d.N * d.D + 2.0 * d.F * d.D + (d.saved ? 3.0 : 1.0) * d.N * d.F));
+    GfPlan p = gf_plan(d.N, 2L * d.F, d.D, GF_BK<T>, gf_direct(d, false));
+    p.splits = 1;
+    return gf_launch<T, GF_K, GF_K, true>(k, p, st, "gated_ff_fwd", fl, by);
 }
-template <class T>
-static int gf_product(GfGemm k, bool large, float* part, hipStream_t st, const char* name, double fl, double bytes) {
+template <class T, int LA>
+static int gf_product(GfGemm k, const GfPlan& p, float* part, hipStream_t st, const char* name, double fl, double bytes) {
     k.partial = part;
-    if (int rc = gf_launch<T, false>(k, large, st, name, fl, bytes)) return rc;
-    if (k.splits > 1) {
-        hipLaunchKernelGGL((gf_reduce<T>), dim3(gf_blocks((long)k.M * k.N)), dim3(256), 0, st, (const float*)part, k.splits, k.M, k.N, k.C0, k.C1, k.ldc, k.msplit);
+    k.splits = p.splits;
+    if (int rc = gf_launch<T, LA, GF_M, false>(k, p, st, name, fl, bytes)) return rc;
+    if (p.splits > 1) {
+        hipLaunchKernelGGL((gf_reduce<T>), dim3(gf_blocks((long)k.M * k.N)), dim3(256), 0, st, k);
         REFIL_LAUNCH_CHECK();
     }
     return 0;
@@ -427,36 +604,26 @@ static int gf_product(GfGemm k, bool large, float* part, hipStream_t st, const c
 template <class T>
 static int gf_backward(const refil_gated_ff_desc& d, hipStream_t st) {
     const GfBwdWs w = gf_bwd_ws(d, d.workspace);
-    const int Fp = pad64(d.F), Np = pad64(d.N), pairs = GfElem<T>::planes == 3 ? 6 : 1;
     const double es = sizeof(T), nf = (double)d.N * d.F;
     GfGrad g{};
-    g.sg = d.saved; g.su = (const T*)d.saved + d.N * d.F; g.dh = d.dh; g.dh_s = d.dh_stride; g.N = d.N; g.F = d.F; g.act = d.act;
-    g.rows = w.rows; g.ldr = 2L * Fp; g.plane_r = (long)d.N * 2 * Fp; g.Fp = Fp; g.cols = w.cols; g.ldc = Np; g.plane_c = 2L * d.F * Np; g.Np = Np;
-    g.colsum = (d.db_gate || d.db_up) ? w.colsum : nullptr;
+    g.sg = d.saved; g.su = d.saved + d.N * d.F; g.dh = d.dh; g.dh_s = d.dh_stride; g.N = d.N; g.rows_out = w.Np; g.F = d.F; g.Fp = (int)w.Fp; g.act = d.act;
+    g.out = w.grad; g.ldo = 2 * w.Fp; g.colsum = (d.db_gate || d.db_up) ? w.colsum : nullptr; g.per = w.per;
     {
-        ProfScope ps("gated_ff_grad", 20 * nf, (3 + 4) * nf * es, st);
-        hipLaunchKernelGGL((gf_grad<T>), dim3(Np / 64, Fp / 64), dim3(256), 0, st, g);
+        ProfScope ps("gated_ff_grad", 20 * nf, nf * (8 + 3 * es), st);
+        hipLaunchKernelGGL((gf_grad<T>), dim3(w.row_blocks, cdiv(w.Fp, 32 * VEC_OF<T>)), dim3(256), 0, st, g);
         REFIL_LAUNCH_CHECK();
     }
     if (g.colsum) {
-        hipLaunchKernelGGL((gf_bias<T>), dim3(cdiv(2 * d.F, 64)), dim3(256), 0, st, (const float*)w.colsum, (long)(Np / 64), d.F, d.db_gate, d.db_up);
+        hipLaunchKernelGGL((gf_bias<T>), dim3(cdiv(2 * d.F, 64)), dim3(1024), 0, st, (const float*)w.colsum, w.row_blocks, d.F, d.db_gate, d.db_up);
         REFIL_LAUNCH_CHECK();
     }
-    typedef typename GfElem<T>::type E;
-    hipLaunchKernelGGL((gf_transpose<T>), dim3(Fp / 64, cdiv(d.D, 64)), dim3(256), 0, st, d.w_gate, (long)d.w_stride, (long)d.F, d.D, (long)Fp, w.wt, 2L * Fp, (long)d.D * 2 * Fp);
-    REFIL_LAUNCH_CHECK();
-    hipLaunchKernelGGL((gf_transpose<T>), dim3(Fp / 64, cdiv(d.D, 64)), dim3(256), 0, st, d.w_up, (long)d.w_stride, (long)d.F, d.D, (long)Fp, (void*)((E*)w.wt + Fp), 2L * Fp, (long)d.D * 2 * Fp);
-    REFIL_LAUNCH_CHECK();
-    hipLaunchKernelGGL((gf_transpose<T>), dim3(Np / 64, cdiv(d.D, 64)), dim3(256), 0, st, d.x, (long)d.x_stride, (long)d.N, d.D, (long)Np, w.xt, (long)Np, (long)d.D * Np);
-    REFIL_LAUNCH_CHECK();
     GfGemm k{};
-    k.pairs = pairs;
-    k.A = w.rows; k.lda = 2L * Fp; k.planeA = (long)d.N * 2 * Fp; k.B0 = w.wt; k.ldb = 2L * Fp; k.planeB = (long)d.D * 2 * Fp;
-    k.M = (int)d.N; k.N = d.D; k.K = 2 * Fp; k.splits = w.split_x; k.C0 = d.dx; k.ldc = d.dx_stride; k.msplit = k.M;
-    if (int rc = gf_product<T>(k, w.large_x, w.part_x, st, "gated_ff_dx", 4.0 * nf * d.D, es * (2 * nf + 2.0 * d.F * d.D + (double)d.N * d.D))) return rc;
-    k.A = w.cols; k.lda = Np; k.planeA = 2L * d.F * Np; k.B0 = w.xt; k.ldb = Np; k.planeB = (long)d.D * Np;
-    k.M = 2 * d.F; k.N = d.D; k.K = Np; k.splits = w.split_w; k.C0 = d.dw_gate; k.C1 = d.dw_up; k.ldc = d.D; k.msplit = d.F;
-    return gf_product<T>(k, w.large_w, w.part_w, st, "gated_ff_dw", 4.0 * nf * d.D, es * (2 * nf + 2.0 * d.F * d.D + (double)d.N * d.D));
+    k.A = w.grad; k.lda = 2 * w.Fp; k.B0 = d.w_gate; k.B1 = d.w_up; k.ldb = d.w_stride; k.ksplit = (int)w.Fp;
+    k.M = (int)d.N; k.N = d.D; k.K = (int)(2 * w.Fp); k.a_rows = k.M; k.b_rows = d.F; k.C0 = d.dx; k.ldc = d.dx_stride; k.msplit = k.mlim = k.M;
+    if (int rc = gf_product<T, GF_K>(k, w.px, w.part, st, "gated_ff_dx", 4.0 * nf * d.D, es * (2 * nf + 2.0 * d.F * d.D + (double)d.N * d.D))) return rc;
+    k.B0 = d.x; k.ldb = d.x_stride; k.ksplit = 1 << 30;
+    k.M = (int)(2 * w.Fp); k.N = d.D; k.K = (int)w.Np; k.a_rows = (int)w.Np; k.b_rows = (int)d.N; k.C0 = d.dw_gate; k.C1 = d.dw_up; k.ldc = d.D; k.msplit = (int)w.Fp; k.mlim = d.F;
+    return gf_product<T, GF_M>(k, w.pw, w.part, st, "gated_ff_dw", 4.0 * nf * d.D, es * (2 * nf + 2.0 * d.F * d.D + (double)d.N * d.D));
 }
 static int gf_check(const refil_gated_ff_desc& d, const char* who) {
     REFIL_CHECK(d.dtype >= REFIL_F32 && d.dtype <= REFIL_F16, "%s: dtype %d is none of REFIL_F32 / REFIL_BF16 / REFIL_F16", who, d.dtype);
@@ -473,15 +640,13 @@ using namespace refil;
 
 extern "C" size_t refil_gated_ff_workspace_bytes(const refil_gated_ff_desc* d, int32_t backward) {
     if (!d || gf_check(*d, "refil_gated_ff_workspace_bytes")) return 0;
-    return backward ? gf_bwd_ws(*d, nullptr).bytes : gf_fwd_ws(*d, nullptr).bytes;
+    return backward ? gf_bwd_ws(*d, nullptr).bytes : 0;
 }
 extern "C" int refil_gated_ff_forward(const refil_gated_ff_desc* d, void* stream) {
     REFIL_CHECK(d, "refil_gated_ff_forward: null desc");
     if (int rc = gf_check(*d, "refil_gated_ff_forward")) return rc;
     if (!d->N) return 0;
     REFIL_CHECK(d->x && d->w_gate && d->w_up && d->h, "refil_gated_ff_forward: x, w_gate, w_up and h are required");
-    const size_t need = refil_gated_ff_workspace_bytes(d, 0);
-    REFIL_CHECK(!need || (d->workspace && d->workspace_bytes >= need), "refil_gated_ff_forward: workspace of %zu bytes, %zu needed", d->workspace_bytes, need);
     hipStream_t st = (hipStream_t)stream;
     return d->dtype == REFIL_F32 ? gf_forward<float>(*d, st) : d->dtype == REFIL_BF16 ? gf_forward<bf16_t>(*d, st) : gf_forward<f16_t>(*d, st);
 }

@@ -273,6 +273,17 @@ __attribute__((always_inline)) static inline v4f mfma_16x16x32_f16(v8h a, v8h b,
     }
     return c;
 }
+typedef short v4s __attribute__((ext_vector_type(4)));
+// ds_read_b64_tr_b16: lane i of a 16-lane group reads 4 elements at its address and receives, as element j, element i & 3 of lane (i >> 2) + 4 j
+__attribute__((always_inline)) static inline v4s ds_read_tr16_b64(const void* p) {
+    v4s mine;
+    memcpy(&mine, p, 8);
+    const Xchg e = xchg(&mine, 8);
+    const int l = lane_ids().lane, g = l & ~15, i = l & 15;
+    v4s r;
+    for (int j = 0; j < 4; ++j) r[j] = lane_get<v4s>(e, g + (i >> 2) + 4 * j)[i & 3];
+    return r;
+}
 // global_load_lds_dwordx4: lane l's 16 bytes land at (wave-uniform base) + 16 l. (Immediate here: the wait in front of the read is not modelled.)
 static inline void global_load_lds(const void* g, void* lds, int bytes, int off, int) {
     memcpy(static_cast<char*>(lds) + off + bytes * lane_ids().lane, g, bytes);
@@ -356,6 +367,7 @@ static inline void raw_buffer_store_b128(V v, rsrc rs, int voff, int soff, int) 
 #define __builtin_amdgcn_mfma_f32_16x16x32_bf16 emu::mfma_16x16x32_bf16
 #define __builtin_amdgcn_mfma_f32_32x32x16_bf16 emu::mfma_32x32x16_bf16
 #define __builtin_amdgcn_mfma_f32_16x16x32_f16 emu::mfma_16x16x32_f16
+#define __builtin_amdgcn_ds_read_tr16_b64_v4i16 emu::ds_read_tr16_b64
 #define __builtin_amdgcn_global_load_lds emu::global_load_lds
 #define __builtin_amdgcn_readfirstlane emu::readfirstlane
 #define __builtin_amdgcn_readlane emu::readlane

@@ -538,6 +538,22 @@ def test_gated_ff_matches_the_definition(N, D, F, act, bias, dtype):
     ff_check(x, wg, wu, bg, bu, act)
 
 
+@pytest.mark.parametrize("dtype", [BF16, F16])
+def test_gated_ff_large_tiles(dtype):
+    """enough tiles for the 256 x 256 variant of every product, ragged in rows and columns (fewer compute units on the emulator, fewer tiles)"""
+    N, D, F = (2060, 2056, 2052) if DEV == "cuda" else (520, 264, 300)
+    K = 64
+    x, wg, wu = rnd(N, K, seed=1, dtype=dtype), rnd(F, K, seed=2, dtype=dtype, scale=0.1), rnd(F, K, seed=3, dtype=dtype, scale=0.1)
+    h, _ = blocks.gated_ff_forward(x, wg, wu)
+    close("h", h, *ff_ref(x, wg, wu, None, None, "silu")["h"])
+    F = 72                                                          # dx: N x D
+    x, wg, wu = rnd(N, D, seed=4, dtype=dtype), rnd(F, D, seed=5, dtype=dtype, scale=0.02), rnd(F, D, seed=6, dtype=dtype, scale=0.02)
+    ff_check(x, wg, wu, None, None, "gelu")
+    N, F = 70, (1030 if DEV == "cuda" else 260)                    # dw: 2 F x D
+    x, wg, wu = rnd(N, D, seed=7, dtype=dtype), rnd(F, D, seed=8, dtype=dtype, scale=0.02), rnd(F, D, seed=9, dtype=dtype, scale=0.02)
+    ff_check(x, wg, wu, rnd(F, seed=10, dtype=dtype), rnd(F, seed=11, dtype=dtype), "silu")
+
+
 def test_gated_ff_shapes_and_strides():
     """agents' rows [B, T, na, D] cut out of wider rows, both weights in one fused matrix with padding, one bias alone, rows expanded over one"""
     D, F = 24, 20
