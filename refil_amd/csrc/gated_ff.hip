@@ -84,10 +84,14 @@ template <class T> constexpr int GF_BK = sizeof(T) == 4 ? 32 : 64;
 template <class T> struct GfElem { typedef T type; };
 template <> struct GfElem<float> { typedef bf16_t type; };
 
-__device__ __forceinline__ void gf_copy16(const void* g, void* lds) {
-    // 64 lanes x 16 bytes of global memory to 1 KB of LDS behind `lds` (wave-uniform), lane order
-    __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)g, (__attribute__((address_space(3))) void*)lds, 16, 0, 0);
+// 64 lanes x 16 bytes of global memory to the 1 KB of LDS behind byte `lds` (wave-uniform), lane order. Inline assembly because the compiler,
+// which knows the builtin as a write to LDS, waits for it in front of every transposing read, of the other tile too; nothing but the copy's
+// own wait (gf_copies_done, in front of the barrier that hands the tile over) orders it. It has no result registers.
+__device__ __forceinline__ void gf_copy16(const void* g, unsigned lds) {
+    asm volatile("s_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, off" : : "v"(g), "s"(lds) : "memory", "m0");
 }
+__device__ __forceinline__ void gf_copies_done() { asm volatile("s_waitcnt vmcnt(0)" : : : "memory"); }
+__device__ __forceinline__ unsigned gf_lds_byte(const char* p) { return (unsigned)(size_t)(const __attribute__((address_space(3))) char*)p; }
 typedef short gf_s16x4 __attribute__((ext_vector_type(4)));
 // four rows of k, 16 columns: lane i of a 16-lane group supplies columns 4 (i & 3) .. of row i >> 2 and receives column i of the four rows
 __device__ __forceinline__ uint2 gf_read_tr(const char* p) {
@@ -164,9 +168,9 @@ __global__ void __launch_bounds__(WM * WN * 64, DIRECT ? 1 : 2) gf_gemm(const Gf
 #pragma unroll
             for (int p = 0; p < P; ++p) {
 #pragma unroll
-                for (int i = 0; i < MT; ++i) fa[p][i] = TA::frag(a + p * TA::BYTES, wm * MT + i, kk, lane);
-#pragma unroll
                 for (int j = 0; j < NT; ++j) fb[p][j] = TB::frag(b + p * TB::BYTES, wn * NT + j, kk, lane);
+#pragma unroll
+                for (int i = 0; i < MT; ++i) fa[p][i] = TA::frag(a + p * TA::BYTES, wm * MT + i, kk, lane);
             }
             // D rows = n, columns = m: a lane holds 4 neighbouring n of one m
 #pragma unroll
@@ -183,10 +187,22 @@ __global__ void __launch_bounds__(WM * WN * 64, DIRECT ? 1 : 2) gf_gemm(const Gf
                     acc[i][j] = gf_mfma<E>(fb[0][j], fa[0][i], acc[i][j]);
                 }
         }
+        if constexpr (DIRECT) {
+            // the order of issue: B's fragments and two of A's in front, then the other reads (the second half's among them) a few matrix
+            // instructions ahead of their use, so that no product waits for the LDS
+            constexpr int RA = LA == GF_K ? 1 : 2, RB = LB == GF_K ? 1 : 2, FIRST = NT * RB + 2 * RA, REST = 2 * (MT * RA + NT * RB) - FIRST, STEPS = 2 * MT - 2;
+            __builtin_amdgcn_sched_group_barrier(0x100, FIRST, 0);
+            static_for<2 * MT>([&](auto sc) {
+                constexpr int s = decltype(sc)::value;
+                __builtin_amdgcn_sched_group_barrier(0x008, NT, 0);
+                if constexpr (s < STEPS) __builtin_amdgcn_sched_group_barrier(0x100, (s + 1) * REST / STEPS - s * REST / STEPS, 0);
+            });
+        }
     };
 
     if constexpr (DIRECT) {
         char* const sa = gf_smem; char* const sb = gf_smem + 2 * TA::BYTES;
+        const unsigned la = gf_lds_byte(sa), lb = gf_lds_byte(sb);
         const T* pa[A_IT]; const T* pb[B_IT]; int ob[B_IT];      // (ob: a column of B, whose rows change hands at ksplit)
 #pragma unroll
         for (int i = 0; i < A_IT; ++i) {
@@ -208,7 +224,7 @@ __global__ void __launch_bounds__(WM * WN * 64, DIRECT ? 1 : 2) gf_gemm(const Gf
             for (int i = 0; i < A_IT; ++i) {
                 const int r = ((i * WAVES + wave) * 64 + lane) / TA::CH;
                 const T* p = LA == GF_K ? pa[i] + k0 : pa[i] + (long)min(k0 + r, k.a_rows - 1) * k.lda;
-                gf_copy16(p, sa + buf * TA::BYTES + (i * WAVES + wave) * 1024);
+                gf_copy16(p, la + buf * TA::BYTES + (i * WAVES + wave) * 1024);
             }
             const T* src = (const T*)k.B0; int kb = k0;
             if (LB == GF_M && k0 >= k.ksplit) { src = (const T*)k.B1; kb -= k.ksplit; }
@@ -216,16 +232,18 @@ __global__ void __launch_bounds__(WM * WN * 64, DIRECT ? 1 : 2) gf_gemm(const Gf
             for (int i = 0; i < B_IT; ++i) {
                 const int r = ((i * WAVES + wave) * 64 + lane) / TB::CH;
                 const T* p = LB == GF_K ? pb[i] + k0 : src + ob[i] + (long)min(kb + r, k.b_rows - 1) * k.ldb;
-                gf_copy16(p, sb + buf * TB::BYTES + (i * WAVES + wave) * 1024);
+                gf_copy16(p, lb + buf * TB::BYTES + (i * WAVES + wave) * 1024);
             }
         };
         if (it0 < it1) stage(it0, 0);
-        __syncthreads();                    // (also waits for the copies)
+        gf_copies_done();
+        lds_barrier();
         for (int it = it0; it < it1; ++it) {
             const int buf = (it - it0) & 1;
             if (it + 1 < it1) stage(it + 1, buf ^ 1);
             products(sa + buf * TA::BYTES, sb + buf * TB::BYTES);
-            __syncthreads();
+            gf_copies_done();
+            lds_barrier();
         }
     } else {
         char* const sa = gf_smem; char* const sb = gf_smem + P * TA::BYTES;

@@ -116,6 +116,10 @@ def _asm_to_c(body, where):
         return f"{outs[0]} = {ins[0]} - {ins[1]};"
     if re.fullmatch(r"s_waitcnt lgkmcnt\(0\)\s*s_barrier", t):
         return "emu::block_sync();"
+    if re.fullmatch(r"s_mov_b32 m0, %1\s+s_nop 0\s+global_load_lds_dwordx4 %0, off", t) and len(ins) == 2:
+        return f"emu::global_load_lds_byte({ins[0]}, {ins[1]});"
+    if t == "s_waitcnt vmcnt(0)":
+        return "(void)emu::xchg(nullptr, 0);"
     raise ValueError(f"{where}: inline asm template not known to the emulator build: {template!r}")
 
 

@@ -288,6 +288,11 @@ __attribute__((always_inline)) static inline v4s ds_read_tr16_b64(const void* p)
 static inline void global_load_lds(const void* g, void* lds, int bytes, int off, int) {
     memcpy(static_cast<char*>(lds) + off + bytes * lane_ids().lane, g, bytes);
 }
+// (the same with the LDS byte address as the instruction takes it: the low half of the host address of the dynamic allocation's byte)
+static inline void global_load_lds_byte(const void* g, unsigned byte) {
+    char* const base = static_cast<char*>(dyn_smem());
+    memcpy(base + (unsigned)(byte - (unsigned)(uintptr_t)base) + 16 * lane_ids().lane, g, 16);
+}
 static inline float bf(const unsigned char* p, int e) {
     unsigned short h; memcpy(&h, p + 2 * e, 2);
     return __uint_as_float((unsigned)h << 16);
