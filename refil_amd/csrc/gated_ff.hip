@@ -92,6 +92,7 @@ __device__ __forceinline__ void gf_copy16(const void* g, unsigned lds) {
 }
 __device__ __forceinline__ void gf_copies_done() { asm volatile("s_waitcnt vmcnt(0)" : : : "memory"); }
 __device__ __forceinline__ unsigned gf_lds_byte(const char* p) { return (unsigned)(size_t)(const __attribute__((address_space(3))) char*)p; }
+static __device__ unsigned gf_zeros[4];        // 16 bytes of zeros that a copy can fetch
 typedef short gf_s16x4 __attribute__((ext_vector_type(4)));
 // four rows of k, 16 columns: lane i of a 16-lane group supplies columns 4 (i & 3) .. of row i >> 2 and receives column i of the four rows
 __device__ __forceinline__ uint2 gf_read_tr(const char* p) {
@@ -122,7 +123,7 @@ template <int LAY, int DIM, int BK> struct GfTile {
 // products of this one. Otherwise (fp32; odd widths, strides or addresses) it goes through registers -- any alignment, ragged ends filled
 // with zeros, fp32 split into its planes -- into one LDS tile, the next one in flight in registers.
 template <class T, int LA, int LB, int WM, int WN, int MT, int NT, bool DIRECT, bool GATED>
-__global__ void __launch_bounds__(WM * WN * 64, DIRECT ? 1 : 2) gf_gemm(const GfGemm k) {
+__global__ void __launch_bounds__(WM * WN * 64, WM * MT == 16 || sizeof(T) == 4 ? 2 : 3) gf_gemm(const GfGemm k) {
     typedef typename GfElem<T>::type E;
     constexpr int P = GF_P<T>, BK = GF_BK<T>, WAVES = WM * WN, THREADS = WAVES * 64, BM = WM * MT * 16, BN = WN * NT * 16, HALF = GATED ? BN / 2 : BN;
     typedef GfTile<LA, BM, BK> TA;
@@ -132,10 +133,10 @@ __global__ void __launch_bounds__(WM * WN * 64, DIRECT ? 1 : 2) gf_gemm(const Gf
     extern __shared__ __attribute__((aligned(16))) char gf_smem[];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
     const int wm = wave / WN, wn = wave % WN;
-    const int mt = cdiv(k.M, BM), nt = cdiv(k.N, HALF);
-    // consecutive workgroups land on different XCDs (8 of them): give each XCD a contiguous run of tiles, in panels of 8 rows, so that its
-    // L2 holds the panels it reads
-    const int total = mt * nt;
+    const int mt = cdiv(k.M, BM), nt = cdiv(k.N, HALF), total = mt * nt;
+    // Consecutive workgroups land on different XCDs (8 of them): each XCD gets a contiguous run of tiles, in panels of 8 rows, so that its
+    // L2 holds the panels it reads. (One tile per workgroup: walking several with the next one's first block in flight under the outputs
+    // measured 517 against 463 us for dx of N 8192, D 2048, F 8192, and no gain elsewhere.)
     int id = blockIdx.x;
     {
         const int per = total / 8, rem = total % 8, xcd = id % 8, pos = id / 8;
@@ -164,28 +165,29 @@ __global__ void __launch_bounds__(WM * WN * 64, DIRECT ? 1 : 2) gf_gemm(const Gf
     auto products = [&](const char* a, const char* b) {
 #pragma unroll
         for (int kk = 0; kk < BK / 32; ++kk) {
-            gf_u32x4 fa[P][MT], fb[P][NT];
+            gf_u32x4 fb[P][NT];
 #pragma unroll
-            for (int p = 0; p < P; ++p) {
+            for (int p = 0; p < P; ++p)
 #pragma unroll
                 for (int j = 0; j < NT; ++j) fb[p][j] = TB::frag(b + p * TB::BYTES, wn * NT + j, kk, lane);
-#pragma unroll
-                for (int i = 0; i < MT; ++i) fa[p][i] = TA::frag(a + p * TA::BYTES, wm * MT + i, kk, lane);
-            }
             // D rows = n, columns = m: a lane holds 4 neighbouring n of one m
 #pragma unroll
-            for (int i = 0; i < MT; ++i)
+            for (int i = 0; i < MT; ++i) {
+                gf_u32x4 fa[P];
+#pragma unroll
+                for (int p = 0; p < P; ++p) fa[p] = TA::frag(a + p * TA::BYTES, wm * MT + i, kk, lane);
 #pragma unroll
                 for (int j = 0; j < NT; ++j) {
                     if constexpr (P == 3) {
-                        acc[i][j] = gf_mfma<E>(fb[0][j], fa[P - 1][i], acc[i][j]);
-                        acc[i][j] = gf_mfma<E>(fb[P - 1][j], fa[0][i], acc[i][j]);
-                        acc[i][j] = gf_mfma<E>(fb[P / 2][j], fa[P / 2][i], acc[i][j]);
-                        acc[i][j] = gf_mfma<E>(fb[0][j], fa[P / 2][i], acc[i][j]);
-                        acc[i][j] = gf_mfma<E>(fb[P / 2][j], fa[0][i], acc[i][j]);
+                        acc[i][j] = gf_mfma<E>(fb[0][j], fa[P - 1], acc[i][j]);
+                        acc[i][j] = gf_mfma<E>(fb[P - 1][j], fa[0], acc[i][j]);
+                        acc[i][j] = gf_mfma<E>(fb[P / 2][j], fa[P / 2], acc[i][j]);
+                        acc[i][j] = gf_mfma<E>(fb[0][j], fa[P / 2], acc[i][j]);
+                        acc[i][j] = gf_mfma<E>(fb[P / 2][j], fa[0], acc[i][j]);
                     }
-                    acc[i][j] = gf_mfma<E>(fb[0][j], fa[0][i], acc[i][j]);
+                    acc[i][j] = gf_mfma<E>(fb[0][j], fa[0], acc[i][j]);
                 }
+            }
         }
         if constexpr (DIRECT) {
             // the order of issue: B's fragments and two of A's in front, then the other reads (the second half's among them) a few matrix
@@ -220,18 +222,21 @@ __global__ void __launch_bounds__(WM * WN * 64, DIRECT ? 1 : 2) gf_gemm(const Gf
         }
         auto stage = [&](int it, int buf) {
             const int k0 = it * BK;
+            const bool tail = k0 + BK > k.K;                  // (GF_K operands: chunks behind K are zeros of their own; wave-uniform)
 #pragma unroll
             for (int i = 0; i < A_IT; ++i) {
-                const int r = ((i * WAVES + wave) * 64 + lane) / TA::CH;
+                const int e = (i * WAVES + wave) * 64 + lane, r = e / TA::CH;
                 const T* p = LA == GF_K ? pa[i] + k0 : pa[i] + (long)min(k0 + r, k.a_rows - 1) * k.lda;
+                if (LA == GF_K && tail && k0 + ((e % TA::CH) ^ TA::swz(r)) * 8 >= k.K) p = (const T*)gf_zeros;
                 gf_copy16(p, la + buf * TA::BYTES + (i * WAVES + wave) * 1024);
             }
             const T* src = (const T*)k.B0; int kb = k0;
             if (LB == GF_M && k0 >= k.ksplit) { src = (const T*)k.B1; kb -= k.ksplit; }
 #pragma unroll
             for (int i = 0; i < B_IT; ++i) {
-                const int r = ((i * WAVES + wave) * 64 + lane) / TB::CH;
+                const int e = (i * WAVES + wave) * 64 + lane, r = e / TB::CH;
                 const T* p = LB == GF_K ? pb[i] + k0 : src + ob[i] + (long)min(kb + r, k.b_rows - 1) * k.ldb;
+                if (LB == GF_K && tail && k0 + ((e % TB::CH) ^ TB::swz(r)) * 8 >= k.K) p = (const T*)gf_zeros;
                 gf_copy16(p, lb + buf * TB::BYTES + (i * WAVES + wave) * 1024);
             }
         };
@@ -332,26 +337,28 @@ __global__ void __launch_bounds__(WM * WN * 64, DIRECT ? 1 : 2) gf_gemm(const Gf
     }
 }
 
-// sums of the split products, in split order
+// sums of the split products, in split order; a thread takes four columns of a row
 template <class T>
 __global__ void __launch_bounds__(256) gf_reduce(const GfGemm k) {
-    const long n = (long)k.M * k.N;
-    for (long e = (long)blockIdx.x * 256 + threadIdx.x; e < n; e += (long)gridDim.x * 256) {
-        const int m = (int)(e / k.N), c = (int)(e - (long)m * k.N);
+    const unsigned q = (unsigned)cdiv(k.N, 4), n = (unsigned)k.M * q;          // (fewer tiles than compute units: far below 2^32)
+    const long plane = (long)k.M * k.N;
+    for (unsigned e = blockIdx.x * 256 + threadIdx.x; e < n; e += gridDim.x * 256) {
+        const int m = (int)(e / q), c0 = (int)(e - (unsigned)m * q) * 4, c = min(k.N - c0, 4);
         const bool first = m < k.msplit;
         const int row = first ? m : m - k.msplit;
         if (row >= k.mlim) continue;
-        float s = 0.f;
-        int p = 0;
-        for (; p + 8 <= k.splits; p += 8) {
-            float v[8];
+        const float* p = k.partial + (long)m * k.N + c0;
+        float s[4] = {0.f, 0.f, 0.f, 0.f};
+        for (int z = 0; z < k.splits; z += 8) {
+            Raw<float> v[8];
 #pragma unroll
-            for (int j = 0; j < 8; ++j) v[j] = k.partial[(p + j) * n + e];
+            for (int j = 0; j < 8; ++j) v[j] = ld_raw<float>(p + min(z + j, k.splits - 1) * plane, c);
 #pragma unroll
-            for (int j = 0; j < 8; ++j) s += v[j];
+            for (int j = 0; j < 8; ++j)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) s[i] += z + j < k.splits ? raw_get(v[j], i) : 0.f;
         }
-        for (; p < k.splits; ++p) s += k.partial[p * n + e];
-        ((T*)(first ? k.C0 : k.C1))[(long)row * k.ldc + c] = from_f32<T>(s);
+        st_raw<T, 4>((T*)(first ? k.C0 : k.C1) + (long)row * k.ldc + c0, raw_pack<T, 4>(s), c);
     }
 }
 
@@ -525,10 +532,9 @@ static int gf_cus() {
     return cus;
 }
 static bool gf_aligned(const refil_gated_ff_desc& d, const void* p, long ld) { return d.dtype != REFIL_F32 && ld % 8 == 0 && (uintptr_t)p % 16 == 0; }
-// global memory straight to LDS: 16-byte chunks that never leave their row (the forward's reduction also needs whole tiles of it)
-static bool gf_direct(const refil_gated_ff_desc& d, bool bwd) {
-    const bool a = gf_aligned(d, d.x, d.x_stride) && gf_aligned(d, d.w_gate, d.w_stride) && gf_aligned(d, d.w_up, d.w_stride);
-    return a && d.D % (bwd ? 8 : 64) == 0;
+// global memory straight to LDS: 16-byte chunks that never leave their row
+static bool gf_direct(const refil_gated_ff_desc& d) {
+    return gf_aligned(d, d.x, d.x_stride) && gf_aligned(d, d.w_gate, d.w_stride) && gf_aligned(d, d.w_up, d.w_stride) && d.D % 8 == 0;
 }
 struct GfPlan { bool direct, large; int splits; };
 static GfPlan gf_plan(long M, long N, long K, int bk, bool direct) {
@@ -566,17 +572,17 @@ static int gf_launch(GfGemm k, const GfPlan& p, hipStream_t st, const char* name
     return gf_go<T, LA, LB, 2, 2, 4, 4, false, GATED>(k, st);
 }
 
-static int gf_blocks(long n) { const long b = cdivl(n, 256 * 4); return (int)(b < 1 ? 1 : b > 8192 ? 8192 : b); }
+static int gf_blocks(long n) { const long b = cdivl(n, 256); return (int)(b < 1 ? 1 : b > 8192 ? 8192 : b); }
 struct GfBwdWs { void* grad; float* colsum; float* part; long Fp, Np; GfPlan px, pw; int row_blocks, per; size_t bytes; };
 static GfBwdWs gf_bwd_ws(const refil_gated_ff_desc& d, void* base) {
     char* const p = (char*)base; size_t n = 0;
     auto take = [&](size_t b) { char* r = p ? p + n : nullptr; n += (b + 255) / 256 * 256; return (void*)r; };
     GfBwdWs w{};
     const int bk = d.dtype == REFIL_F32 ? 32 : 64;
-    const bool direct = gf_direct(d, true);
+    const bool direct = gf_direct(d);
     w.Fp = pad64(d.F); w.Np = pad64(d.N);
     w.grad = take((size_t)w.Np * 2 * w.Fp * (d.dtype == REFIL_F32 ? 4 : 2));
-    w.per = (int)(w.Np / 256 > 64 ? pad64(cdivl(w.Np, 256)) : 64);
+    w.per = (int)(cdivl(cdivl(w.Np, 256), 8) * 8);          // at most 256 partial rows of bias sums, whole rounds of 8 rows
     w.row_blocks = (int)cdivl(w.Np, w.per);
     w.colsum = (float*)take((size_t)w.row_blocks * 2 * d.F * 4);
     w.px = gf_plan(d.N, d.D, 2 * w.Fp, bk, direct);
@@ -604,7 +610,7 @@ static int gf_forward(const refil_gated_ff_desc& d, hipStream_t st) {
         REFIL_LAUNCH_CHECK();
         return 0;
     }
-    GfPlan p = gf_plan(d.N, 2L * d.F, d.D, GF_BK<T>, gf_direct(d, false));
+    GfPlan p = gf_plan(d.N, 2L * d.F, d.D, GF_BK<T>, gf_direct(d));
     p.splits = 1;
     return gf_launch<T, GF_K, GF_K, true>(k, p, st, "gated_ff_fwd", fl, by);
 }
@@ -614,7 +620,7 @@ static int gf_product(GfGemm k, const GfPlan& p, float* part, hipStream_t st, co
     k.splits = p.splits;
     if (int rc = gf_launch<T, LA, GF_M, false>(k, p, st, name, fl, bytes)) return rc;
     if (p.splits > 1) {
-        hipLaunchKernelGGL((gf_reduce<T>), dim3(gf_blocks((long)k.M * k.N)), dim3(256), 0, st, k);
+        hipLaunchKernelGGL((gf_reduce<T>), dim3(gf_blocks((long)k.M * k.N / 4)), dim3(256), 0, st, k);
         REFIL_LAUNCH_CHECK();
     }
     return 0;
