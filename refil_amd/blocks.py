@@ -286,8 +286,8 @@ def _norm_desc(who, x, o, gate, post_weight, res_scale, pre_weight, alpha, eps, 
             raise ValueError(f"{who}: a gate needs the block's output o")
         _like(gate, x, "gate", who)
     post_weight, res_scale, pre_weight = (_f32(t, x, n, who, (D,)) for t, n in ((post_weight, "post_weight"), (res_scale, "res_scale"), (pre_weight, "pre_weight")))
-    if not eps > 0:
-        raise ValueError(f"{who}: eps must be positive")
+    if not 1.17549435e-38 <= eps < 1e30:
+        raise ValueError(f"{who}: eps must be positive (a normal fp32 number) and finite")
     row_mask = _bytes(row_mask, x, "row_mask", who, x.shape[:-1])
     d = NormGateDesc()
     x2, d.x_stride = _rows(x, D)

@@ -29,44 +29,84 @@ struct NormGateK {
     long N; int D;
 };
 
-template <int TPR>
-__device__ __forceinline__ float row_sum(float v, float* s_red) {
-    constexpr int W = TPR < 64 ? TPR : 64;
+// Sums of NS values over the TPR threads of a row, in a fixed tree order: neighbours, quads, halves and rows of 16 lanes by DPP, the rest by
+// shuffles, the waves of a wide row through LDS. The LDS slots alternate (`turn`), so one barrier per sum suffices; it orders LDS only and
+// leaves the next row's loads in flight.
+template <int CTRL> __device__ __forceinline__ float dpp_add(float v) {
+    return v + __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(v), CTRL, 0xF, 0xF, true));
+}
+template <int TPR, int NS>
+__device__ __forceinline__ void row_sums(float (&v)[NS], float* s_red, int& turn) {
 #pragma unroll
-    for (int d = 1; d < W; d *= 2) v += __shfl_xor(v, d);
+    for (int q = 0; q < NS; ++q) {
+        v[q] = dpp_add<0xB1>(v[q]);             // lane ^ 1
+        v[q] = dpp_add<0x4E>(v[q]);             // lane ^ 2
+        v[q] = dpp_add<0x141>(v[q]);            // the other four of eight
+        if constexpr (TPR >= 16) v[q] = dpp_add<0x140>(v[q]);      // the other eight of sixteen
+        if constexpr (TPR >= 32) v[q] += __shfl_xor(v[q], 16);
+        if constexpr (TPR >= 64) v[q] += __shfl_xor(v[q], 32);
+    }
     if constexpr (TPR > 64) {
         constexpr int NW = TPR / 64;                       // waves of a row; the row groups of a workgroup are whole waves
         const int wave = threadIdx.x >> 6, g0 = wave / NW * NW;
-        if ((threadIdx.x & 63) == 0) s_red[wave] = v;
-        __syncthreads();
-        float t = 0.f;
+        float* s = s_red + turn * 32;
+        turn ^= 1;
+        if ((threadIdx.x & 63) == 0) {
 #pragma unroll
-        for (int i = 0; i < NW; ++i) t += s_red[g0 + i];
-        __syncthreads();
-        v = t;
+            for (int q = 0; q < NS; ++q) s[q * 16 + wave] = v[q];
+        }
+        lds_barrier();
+#pragma unroll
+        for (int q = 0; q < NS; ++q) {
+            float t = 0.f;
+#pragma unroll
+            for (int i = 0; i < NW; ++i) t += s[q * 16 + g0 + i];
+            v[q] = t;
+        }
     }
-    return v;
 }
 
+template <class T, int K>
+struct NgRow { Raw<T> x[K], o[K], g[K]; };
+template <class T, int K>
+struct NgGrad { Raw<T> dy[K], dn[K]; };
+
+// WEIGHTS: the weights stay in registers over the rows of the workgroup (else they are read again for every row: rows so wide that the
+// registers do not reach). AHEAD: the next row's loads are issued in front of this row's sums.
 template <class T, int TPR, int K, bool BWD>
 __global__ void __launch_bounds__(TPR > 256 ? TPR : 256) norm_gate_kernel(const NormGateK k) {
     constexpr int VEC = VEC_OF<T>, THREADS = TPR > 256 ? TPR : 256, GROUPS = THREADS / TPR;
-    __shared__ float s_red[16];
+    constexpr bool WEIGHTS = TPR < 1024, AHEAD = TPR < 1024;
+    constexpr int KW = WEIGHTS ? K : 1;
+    __shared__ float s_red[64];
     const int col = threadIdx.x % TPR, grp = threadIdx.x / TPR;
     const float inv_d = 1.f / (float)k.D;
-    int nv[K];
-    float wp[K][VEC], sc[K][VEC], wq[K][VEC];
+    int turn = 0, nv[K];
+    float wp[KW][VEC], sc[KW][VEC], wq[KW][VEC];
+    auto weights = [&](int j, float (&p)[VEC], float (&s)[VEC], float (&q)[VEC]) {
+        const int c0 = (j * TPR + col) * VEC;
+        auto get = [&](const float* w, float (&o)[VEC]) {
+#pragma unroll
+            for (int h = 0; h < VEC / 4; ++h) {
+                const int n = min(max(nv[j] - h * 4, 0), 4);
+                if (w) {
+                    const auto r = ld_raw<float, 4>(w + c0 + h * 4, n);
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) o[h * 4 + i] = raw_get(r, i);
+                } else {
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) o[h * 4 + i] = i < n ? 1.f : 0.f;
+                }
+            }
+        };
+        get(k.w_post, p);
+        get(k.scale, s);
+        get(k.w_pre, q);
+    };
 #pragma unroll
     for (int j = 0; j < K; ++j) {
-        const int c0 = (j * TPR + col) * VEC;
-        nv[j] = min(max(k.D - c0, 0), VEC);
-#pragma unroll
-        for (int i = 0; i < VEC; ++i) {
-            const bool in = i < nv[j];
-            wp[j][i] = in ? (k.w_post ? k.w_post[c0 + i] : 1.f) : 0.f;
-            sc[j][i] = in ? (k.scale ? k.scale[c0 + i] : 1.f) : 0.f;
-            wq[j][i] = in ? (k.w_pre ? k.w_pre[c0 + i] : 1.f) : 0.f;
-        }
+        nv[j] = min(max(k.D - (j * TPR + col) * VEC, 0), VEC);
+        if constexpr (WEIGHTS) weights(j, wp[j], sc[j], wq[j]);
     }
     float awp[BWD ? K : 1][VEC], asc[BWD ? K : 1][VEC], awq[BWD ? K : 1][VEC];
     if (BWD) {
@@ -75,99 +115,129 @@ __global__ void __launch_bounds__(TPR > 256 ? TPR : 256) norm_gate_kernel(const 
 #pragma unroll
             for (int i = 0; i < VEC; ++i) awp[j][i] = asc[j][i] = awq[j][i] = 0.f;
     }
+    NgRow<T, K> a;
+    NgGrad<T, BWD ? K : 1> b;
+    // (every thread takes every round: the sums hold workgroup barriers)
     const long rounds = cdivl(k.N, (long)gridDim.x * GROUPS);
-    for (long it = 0; it < rounds; ++it) {
-        // (every thread takes every round: the reductions hold workgroup barriers)
-        const long r = (it * gridDim.x + blockIdx.x) * GROUPS + grp;
-        const bool in = r < k.N, live = in && !(k.mask && k.mask[r]);
-        Raw<T> rx[K], ro[K], rg[K], rdy[K], rdn[K];
+    auto row_of = [&](long it) { return (it * gridDim.x + blockIdx.x) * GROUPS + grp; };
+    auto alive = [&](long r) { return r < k.N && !(k.mask && k.mask[r]); };
+    auto load = [&](long r, bool live) {
 #pragma unroll
         for (int j = 0; j < K; ++j) {
             const int c0 = (j * TPR + col) * VEC, n = live ? nv[j] : 0;
-            rx[j] = ld_raw<T>((const T*)k.x + r * k.x_s + c0, n);
-            ro[j] = ld_raw<T>((const T*)k.o + r * k.o_s + c0, k.o ? n : 0);
-            rg[j] = ld_raw<T>((const T*)k.g + r * k.g_s + c0, k.g ? n : 0);
-            if (BWD) {
-                rdy[j] = ld_raw<T>((const T*)k.dy + r * k.dy_s + c0, k.dy ? n : 0);
-                rdn[j] = ld_raw<T>((const T*)k.dn + r * k.dn_s + c0, k.dn ? n : 0);
+            a.x[j] = ld_raw<T>((const T*)k.x + r * k.x_s + c0, n);
+            a.o[j] = ld_raw<T>((const T*)k.o + r * k.o_s + c0, k.o ? n : 0);
+            a.g[j] = ld_raw<T>((const T*)k.g + r * k.g_s + c0, k.g ? n : 0);
+            if constexpr (BWD) {
+                b.dy[j] = ld_raw<T>((const T*)k.dy + r * k.dy_s + c0, k.dy ? n : 0);
+                b.dn[j] = ld_raw<T>((const T*)k.dn + r * k.dn_s + c0, k.dn ? n : 0);
             }
         }
+    };
+    bool live_next = alive(row_of(0));
+    if (AHEAD) load(row_of(0), live_next);
+    for (long it = 0; it < rounds; ++it) {
+        const long r = row_of(it);
+        const bool in = r < k.N, live = live_next;
+        if (it + 1 < rounds) live_next = alive(row_of(it + 1));
+        if (!AHEAD) load(r, live);
+        const NgRow<T, K> c = a;
+        const NgGrad<T, BWD ? K : 1> d = b;
+        if (AHEAD && it + 1 < rounds) load(row_of(it + 1), live_next);
         float irms_o = 0.f;
         if (k.o) {
-            float q = 0.f;
+            float q[1] = {0.f};
 #pragma unroll
             for (int j = 0; j < K; ++j)
 #pragma unroll
-                for (int i = 0; i < VEC; ++i) { const float v = raw_get(ro[j], i); q = fmaf(v, v, q); }
-            irms_o = __builtin_amdgcn_rsqf(fmaf(row_sum<TPR>(q, s_red), inv_d, k.eps));
+                for (int i = 0; i < VEC; ++i) { const float v = raw_get(c.o[j], i); q[0] = fmaf(v, v, q[0]); }
+            row_sums<TPR, 1>(q, s_red, turn);
+            irms_o = __builtin_amdgcn_rsqf(fmaf(q[0], inv_d, k.eps));
         }
-        float y[K][VEC], sg[K][VEC], q = 0.f, ey = 0.f;
+        float y[K][VEC], sg[K][VEC], q[2] = {0.f, 0.f};
 #pragma unroll
-        for (int j = 0; j < K; ++j)
+        for (int j = 0; j < K; ++j) {
+            if constexpr (!WEIGHTS) weights(j, wp[0], sc[0], wq[0]);
+            const int w = WEIGHTS ? j : 0;
 #pragma unroll
             for (int i = 0; i < VEC; ++i) {
-                sg[j][i] = k.g ? fast_sigmoid(raw_get(rg[j], i)) : 1.f;
-                const float v = sc[j][i] * sg[j][i] * (raw_get(ro[j], i) * irms_o * wp[j][i]);
-                y[j][i] = fmaf(k.alpha, raw_get(rx[j], i), v);
-                q = fmaf(y[j][i], y[j][i], q);
-                if (BWD) ey = fmaf(raw_get(rdn[j], i) * wq[j][i], y[j][i], ey);
+                sg[j][i] = k.g ? fast_sigmoid(raw_get(c.g[j], i)) : 1.f;
+                const float v = sc[w][i] * sg[j][i] * (raw_get(c.o[j], i) * irms_o * wp[w][i]);
+                y[j][i] = fmaf(k.alpha, raw_get(c.x[j], i), v);
+                q[0] = fmaf(y[j][i], y[j][i], q[0]);
+                if constexpr (BWD) q[1] = fmaf(raw_get(d.dn[j], i) * wq[w][i], y[j][i], q[1]);
             }
+        }
         float irms_y = 0.f;
-        if (BWD ? k.dn != nullptr : k.n != nullptr) irms_y = __builtin_amdgcn_rsqf(fmaf(row_sum<TPR>(q, s_red), inv_d, k.eps));
-        if (!BWD) {
+        if constexpr (!BWD) {
+            if (k.n) {
+                float q1[1] = {q[0]};
+                row_sums<TPR, 1>(q1, s_red, turn);
+                irms_y = __builtin_amdgcn_rsqf(fmaf(q1[0], inv_d, k.eps));
+            }
 #pragma unroll
             for (int j = 0; j < K; ++j) {
-                const int c0 = (j * TPR + col) * VEC, n = in ? nv[j] : 0;
+                const int c0 = (j * TPR + col) * VEC, n = in ? nv[j] : 0, w = WEIGHTS ? j : 0;
                 if (k.y) {
                     float v[VEC];
 #pragma unroll
                     for (int i = 0; i < VEC; ++i) v[i] = live ? y[j][i] : 0.f;
-                    st_raw<T>((T*)k.y + r * k.y_s + c0, raw_pack<T>(v), n);
+                    st_raw<T, VEC>((T*)k.y + r * k.y_s + c0, raw_pack<T>(v), n);
                 }
                 if (k.n) {
+                    if constexpr (!WEIGHTS) { if (K > 1) weights(j, wp[0], sc[0], wq[0]); }
                     float v[VEC];
 #pragma unroll
-                    for (int i = 0; i < VEC; ++i) v[i] = live ? y[j][i] * irms_y * wq[j][i] : 0.f;
-                    st_raw<T>((T*)k.n + r * k.n_s + c0, raw_pack<T>(v), n);
+                    for (int i = 0; i < VEC; ++i) v[i] = live ? y[j][i] * irms_y * wq[w][i] : 0.f;
+                    st_raw<T, VEC>((T*)k.n + r * k.n_s + c0, raw_pack<T>(v), n);
                 }
             }
         } else {
             float m = 0.f;
-            if (k.dn) m = row_sum<TPR>(ey, s_red) * inv_d * irms_y;          // mean(e yh)
-            float e2o = 0.f;
-#pragma unroll
-            for (int j = 0; j < K; ++j)
-#pragma unroll
-                for (int i = 0; i < VEC; ++i) {
-                    const float yh = y[j][i] * irms_y, dn = raw_get(rdn[j], i);
-                    const float d = raw_get(rdy[j], i) + irms_y * (dn * wq[j][i] - yh * m);
-                    awq[j][i] = live ? fmaf(dn, yh, awq[j][i]) : awq[j][i];
-                    const float oh = raw_get(ro[j], i) * irms_o, f = d * sc[j][i] * sg[j][i];
-                    awp[j][i] = live ? fmaf(f, oh, awp[j][i]) : awp[j][i];
-                    asc[j][i] = live ? fmaf(d * sg[j][i], oh * wp[j][i], asc[j][i]) : asc[j][i];
-                    e2o = fmaf(f * wp[j][i], oh, e2o);
-                    y[j][i] = d;
-                }
-            float m2 = 0.f;
-            if (k.o) m2 = row_sum<TPR>(e2o, s_red) * inv_d;
+            if (k.dn) {
+                row_sums<TPR, 2>(q, s_red, turn);
+                irms_y = __builtin_amdgcn_rsqf(fmaf(q[0], inv_d, k.eps));
+                m = q[1] * inv_d * irms_y;                                    // mean(e yh)
+            }
+            float e2o[1] = {0.f};
 #pragma unroll
             for (int j = 0; j < K; ++j) {
-                const int c0 = (j * TPR + col) * VEC, n = in ? nv[j] : 0;
+                if constexpr (!WEIGHTS) { if (K > 1) weights(j, wp[0], sc[0], wq[0]); }
+                const int w = WEIGHTS ? j : 0;
+#pragma unroll
+                for (int i = 0; i < VEC; ++i) {
+                    const float yh = y[j][i] * irms_y, dn = raw_get(d.dn[j], i);
+                    const float dd = raw_get(d.dy[j], i) + irms_y * (dn * wq[w][i] - yh * m);
+                    const float oh = raw_get(c.o[j], i) * irms_o, dg = dd * sg[j][i], f = dg * sc[w][i];
+                    // (masked rows were read as zeros: they add zeros)
+                    awq[j][i] = fmaf(dn, yh, awq[j][i]);
+                    awp[j][i] = fmaf(f, oh, awp[j][i]);
+                    asc[j][i] = fmaf(dg, oh * wp[w][i], asc[j][i]);
+                    e2o[0] = fmaf(f * wp[w][i], oh, e2o[0]);
+                    y[j][i] = dd;
+                }
+            }
+            float m2 = 0.f;
+            if (k.o) { row_sums<TPR, 1>(e2o, s_red, turn); m2 = e2o[0] * inv_d; }
+#pragma unroll
+            for (int j = 0; j < K; ++j) {
+                if constexpr (!WEIGHTS) { if (K > 1) weights(j, wp[0], sc[0], wq[0]); }
+                const int c0 = (j * TPR + col) * VEC, n = in ? nv[j] : 0, w = WEIGHTS ? j : 0;
                 float ox[VEC], oo[VEC], og[VEC];
 #pragma unroll
                 for (int i = 0; i < VEC; ++i) {
-                    const float d = y[j][i], oh = raw_get(ro[j], i) * irms_o, f = d * sc[j][i] * sg[j][i];
-                    ox[i] = live ? k.alpha * d : 0.f;
-                    oo[i] = live ? irms_o * (f * wp[j][i] - oh * m2) : 0.f;
-                    og[i] = live ? f * oh * wp[j][i] * (1.f - sg[j][i]) : 0.f;
+                    const float dd = y[j][i], oh = raw_get(c.o[j], i) * irms_o, e2 = dd * sc[w][i] * sg[j][i] * wp[w][i];
+                    ox[i] = k.alpha * dd;
+                    oo[i] = irms_o * (e2 - oh * m2);
+                    og[i] = e2 * oh * (1.f - sg[j][i]);
                 }
-                st_raw<T>((T*)k.dx + r * k.dx_s + c0, raw_pack<T>(ox), n);
-                if (k.o) st_raw<T>((T*)k.d_o + r * k.do_s + c0, raw_pack<T>(oo), n);
-                if (k.g) st_raw<T>((T*)k.dg + r * k.dg_s + c0, raw_pack<T>(og), n);
+                st_raw<T, VEC>((T*)k.dx + r * k.dx_s + c0, raw_pack<T>(ox), n);
+                if (k.o) st_raw<T, VEC>((T*)k.d_o + r * k.do_s + c0, raw_pack<T>(oo), n);
+                if (k.g) st_raw<T, VEC>((T*)k.dg + r * k.dg_s + c0, raw_pack<T>(og), n);
             }
         }
     }
-    if (BWD) {
+    if constexpr (BWD) {
         // column sums of the workgroup: its row groups in order
         __shared__ float s_col[GROUPS > 1 ? THREADS * VEC : 1];
 #pragma unroll
@@ -179,8 +249,7 @@ __global__ void __launch_bounds__(TPR > 256 ? TPR : 256) norm_gate_kernel(const 
                 const float (&acc)[VEC] = q == 0 ? awp[j] : q == 1 ? asc[j] : awq[j];
                 if constexpr (GROUPS == 1) {
 #pragma unroll
-                    for (int i = 0; i < VEC; ++i)
-                        if (i < nv[j]) dst[c0 + i] = acc[i];
+                    for (int h = 0; h < VEC / 4; ++h) st_raw<float, 4>(dst + c0 + h * 4, raw_pack<float, 4>(acc + h * 4), min(max(nv[j] - h * 4, 0), 4));
                 } else {
                     __syncthreads();
 #pragma unroll
@@ -198,7 +267,7 @@ __global__ void __launch_bounds__(TPR > 256 ? TPR : 256) norm_gate_kernel(const 
     }
 }
 
-// the three weight gradients: blockIdx.y picks the field, the partial rows are added in order
+// the three weight gradients: blockIdx.y picks the field; the partial rows are added in order, a wave's eight at a time
 __global__ void __launch_bounds__(1024) norm_gate_colsum(const float* part, int R, int D, float* d0, float* d1, float* d2) {
     __shared__ float s[16][64];
     float* dst = blockIdx.y == 0 ? d0 : blockIdx.y == 1 ? d1 : d2;
@@ -206,8 +275,17 @@ __global__ void __launch_bounds__(1024) norm_gate_colsum(const float* part, int 
     const int lane = threadIdx.x & 63, w = threadIdx.x >> 6, d = blockIdx.x * 64 + lane;
     const float* src = part + (long)blockIdx.y * R * D;
     float acc = 0.f;
-    if (d < D)
-        for (int r = w; r < R; r += 16) acc += src[(long)r * D + d];
+    if (d < D) {
+        int r = w;
+        for (; r + 7 * 16 < R; r += 8 * 16) {
+            float v[8];
+#pragma unroll
+            for (int j = 0; j < 8; ++j) v[j] = src[(long)(r + j * 16) * D + d];
+#pragma unroll
+            for (int j = 0; j < 8; ++j) acc += v[j];
+        }
+        for (; r < R; r += 16) acc += src[(long)r * D + d];
+    }
     s[w][lane] = acc;
     __syncthreads();
     if (w == 0 && d < D) {
@@ -229,7 +307,7 @@ static int ng_tpr(int D, int vec) {
 static int ng_groups(int tpr) { return tpr >= 256 ? 1 : 256 / tpr; }
 static long ng_blocks(const refil_norm_gate_desc& d, bool bwd) {
     const int tpr = ng_tpr(d.D, d.dtype == REFIL_F32 ? 4 : 8);
-    const long n = cdivl(d.N, ng_groups(tpr)), most = bwd ? NG_BLOCKS : 4096;
+    const long n = cdivl(d.N, ng_groups(tpr)), most = bwd ? NG_BLOCKS : 2048;
     return n < most ? n : most;
 }
 
@@ -262,7 +340,7 @@ static int ng_pick(const NormGateK& k, bool bwd, long blocks, hipStream_t st) {
 static int ng_check(const refil_norm_gate_desc& d, const char* who) {
     REFIL_CHECK(d.dtype >= REFIL_F32 && d.dtype <= REFIL_F16, "%s: dtype %d is none of REFIL_F32 / REFIL_BF16 / REFIL_F16", who, d.dtype);
     REFIL_CHECK(d.N >= 0 && d.D > 0 && d.D <= NG_MAX_D, "%s: N %lld must not be negative, D %d in 1 .. %d", who, (long long)d.N, d.D, NG_MAX_D);
-    REFIL_CHECK(d.eps > 0.f, "%s: eps must be positive", who);
+    REFIL_CHECK(d.eps >= 1.17549435e-38f && d.eps < 1e30f, "%s: eps must be positive (a normal fp32 number) and finite", who);
     REFIL_CHECK(!d.gate || d.o, "%s: a gate needs the block's output", who);
     return 0;
 }

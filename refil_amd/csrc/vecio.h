@@ -44,17 +44,22 @@ __device__ __forceinline__ Raw<T, V> ld_raw(const T* p, int n, unsigned absent =
     }
 #pragma unroll
     for (int i = 0; i < W; ++i) r.w[i] = absent;
-    if constexpr (sizeof(T) == 4) {
+    if (n > 0) {
+        // (V loads at once from places that exist, one wait, then the choice)
+        T e[V];
 #pragma unroll
-        for (int i = 0; i < V; ++i)
-            if (i < n) r.w[i] = __builtin_bit_cast(unsigned, p[i]);
-    } else {
+        for (int i = 0; i < V; ++i) e[i] = p[i < n ? i : n - 1];
+        if constexpr (sizeof(T) == 4) {
 #pragma unroll
-        for (int i = 0; i < V; ++i)
-            if (i < n) {
-                const unsigned e = __builtin_bit_cast(unsigned short, p[i]);
-                r.w[i >> 1] = (i & 1) ? (r.w[i >> 1] & 0xFFFFu) | (e << 16) : (r.w[i >> 1] & 0xFFFF0000u) | e;
+            for (int i = 0; i < V; ++i) r.w[i] = i < n ? __builtin_bit_cast(unsigned, e[i]) : absent;
+        } else {
+#pragma unroll
+            for (int i = 0; i < V; i += 2) {
+                const unsigned lo = i < n ? __builtin_bit_cast(unsigned short, e[i]) : (absent & 0xFFFFu);
+                const unsigned hi = i + 1 < n ? (unsigned)__builtin_bit_cast(unsigned short, e[i + 1]) << 16 : (absent & 0xFFFF0000u);
+                r.w[i >> 1] = lo | hi;
             }
+        }
     }
     return r;
 }
