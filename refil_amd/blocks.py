@@ -36,11 +36,17 @@ def _require_gpu(t, who):
 
 
 def _launch(fn, desc, dev, what):
-    if dev.type == "cuda" and dev.index != torch.cuda.current_device():
-        with torch.cuda.device(dev):
-            check(fn(C.byref(desc), _lib.current_stream_ptr()), what)
+    if dev.type == "cuda":
+        i = dev.index
+        if i != torch._C._cuda_getDevice():
+            with torch.cuda.device(dev):
+                rc = fn(C.byref(desc), torch._C._cuda_getCurrentRawStream(i))
+        else:
+            rc = fn(C.byref(desc), torch._C._cuda_getCurrentRawStream(i))
     else:
-        check(fn(C.byref(desc), _lib.current_stream_ptr()), what)
+        rc = fn(C.byref(desc), _lib.current_stream_ptr())
+    if rc:
+        check(rc, what)
 
 
 def _first(x, who):
@@ -54,42 +60,47 @@ def _first(x, who):
 
 def _like(t, x, name, who, shape=None):
     """an activation tensor beside x: same device and dtype, the given shape (x's)"""
+    want = x.shape if shape is None else shape
+    if t.shape == want and t.dtype == x.dtype and t.device == x.device:
+        return t
     if t.device != x.device:
         raise ValueError(f"{who}: {name} is on {t.device}, the other tensors on {x.device}")
     if t.dtype != x.dtype:
         raise TypeError(f"{who}: {name} is {t.dtype}, the other activations {x.dtype}")
-    want = x.shape if shape is None else shape
-    if t.shape != torch.Size(want):
-        raise ValueError(f"{who}: {name} has shape {tuple(t.shape)}, expected {tuple(want)}")
-    return t
+    raise ValueError(f"{who}: {name} has shape {tuple(t.shape)}, expected {tuple(want)}")
 
 
 def _f32(t, x, name, who, shape):
     """an fp32 parameter / state tensor, dense"""
     if t is None:
         return None
+    if t.shape == shape and t.dtype is torch.float32 and t.device == x.device:
+        return t if t.is_contiguous() else t.contiguous()
     if t.device != x.device:
         raise ValueError(f"{who}: {name} is on {t.device}, the other tensors on {x.device}")
     if t.dtype != torch.float32:
         raise TypeError(f"{who}: {name} is {t.dtype}, expected float32")
-    if t.shape != torch.Size(shape):
-        raise ValueError(f"{who}: {name} has shape {tuple(t.shape)}, expected {tuple(shape)}")
-    return t if t.is_contiguous() else t.contiguous()
+    raise ValueError(f"{who}: {name} has shape {tuple(t.shape)}, expected {tuple(shape)}")
 
 
 def _bytes(t, x, name, who, shape):
     """a uint8 / bool mask"""
     if t is None:
         return None
+    if t.dtype is torch.bool:
+        t = t.view(torch.uint8)
+    if t.shape == shape and t.dtype is torch.uint8 and t.device == x.device:
+        return t
     if t.device != x.device:
         raise ValueError(f"{who}: {name} is on {t.device}, the other tensors on {x.device}")
-    if t.dtype == torch.bool:
-        t = t.view(torch.uint8)
     if t.dtype != torch.uint8:
         raise TypeError(f"{who}: {name} is {t.dtype}, expected uint8 or bool")
-    if t.shape != torch.Size(shape):
-        raise ValueError(f"{who}: {name} has shape {tuple(t.shape)}, expected {tuple(shape)}")
-    return t
+    raise ValueError(f"{who}: {name} has shape {tuple(t.shape)}, expected {tuple(shape)}")
+
+
+def _new(x):
+    """an uninitialised dense tensor of x's shape, type and device"""
+    return torch.empty_like(x, memory_format=torch.contiguous_format)
 
 
 def _p(t):
@@ -132,14 +143,14 @@ def _linrec_desc(who, x, decay_gate, input_gate, decay, scale, h0, reset, length
     h0 = _f32(h0, x, "h0", who, (B, *inner))
     reset = _bytes(reset, x, "reset", who, (B, T))
     if lengths is not None:
-        if lengths.device != x.device or lengths.shape != torch.Size((B,)) or lengths.dtype not in (torch.int32, torch.int64):
+        if lengths.device != x.device or lengths.shape != (B,) or lengths.dtype not in (torch.int32, torch.int64):
             raise ValueError(f"{who}: lengths must be an integer tensor of shape ({B},) on {x.device}")
-        lengths = lengths.to(torch.int32).contiguous()
-    d = LinrecDesc()
-    x, d.x_sB, d.x_sT = _seq(x)
-    decay_gate, d.ga_sB, d.ga_sT = _seq(decay_gate)
-    input_gate, d.gi_sB, d.gi_sT = _seq(input_gate)
-    d.x, d.ga, d.gi, d.decay, d.h0, d.lengths = x.data_ptr(), decay_gate.data_ptr(), input_gate.data_ptr(), decay.data_ptr(), _p(h0), _p(lengths)
+        lengths = (lengths if lengths.dtype is torch.int32 else lengths.clamp(0, T).to(torch.int32)).contiguous()
+    x, xb, xt = _seq(x)
+    decay_gate, ab, at = _seq(decay_gate)
+    input_gate, ib, it = _seq(input_gate)
+    d = LinrecDesc(x.data_ptr(), xb, xt, decay_gate.data_ptr(), ab, at, input_gate.data_ptr(), ib, it, decay.data_ptr(), _p(h0))
+    d.lengths = _p(lengths)
     if reset is not None:
         d.reset, d.rs_sB, d.rs_sT = reset.data_ptr(), reset.stride(0), reset.stride(1)
     width = 1
@@ -159,7 +170,7 @@ def linrec_forward(x, decay_gate, input_gate, decay, *, scale=8.0, h0=None, rese
     who = "linrec_forward"
     d = _linrec_desc(who, x, decay_gate, input_gate, decay, scale, h0, reset, lengths)
     L = _lib.lib()
-    y = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+    y = _new(x)
     h_last = torch.empty((x.shape[0], *x.shape[2:]), dtype=torch.float32, device=x.device)
     saved = torch.empty(L.refil_linrec_saved_floats(C.byref(d)), dtype=torch.float32, device=x.device) if save else None
     ws = _workspace(L.refil_linrec_workspace_bytes(C.byref(d), 0), x)
@@ -179,7 +190,7 @@ def linrec_backward(dy, x, decay_gate, input_gate, decay, saved, *, scale=8.0, h
     dh_last = _f32(dh_last, x, "dh_last", who, state)
     saved = _f32(saved, x, "saved", who, (L.refil_linrec_saved_floats(C.byref(d)),))
     dy, d.dy_sB, d.dy_sT = _seq(dy)
-    dx, dga, dgi = (torch.empty(x.shape, dtype=x.dtype, device=x.device) for _ in range(3))
+    dx, dga, dgi = (_new(x) for _ in range(3))
     ddecay = torch.empty(x.shape[-1], dtype=torch.float32, device=x.device)
     dh0 = torch.empty(state, dtype=torch.float32, device=x.device)
     ws = _workspace(L.refil_linrec_workspace_bytes(C.byref(d), 1), x)
@@ -203,16 +214,17 @@ def linrec_step(x, decay_gate, input_gate, decay, state, *, scale=8.0, slots=Non
     B, D = x.shape[0], x.shape[-1]
     decay = _f32(decay, x, "decay", who, (D,))
     out = state if state_out is None else state_out
-    for name, t in (("state", state), ("state_out", out)):
-        if t.device != x.device or t.dtype != torch.float32 or not t.is_contiguous() or t.dim() != x.dim() or t.shape[1:] != x.shape[1:]:
-            raise ValueError(f"{who}: {name} must be a dense float32 tensor [n, {', '.join(map(str, x.shape[1:]))}] on {x.device}")
-    if out.shape != state.shape:
+    inner = x.shape[1:]
+    for name, t in ((("state", state),) if out is state else (("state", state), ("state_out", out))):
+        if t.device != x.device or t.dtype is not torch.float32 or t.dim() != x.dim() or t.shape[1:] != inner or not t.is_contiguous():
+            raise ValueError(f"{who}: {name} must be a dense float32 tensor [n, {', '.join(map(str, inner))}] on {x.device}")
+    if out is not state and out.shape != state.shape:
         raise ValueError(f"{who}: state_out has shape {tuple(out.shape)}, state {tuple(state.shape)}")
     a, b, n = state.data_ptr(), out.data_ptr(), 4 * state.numel()
     if a != b and a < b + n and b < a + n:
         raise ValueError(f"{who}: state_out overlaps state without being it")
     if slots is not None:
-        if slots.device != x.device or slots.dtype != torch.int32 or slots.shape != torch.Size((B,)):
+        if slots.shape != (B,) or slots.dtype is not torch.int32 or slots.device != x.device:
             raise ValueError(f"{who}: slots must be an int32 tensor of shape ({B},) on {x.device}")
         slots = slots.contiguous()
     elif state.shape[0] < B:
@@ -223,12 +235,10 @@ def linrec_step(x, decay_gate, input_gate, decay, state, *, scale=8.0, slots=Non
     def rows(t):
         return t if t.stride(-1) == 1 and (t.dim() == 2 or t.stride(1) == D) else t.contiguous()
     x, decay_gate, input_gate = rows(x), rows(decay_gate), rows(input_gate)
-    y = torch.empty(x.shape, dtype=x.dtype, device=x.device)
-    d = LinrecStepDesc()
-    d.x, d.x_sB, d.ga, d.ga_sB, d.gi, d.gi_sB = x.data_ptr(), x.stride(0), decay_gate.data_ptr(), decay_gate.stride(0), input_gate.data_ptr(), input_gate.stride(0)
-    d.decay, d.state, d.state_out, d.slots, d.y, d.y_sB = decay.data_ptr(), a, b, _p(slots), y.data_ptr(), y.stride(0)
+    y = _new(x)
     width = D if x.dim() == 2 else D * x.shape[1]
-    d.B, d.C, d.D, d.n_slots, d.dtype, d.scale = B, width, D, state.shape[0], code, scale
+    d = LinrecStepDesc(x.data_ptr(), x.stride(0), decay_gate.data_ptr(), decay_gate.stride(0), input_gate.data_ptr(), input_gate.stride(0), decay.data_ptr(),
+                       a, b, _p(slots), y.data_ptr(), width, B, width, D, state.shape[0], code, scale)
     _launch(_lib.lib().refil_linrec_step, d, x.device, who)
     return y
 
@@ -268,10 +278,13 @@ def _rows(t, D):
     """[..., D] as rows with a dense last dimension; (tensor kept alive, row stride)"""
     if t is None:
         return None, 0
-    t = t.reshape(-1, D)
-    if t.stride(1) != 1 and D > 1:
+    if t.dim() != 2:
+        t = t.reshape(-1, D)
+    st = t.stride()
+    if st[1] != 1 and D > 1:
         t = t.contiguous()
-    return t, t.stride(0)
+        return t, D
+    return t, st[0]
 
 
 def _norm_desc(who, x, o, gate, post_weight, res_scale, pre_weight, alpha, eps, row_mask):
@@ -285,18 +298,17 @@ def _norm_desc(who, x, o, gate, post_weight, res_scale, pre_weight, alpha, eps, 
         if o is None:
             raise ValueError(f"{who}: a gate needs the block's output o")
         _like(gate, x, "gate", who)
-    post_weight, res_scale, pre_weight = (_f32(t, x, n, who, (D,)) for t, n in ((post_weight, "post_weight"), (res_scale, "res_scale"), (pre_weight, "pre_weight")))
+    one = (D,)
+    post_weight, res_scale, pre_weight = _f32(post_weight, x, "post_weight", who, one), _f32(res_scale, x, "res_scale", who, one), _f32(pre_weight, x, "pre_weight", who, one)
     if not 1.17549435e-38 <= eps < 1e30:
         raise ValueError(f"{who}: eps must be positive (a normal fp32 number) and finite")
     row_mask = _bytes(row_mask, x, "row_mask", who, x.shape[:-1])
-    d = NormGateDesc()
-    x2, d.x_stride = _rows(x, D)
-    o2, d.o_stride = _rows(o, D)
-    g2, d.gate_stride = _rows(gate, D)
-    if row_mask is not None:
+    x2, xs = _rows(x, D)
+    o2, os_ = _rows(o, D)
+    g2, gs = _rows(gate, D)
+    if row_mask is not None and (row_mask.dim() != 1 or not row_mask.is_contiguous()):
         row_mask = row_mask.reshape(-1).contiguous()
-    d.x, d.o, d.gate, d.row_mask = x2.data_ptr(), _p(o2), _p(g2), _p(row_mask)
-    d.post_weight, d.res_scale, d.pre_weight = _p(post_weight), _p(res_scale), _p(pre_weight)
+    d = NormGateDesc(x2.data_ptr(), xs, _p(o2), os_, _p(g2), gs, _p(post_weight), _p(res_scale), _p(pre_weight), _p(row_mask))
     d.N, d.D, d.dtype, d.alpha, d.eps = x2.shape[0], D, code, alpha, eps
     d._keep = [x2, o2, g2, post_weight, res_scale, pre_weight, row_mask]
     return d
@@ -311,8 +323,8 @@ def norm_gate_forward(x, o=None, gate=None, *, post_weight=None, res_scale=None,
     d = _norm_desc(who, x, o, gate, post_weight, res_scale, pre_weight, alpha, eps, row_mask)
     if not (want_y or want_n):
         raise ValueError(f"{who}: neither y nor n is asked for")
-    y = torch.empty(x.shape, dtype=x.dtype, device=x.device) if want_y else None
-    n = torch.empty(x.shape, dtype=x.dtype, device=x.device) if want_n else None
+    y = _new(x) if want_y else None
+    n = _new(x) if want_n else None
     d.y, d.n, d.y_stride, d.n_stride = _p(y), _p(n), d.D, d.D
     _launch(_lib.lib().refil_norm_gate_forward, d, x.device, who)
     return y, n
@@ -327,9 +339,9 @@ def norm_gate_backward(dy, dn, x, o=None, gate=None, *, post_weight=None, res_sc
     L, D = _lib.lib(), d.D
     dy2, d.dy_stride = _rows(None if dy is None else _like(dy, x, "dy", who), D)
     dn2, d.dn_stride = _rows(None if dn is None else _like(dn, x, "dn", who), D)
-    dx = torch.empty(x.shape, dtype=x.dtype, device=x.device)
-    do = None if o is None else torch.empty(x.shape, dtype=x.dtype, device=x.device)
-    dg = None if gate is None else torch.empty(x.shape, dtype=x.dtype, device=x.device)
+    dx = _new(x)
+    do = None if o is None else _new(x)
+    dg = None if gate is None else _new(x)
     dwp, dsc, dwq = (None if t is None else torch.empty(D, dtype=torch.float32, device=x.device) for t in (post_weight, res_scale, pre_weight))
     ws = _workspace(L.refil_norm_gate_workspace_bytes(C.byref(d)), x)
     d.dy, d.dn, d.dx, d.d_o, d.dgate, d.dx_stride, d.do_stride, d.dgate_stride = _p(dy2), _p(dn2), dx.data_ptr(), _p(do), _p(dg), D, D, D
@@ -378,14 +390,13 @@ def _ff_desc(who, x, w_gate, w_up, act):
     F, D = w_gate.shape
     _like(w_gate, x, "w_gate", who, (F, D))
     _like(w_up, x, "w_up", who, (F, D))
-    if w_gate.stride() != w_up.stride() or w_gate.stride(1) != 1 or w_gate.stride(0) < D:
-        w_gate, w_up = w_gate.contiguous(), w_up.contiguous()
-    d = GatedFfDesc()
-    x2, d.x_stride = _rows(x, D)
-    if d.x_stride < D:                    # (one row, or rows expanded over one another)
-        x2 = x2.contiguous()
-        d.x_stride = D
-    d.x, d.w_gate, d.w_up, d.w_stride = x2.data_ptr(), w_gate.data_ptr(), w_up.data_ptr(), max(w_gate.stride(0), D)
+    ws = w_gate.stride()
+    if ws != w_up.stride() or ws[1] != 1 or ws[0] < D:
+        w_gate, w_up, ws = w_gate.contiguous(), w_up.contiguous(), (D, 1)
+    x2, xs = _rows(x, D)
+    if xs < D:                            # (one row, or rows expanded over one another)
+        x2, xs = x2.contiguous(), D
+    d = GatedFfDesc(x2.data_ptr(), xs, w_gate.data_ptr(), w_up.data_ptr(), ws[0])
     d.N, d.D, d.F, d.act, d.dtype = x2.shape[0], D, F, _ACTS[act], code
     d._keep = [x2, w_gate, w_up]
     return d
@@ -420,7 +431,7 @@ def gated_ff_backward(dh, x, w_gate, w_up, saved, *, act="silu", bias=False):
     _like(dh, x, "dh", who, (*x.shape[:-1], F))
     saved = _f32(saved, x, "saved", who, (2, d.N, F))
     new = torch.empty if d.N else torch.zeros
-    dx = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+    dx = _new(x)
     dwg, dwu = (new((F, D), dtype=x.dtype, device=x.device) for _ in range(2))
     dbg, dbu = (new(F, dtype=x.dtype, device=x.device) if bias else None for _ in range(2))
     if d.N:
