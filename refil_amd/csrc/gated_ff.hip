@@ -546,7 +546,7 @@ static int gf_go(const GfGemm& k, hipStream_t st) {
     constexpr int BM = WM * MT * 16, BN = WN * NT * 16, HALF = GATED ? BN / 2 : BN;
     constexpr size_t LDS = (size_t)(DIRECT ? 2 : GF_P<T>) * (GfTile<LA, BM, GF_BK<T>>::BYTES + GfTile<LB, BN, GF_BK<T>>::BYTES);
     const long tiles = cdivl(k.M, BM) * cdivl(k.N, HALF);
-    REFIL_CHECK(tiles < (1L << 31), "refil_gated_ff: too many tiles");
+    REFIL_CHECK(tiles * k.splits < (1L << 23), "refil_gated_ff: %ld tiles are too many for one launch", tiles);      // (fewer than 2^32 lanes)
     auto* f = gf_gemm<T, LA, LB, WM, WN, MT, NT, DIRECT, GATED>;
     REFIL_HIP(hipFuncSetAttribute((const void*)f, (hipFuncAttribute)hipFuncAttributeMaxDynamicSharedMemorySize, (int)LDS));
     hipLaunchKernelGGL(f, dim3((unsigned)tiles, k.splits), dim3(WM * WN * 64), LDS, st, k);

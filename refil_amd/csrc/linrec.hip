@@ -633,10 +633,12 @@ static LrPlan lr_plan(const refil_linrec_desc& d, bool bwd) {
     p.ncol = cdiv(d.C, LR_CH);
     p.ntile = cdiv(d.T, lr_tile(d.dtype));
     // Too few (episode, column) pairs to fill the card: the time axis is cut into chunks of whole tiles, at the price of reading the
-    // inputs once more for the chunks' maps. B 4, T 8192, C 1024 bf16: forward 125 us at 1024 workgroups, 121 at 2048 (three fit a CU:
-    // the last round is shorter); backward, two a CU, 148 and 163 us (each workgroup composes the maps in front of it).
-    const long pairs = (long)d.B * p.ncol, want = bwd ? 1024 : 2048;
-    long n = pairs > 0 && pairs < 512 ? cdivl(want, pairs) : 1;
+    // inputs once more for the chunks' maps -- as many as the card holds at once (waves per SIMD by registers: launch bounds), so that
+    // there is one round of workgroups and each starts once.
+    const bool wide = d.dtype == REFIL_F32;
+    const long pairs = (long)d.B * p.ncol, hold = 256L * (bwd ? (wide ? 3 : 2) : (wide ? 4 : 3));
+    long n = pairs > 0 ? hold / pairs : 1;
+    if (n < 1) n = 1;
     if (n > p.ntile) n = p.ntile;
     if (n > 256) n = 256;
     p.tiles_per_chunk = n > 1 ? (int)cdivl(p.ntile, n) : p.ntile;
@@ -647,7 +649,8 @@ static int lr_check(const refil_linrec_desc& d, const char* who) {
     REFIL_CHECK(d.dtype >= REFIL_F32 && d.dtype <= REFIL_F16, "%s: dtype %d is none of REFIL_F32 / REFIL_BF16 / REFIL_F16", who, d.dtype);
     REFIL_CHECK(d.B >= 0 && d.T >= 0 && d.C >= 0 && d.D > 0, "%s: B %d, T %d, C %d must not be negative, D %d positive", who, d.B, d.T, d.C, d.D);
     REFIL_CHECK(d.C % d.D == 0, "%s: C %d must be a multiple of D %d", who, d.C, d.D);
-    REFIL_CHECK((long)d.B * cdiv(d.C, LR_CH) < (1L << 31) && d.T <= (1 << 30), "%s: B %d x C %d x T %d too large", who, d.B, d.C, d.T);
+    // (a launch holds fewer than 2^32 lanes)
+    REFIL_CHECK((long)d.B * cdiv(d.C, LR_CH) < (1L << 24) && d.T <= (1 << 30), "%s: B %d x C %d (64 channels a workgroup) or T %d too large", who, d.B, d.C, d.T);
     REFIL_CHECK(d.scale > 0.f && d.scale < 1e30f, "%s: scale must be positive and finite", who);
     return 0;
 }
@@ -774,7 +777,7 @@ extern "C" int refil_linrec_step(const refil_linrec_step_desc* d, void* stream) 
     REFIL_CHECK(d->B >= 0 && d->C >= 0 && d->D > 0 && d->C % d->D == 0, "refil_linrec_step: B %d, C %d must not be negative, C a multiple of D %d", d->B, d->C, d->D);
     REFIL_CHECK(d->scale > 0.f && d->scale < 1e30f, "refil_linrec_step: scale must be positive and finite");
     REFIL_CHECK(d->slots || d->n_slots >= d->B, "refil_linrec_step: %d state rows for %d rows without slots", d->n_slots, d->B);
-    REFIL_CHECK((long)d->C <= 65535L * 256, "refil_linrec_step: C %d too large", d->C);
+    REFIL_CHECK((long)d->C <= 65535L * 256 && (long)d->B < (1L << 26), "refil_linrec_step: B %d or C %d too large", d->B, d->C);
     if (!d->B || !d->C) return 0;
     REFIL_CHECK(d->x && d->ga && d->gi && d->decay && d->state && d->state_out && d->y, "refil_linrec_step: x, ga, gi, decay, state, state_out and y are required");
     hipStream_t st = (hipStream_t)stream;

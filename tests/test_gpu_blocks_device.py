@@ -70,28 +70,29 @@ def test_captured_graphs_replay_on_new_inputs():
 
 
 def test_autograd_backward_under_capture_is_refused():
-    """the explicit backward is what a graph holds; the autograd one raises and leaves the process and the eager graph alive"""
+    """a whole step captured while an eager graph of the same leaf lives: the backward raises, the process, the eager graph and later captures live on"""
     s = _inputs(5, B=2, T=20, D=16, F=24)
     x = s["x"].clone().requires_grad_(True)
-    eager = blocks.gated_ff(x, s["wg"], s["wu"])                       # an eager graph of the same leaf
-    ins = [(lambda: blocks.linear_recurrence(x, s["ga"], s["gi"], s["decay"])[0]), (lambda: blocks.norm_gate_residual(x, s["g"])[0]), (lambda: blocks.gated_ff(x, s["wg"], s["wu"]))]
-    for fwd in ins:
-        seen = []
-
-        class Capturing:
-            def __enter__(self):
-                self.was = torch.cuda.is_current_stream_capturing
-                torch.cuda.is_current_stream_capturing = lambda: True
-
-            def __exit__(self, *a):
-                torch.cuda.is_current_stream_capturing = self.was
-        y = fwd()
-        with Capturing():                                               # (what a backward inside torch.cuda.graph sees)
-            with pytest.raises(RuntimeError, match="cannot run under graph capture"):
-                y.sum().backward()
-        assert not seen
-    eager.sum().backward()
-    assert torch.isfinite(x.grad).all()
+    calls = [lambda: blocks.linear_recurrence(x, s["ga"], s["gi"], s["decay"])[0], lambda: blocks.norm_gate_residual(x, s["g"])[0], lambda: blocks.gated_ff(x, s["wg"], s["wu"])]
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side), torch.no_grad():
+        for call in calls:
+            call()
+    torch.cuda.current_stream().wait_stream(side)
+    for call in calls:
+        eager = call().sum()
+        with pytest.raises(RuntimeError, match="cannot run under graph capture"):
+            with torch.cuda.graph(torch.cuda.CUDAGraph()):
+                call().sum().backward()
+        x.grad = None
+        eager.backward()
+        assert torch.isfinite(x.grad).all()
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        h, _ = blocks.gated_ff_forward(x.detach(), s["wg"], s["wu"])
+    g.replay()
+    assert torch.equal(h, blocks.gated_ff(x.detach(), s["wg"], s["wu"]))
 
 
 def test_tensors_of_the_other_device_are_refused():
