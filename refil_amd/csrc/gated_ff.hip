@@ -329,31 +329,6 @@ __global__ void __launch_bounds__(WM * WN * 64, WM * MT == 16 || sizeof(T) == 4 
     }
 }
 
-// sums of the split products, in split order; a thread takes four columns of a row
-template <class T>
-__global__ void __launch_bounds__(256) gf_reduce(const GfGemm k) {
-    const unsigned q = (unsigned)cdiv(k.N, 4), n = (unsigned)k.M * q;          // (fewer tiles than compute units: far below 2^32)
-    const long plane = (long)k.M * k.N;
-    for (unsigned e = blockIdx.x * 256 + threadIdx.x; e < n; e += gridDim.x * 256) {
-        const int m = (int)(e / q), c0 = (int)(e - (unsigned)m * q) * 4, c = min(k.N - c0, 4);
-        const bool first = m < k.msplit;
-        const int row = first ? m : m - k.msplit;
-        if (row >= k.mlim) continue;
-        const float* p = k.partial + (long)m * k.N + c0;
-        float s[4] = {0.f, 0.f, 0.f, 0.f};
-        for (int z = 0; z < k.splits; z += 8) {
-            Raw<float> v[8];
-#pragma unroll
-            for (int j = 0; j < 8; ++j) v[j] = ld_raw<float>(p + min(z + j, k.splits - 1) * plane, c);
-#pragma unroll
-            for (int j = 0; j < 8; ++j)
-#pragma unroll
-                for (int i = 0; i < 4; ++i) s[i] += z + j < k.splits ? raw_get(v[j], i) : 0.f;
-        }
-        st_raw<T, 4>((T*)(first ? k.C0 : k.C1) + (long)row * k.ldc + c0, raw_pack<T, 4>(s), c);
-    }
-}
-
 // ---- few rows: every weight is read once, straight into fragments ----
 // A workgroup owns 16 columns of h, its eight waves share the reduction; a lane reads 16 neighbouring k (two matrix steps) of one weight
 // row, so that a row's reads are whole cache lines -- the order of k inside a product is free as long as both operands share it.
@@ -494,22 +469,56 @@ __global__ void __launch_bounds__(256) gf_grad(const GfGrad k) {
         if (col < k.F) k.colsum[(long)blockIdx.y * 2 * k.F + z * k.F + col] = t;
     }
 }
-// bias gradients: the partial rows in order
+// The end of a backward in one launch: the sums of the split products (dx, then dw) in split order, a thread takes four columns of a row;
+// then the bias gradients, 64 columns a workgroup, their partial rows in order.
+struct GfFinish { GfGemm dx, dw; int dx_blocks, dw_blocks; const float* colsum; int rows, F; void* dbg; void* dbu; };
 template <class T>
-__global__ void __launch_bounds__(1024) gf_bias(const float* part, int R, int F, void* dbg, void* dbu) {
-    __shared__ float s[16][64];
-    const int lane = threadIdx.x & 63, w = threadIdx.x >> 6, c = blockIdx.x * 64 + lane;
+__device__ __forceinline__ void gf_reduce(const GfGemm& k, unsigned block, unsigned blocks) {
+    const unsigned q = (unsigned)cdiv(k.N, 4), n = (unsigned)k.M * q;          // (fewer tiles than compute units: far below 2^32)
+    const long plane = (long)k.M * k.N;
+    for (unsigned e = block * 256 + threadIdx.x; e < n; e += blocks * 256) {
+        const int m = (int)(e / q), c0 = (int)(e - (unsigned)m * q) * 4, c = min(k.N - c0, 4);
+        const bool first = m < k.msplit;
+        const int row = first ? m : m - k.msplit;
+        if (row >= k.mlim) continue;
+        const float* p = k.partial + (long)m * k.N + c0;
+        float s[4] = {0.f, 0.f, 0.f, 0.f};
+        for (int z = 0; z < k.splits; z += 8) {
+            Raw<float> v[8];
+#pragma unroll
+            for (int j = 0; j < 8; ++j) v[j] = ld_raw<float>(p + min(z + j, k.splits - 1) * plane, c);
+#pragma unroll
+            for (int j = 0; j < 8; ++j)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) s[i] += z + j < k.splits ? raw_get(v[j], i) : 0.f;
+        }
+        st_raw<T, 4>((T*)(first ? k.C0 : k.C1) + (long)row * k.ldc + c0, raw_pack<T, 4>(s), c);
+    }
+}
+template <class T>
+__global__ void __launch_bounds__(256) gf_finish(const GfFinish k) {
+    __shared__ float s[4][64];
+    if ((int)blockIdx.x < k.dx_blocks) { gf_reduce<T>(k.dx, blockIdx.x, k.dx_blocks); return; }
+    if ((int)blockIdx.x < k.dx_blocks + k.dw_blocks) { gf_reduce<T>(k.dw, blockIdx.x - k.dx_blocks, k.dw_blocks); return; }
+    const int lane = threadIdx.x & 63, w = threadIdx.x >> 6, c = ((int)blockIdx.x - k.dx_blocks - k.dw_blocks) * 64 + lane;
+    const long ld = 2L * k.F;
     float acc = 0.f;
-    if (c < 2 * F)
-        for (int r = w; r < R; r += 16) acc += part[(long)r * 2 * F + c];
+    if (c < 2 * k.F) {
+        int r = w;
+        for (; r + 7 * 4 < k.rows; r += 8 * 4) {
+            float v[8];
+#pragma unroll
+            for (int j = 0; j < 8; ++j) v[j] = k.colsum[(r + j * 4) * ld + c];
+#pragma unroll
+            for (int j = 0; j < 8; ++j) acc += v[j];
+        }
+        for (; r < k.rows; r += 4) acc += k.colsum[r * ld + c];
+    }
     s[w][lane] = acc;
     __syncthreads();
-    if (w == 0 && c < 2 * F) {
-        float v = 0.f;
-#pragma unroll
-        for (int j = 0; j < 16; ++j) v += s[j][lane];
-        T* o = (T*)(c < F ? dbg : dbu);
-        if (o) o[c < F ? c : c - F] = from_f32<T>(v);
+    if (w == 0 && c < 2 * k.F) {
+        T* o = (T*)(c < k.F ? k.dbg : k.dbu);
+        if (o) o[c < k.F ? c : c - k.F] = from_f32<T>((s[0][lane] + s[1][lane]) + (s[2][lane] + s[3][lane]));
     }
 }
 
@@ -565,7 +574,7 @@ static int gf_launch(GfGemm k, const GfPlan& p, hipStream_t st, const char* name
 }
 
 static int gf_blocks(long n) { const long b = cdivl(n, 256); return (int)(b < 1 ? 1 : b > 8192 ? 8192 : b); }
-struct GfBwdWs { void* grad; float* colsum; float* part; long Fp, Np; GfPlan px, pw; int row_blocks, per; size_t bytes; };
+struct GfBwdWs { void* grad; float* colsum; float* part_x; float* part_w; long Fp, Np; GfPlan px, pw; int row_blocks, per; size_t bytes; };
 static GfBwdWs gf_bwd_ws(const refil_gated_ff_desc& d, void* base) {
     char* const p = (char*)base; size_t n = 0;
     auto take = [&](size_t b) { char* r = p ? p + n : nullptr; n += (b + 255) / 256 * 256; return (void*)r; };
@@ -579,8 +588,8 @@ static GfBwdWs gf_bwd_ws(const refil_gated_ff_desc& d, void* base) {
     w.colsum = (float*)take((size_t)w.row_blocks * 2 * d.F * 4);
     w.px = gf_plan(d.N, d.D, 2 * w.Fp, bk, direct);
     w.pw = gf_plan(2 * w.Fp, d.D, w.Np, bk, direct);
-    const size_t a = w.px.splits > 1 ? (size_t)w.px.splits * d.N * d.D : 0, b = w.pw.splits > 1 ? (size_t)w.pw.splits * 2 * w.Fp * d.D : 0;
-    w.part = (float*)take(4 * (a > b ? a : b));
+    if (w.px.splits > 1) w.part_x = (float*)take((size_t)4 * w.px.splits * d.N * d.D);
+    if (w.pw.splits > 1) w.part_w = (float*)take((size_t)4 * w.pw.splits * 2 * w.Fp * d.D);
     w.bytes = n;
     return w;
 }
@@ -606,17 +615,6 @@ static int gf_forward(const refil_gated_ff_desc& d, hipStream_t st) {
     p.splits = 1;
     return gf_launch<T, GF_K, GF_K, true>(k, p, st, "gated_ff_fwd", fl, by);
 }
-template <class T, int LA>
-static int gf_product(GfGemm k, const GfPlan& p, float* part, hipStream_t st, const char* name, double fl, double bytes) {
-    k.partial = part;
-    k.splits = p.splits;
-    if (int rc = gf_launch<T, LA, GF_M, false>(k, p, st, name, fl, bytes)) return rc;
-    if (p.splits > 1) {
-        hipLaunchKernelGGL((gf_reduce<T>), dim3(gf_blocks((long)k.M * k.N / 4)), dim3(256), 0, st, k);
-        REFIL_LAUNCH_CHECK();
-    }
-    return 0;
-}
 template <class T>
 static int gf_backward(const refil_gated_ff_desc& d, hipStream_t st) {
     const GfBwdWs w = gf_bwd_ws(d, d.workspace);
@@ -629,17 +627,29 @@ static int gf_backward(const refil_gated_ff_desc& d, hipStream_t st) {
         hipLaunchKernelGGL((gf_grad<T>), dim3(cdiv(w.Fp, 32 * VEC_OF<T>), w.row_blocks), dim3(256), 0, st, g);
         REFIL_LAUNCH_CHECK();
     }
-    if (g.colsum) {
-        hipLaunchKernelGGL((gf_bias<T>), dim3(cdiv(2 * d.F, 64)), dim3(1024), 0, st, (const float*)w.colsum, w.row_blocks, d.F, d.db_gate, d.db_up);
-        REFIL_LAUNCH_CHECK();
-    }
     GfGemm k{};
     k.A = w.grad; k.lda = 2 * w.Fp; k.B0 = d.w_gate; k.B1 = d.w_up; k.ldb = d.w_stride; k.ksplit = (int)w.Fp;
     k.M = (int)d.N; k.N = d.D; k.K = (int)(2 * w.Fp); k.a_rows = k.M; k.b_rows = d.F; k.C0 = d.dx; k.ldc = d.dx_stride; k.msplit = k.mlim = k.M;
-    if (int rc = gf_product<T, GF_K>(k, w.px, w.part, st, "gated_ff_dx", 4.0 * nf * d.D, es * (2 * nf + 2.0 * d.F * d.D + (double)d.N * d.D))) return rc;
+    k.splits = w.px.splits; k.partial = w.part_x;
+    GfFinish f{};
+    f.dx = k;
+    const double fl = 4.0 * nf * d.D, by = es * (2 * nf + 2.0 * d.F * d.D + (double)d.N * d.D);
+    if (int rc = gf_launch<T, GF_K, GF_M, false>(k, w.px, st, "gated_ff_dx", fl, by)) return rc;
     k.B0 = d.x; k.ldb = d.x_stride; k.ksplit = 1 << 30;
     k.M = (int)(2 * w.Fp); k.N = d.D; k.K = (int)w.Np; k.a_rows = (int)w.Np; k.b_rows = (int)d.N; k.C0 = d.dw_gate; k.C1 = d.dw_up; k.ldc = d.D; k.msplit = (int)w.Fp; k.mlim = d.F;
-    return gf_product<T, GF_M>(k, w.pw, w.part, st, "gated_ff_dw", 4.0 * nf * d.D, es * (2 * nf + 2.0 * d.F * d.D + (double)d.N * d.D));
+    k.splits = w.pw.splits; k.partial = w.part_w;
+    f.dw = k;
+    if (int rc = gf_launch<T, GF_M, GF_M, false>(k, w.pw, st, "gated_ff_dw", fl, by)) return rc;
+    f.dx_blocks = f.dx.splits > 1 ? gf_blocks((long)f.dx.M * f.dx.N / 4) : 0;
+    f.dw_blocks = f.dw.splits > 1 ? gf_blocks((long)f.dw.M * f.dw.N / 4) : 0;
+    f.colsum = w.colsum; f.rows = w.row_blocks; f.F = d.F; f.dbg = d.db_gate; f.dbu = d.db_up;
+    const int blocks = f.dx_blocks + f.dw_blocks + (g.colsum ? cdiv(2 * d.F, 64) : 0);
+    if (blocks) {
+        ProfScope ps("gated_ff_finish", 0, 4.0 * ((double)f.dx.splits * f.dx.M * f.dx.N + (double)f.dw.splits * f.dw.M * f.dw.N), st);
+        hipLaunchKernelGGL((gf_finish<T>), dim3(blocks), dim3(256), 0, st, f);
+        REFIL_LAUNCH_CHECK();
+    }
+    return 0;
 }
 static int gf_check(const refil_gated_ff_desc& d, const char* who) {
     REFIL_CHECK(d.dtype >= REFIL_F32 && d.dtype <= REFIL_F16, "%s: dtype %d is none of REFIL_F32 / REFIL_BF16 / REFIL_F16", who, d.dtype);
