@@ -61,7 +61,7 @@ def _first(x, who):
 def _like(t, x, name, who, shape=None):
     """an activation tensor beside x: same device and dtype, the given shape (x's)"""
     want = x.shape if shape is None else shape
-    if t.shape == want and t.dtype == x.dtype and t.device == x.device:
+    if t.shape == want and t.dtype is x.dtype and t.get_device() == x.get_device():
         return t
     if t.device != x.device:
         raise ValueError(f"{who}: {name} is on {t.device}, the other tensors on {x.device}")
@@ -74,7 +74,7 @@ def _f32(t, x, name, who, shape):
     """an fp32 parameter / state tensor, dense"""
     if t is None:
         return None
-    if t.shape == shape and t.dtype is torch.float32 and t.device == x.device:
+    if t.shape == shape and t.dtype is torch.float32 and t.get_device() == x.get_device():
         return t if t.is_contiguous() else t.contiguous()
     if t.device != x.device:
         raise ValueError(f"{who}: {name} is on {t.device}, the other tensors on {x.device}")
@@ -89,7 +89,7 @@ def _bytes(t, x, name, who, shape):
         return None
     if t.dtype is torch.bool:
         t = t.view(torch.uint8)
-    if t.shape == shape and t.dtype is torch.uint8 and t.device == x.device:
+    if t.shape == shape and t.dtype is torch.uint8 and t.get_device() == x.get_device():
         return t
     if t.device != x.device:
         raise ValueError(f"{who}: {name} is on {t.device}, the other tensors on {x.device}")
@@ -108,7 +108,7 @@ def _p(t):
 
 
 def _workspace(nbytes, x):
-    return torch.empty(nbytes, dtype=torch.uint8, device=x.device) if nbytes else None
+    return x.new_empty(nbytes, dtype=torch.uint8) if nbytes else None
 
 
 def _grad(*tensors):
@@ -191,7 +191,7 @@ def linrec_backward(dy, x, decay_gate, input_gate, decay, saved, *, scale=8.0, h
     saved = _f32(saved, x, "saved", who, (L.refil_linrec_saved_floats(C.byref(d)),))
     dy, d.dy_sB, d.dy_sT = _seq(dy)
     dx, dga, dgi = (_new(x) for _ in range(3))
-    ddecay = torch.empty(x.shape[-1], dtype=torch.float32, device=x.device)
+    ddecay = _new(decay)
     dh0 = torch.empty(state, dtype=torch.float32, device=x.device)
     ws = _workspace(L.refil_linrec_workspace_bytes(C.byref(d), 1), x)
     d.dy, d.dh_last, d.saved = dy.data_ptr(), _p(dh_last), saved.data_ptr()
@@ -216,7 +216,7 @@ def linrec_step(x, decay_gate, input_gate, decay, state, *, scale=8.0, slots=Non
     out = state if state_out is None else state_out
     inner = x.shape[1:]
     for name, t in ((("state", state),) if out is state else (("state", state), ("state_out", out))):
-        if t.device != x.device or t.dtype is not torch.float32 or t.dim() != x.dim() or t.shape[1:] != inner or not t.is_contiguous():
+        if t.get_device() != x.get_device() or t.dtype is not torch.float32 or t.shape[1:] != inner or not t.is_contiguous():
             raise ValueError(f"{who}: {name} must be a dense float32 tensor [n, {', '.join(map(str, inner))}] on {x.device}")
     if out is not state and out.shape != state.shape:
         raise ValueError(f"{who}: state_out has shape {tuple(out.shape)}, state {tuple(state.shape)}")
@@ -224,7 +224,7 @@ def linrec_step(x, decay_gate, input_gate, decay, state, *, scale=8.0, slots=Non
     if a != b and a < b + n and b < a + n:
         raise ValueError(f"{who}: state_out overlaps state without being it")
     if slots is not None:
-        if slots.shape != (B,) or slots.dtype is not torch.int32 or slots.device != x.device:
+        if slots.shape != (B,) or slots.dtype is not torch.int32 or slots.get_device() != x.get_device():
             raise ValueError(f"{who}: slots must be an int32 tensor of shape ({B},) on {x.device}")
         slots = slots.contiguous()
     elif state.shape[0] < B:
@@ -233,7 +233,7 @@ def linrec_step(x, decay_gate, input_gate, decay, state, *, scale=8.0, slots=Non
         raise ValueError(f"{who}: D must be positive")
 
     def rows(t):
-        return t if t.stride(-1) == 1 and (t.dim() == 2 or t.stride(1) == D) else t.contiguous()
+        return t if t.is_contiguous() or (t.stride(-1) == 1 and (t.dim() == 2 or t.stride(1) == D)) else t.contiguous()
     x, decay_gate, input_gate = rows(x), rows(decay_gate), rows(input_gate)
     y = _new(x)
     width = D if x.dim() == 2 else D * x.shape[1]
@@ -342,7 +342,7 @@ def norm_gate_backward(dy, dn, x, o=None, gate=None, *, post_weight=None, res_sc
     dx = _new(x)
     do = None if o is None else _new(x)
     dg = None if gate is None else _new(x)
-    dwp, dsc, dwq = (None if t is None else torch.empty(D, dtype=torch.float32, device=x.device) for t in (post_weight, res_scale, pre_weight))
+    dwp, dsc, dwq = (None if t is None else _new(t) for t in (post_weight, res_scale, pre_weight))
     ws = _workspace(L.refil_norm_gate_workspace_bytes(C.byref(d)), x)
     d.dy, d.dn, d.dx, d.d_o, d.dgate, d.dx_stride, d.do_stride, d.dgate_stride = _p(dy2), _p(dn2), dx.data_ptr(), _p(do), _p(dg), D, D, D
     d.dpost_weight, d.dres_scale, d.dpre_weight = _p(dwp), _p(dsc), _p(dwq)

@@ -29,17 +29,24 @@ struct LinrecK {
     void* y; long y_sB, y_sT; float* h_last; float* saved;
     const void* dy; long dy_sB, dy_sT; const float* dh_last;
     void* dx; void* dga; void* dgi; long d_sB, d_sT; float* dh0; float* part;
-    int B, T, C, D, ncol, nchunk, tiles_per_chunk, ntile;
+    int B, T, C, D, ch, ncol, nchunk, tiles_per_chunk, ntile;      // ch: channels of a workgroup (64, or 256 for few 16-bit sequences)
     float* sumA; float* sumH;          // [B][nchunk][C]: the maps of whole chunks (A = -1: the chunk holds a reset)
 };
 
-constexpr int LR_CH = 64;              // channels of a workgroup: 16 lanes x 4
-constexpr int LR_V = 4, LR_TC = LR_CH / LR_V, LR_TW = 64 / LR_TC, LR_WAVES = 4;
-// steps of a thread: the scan over the wave's time-threads costs the same whatever S is, registers grow with it. fp32 (64 bytes of raw
-// data per step and thread) is bound by occupancy, 16-bit types by instructions.
-template <class T> constexpr int LR_S_OF = sizeof(T) == 4 ? 2 : 4;
-template <class T> constexpr int LR_TT_OF = LR_WAVES * LR_TW * LR_S_OF<T>;         // 32 / 64 steps of a tile
-static int lr_tile(int dtype) { return dtype == REFIL_F32 ? LR_TT_OF<float> : LR_TT_OF<bf16_t>; }
+constexpr int LR_V = 4, LR_WAVES = 4;
+// TC lanes of a wave lie along the channels (4 each), the other 64 / TC along time. 64: a wave reads 256 neighbouring channels at a time and
+// needs no scan of its own; 16, for narrow rows: 64 channels, four time-threads joined by shuffles.
+// Steps of a thread: what joins a tile costs the same whatever S is, registers grow with it. fp32 (16 bytes a value and stream) is bound by
+// occupancy -- 96 episodes of 81 steps, 1024 channels: 31 + 46 us at S 2, 37 + 64 at S 4 -- 16-bit types by instructions.
+template <class T, int TC> struct LrGeo {
+    static constexpr int CH = TC * LR_V, TW = 64 / TC, S = sizeof(T) == 4 ? 2 : 4, TT = LR_WAVES * TW * S;
+};
+// Which: B 4, T 8192, C 1024 bf16 took 98 + 133 us (forward, backward) with 64 lanes and 105 + 143 with 16; fp32 does not gain (78 + 116
+// against 78 + 120 us at T 4096), and many short episodes lose (96 of 81 steps: 45 against 31 us): few 16-bit sequences, wide rows.
+static int lr_tc(int dtype, int B, int C) { return dtype != REFIL_F32 && C > 128 && (long)B * cdiv(C, 64) <= 512 ? 64 : 16; }
+static int lr_tile(int dtype, int B, int C) {
+    return dtype == REFIL_F32 ? LrGeo<float, 16>::TT : lr_tc(dtype, B, C) == 64 ? LrGeo<bf16_t, 64>::TT : LrGeo<bf16_t, 16>::TT;
+}
 
 __device__ __forceinline__ float softplus_(float v) { return fmaxf(v, 0.f) + log1pf(expf(-fabsf(v))); }
 
@@ -63,25 +70,41 @@ __device__ __forceinline__ LrGate lr_gate(float ga, float gi, float rate) {
     return g;
 }
 
-// rates of the workgroup's 64 channels, one softplus each (the caller issues its first loads in front of the barrier)
-__device__ __forceinline__ void lr_rates(const LinrecK& k, int ch0, float* s_rate) {
-    if (threadIdx.x < LR_CH) {
+// rates of the workgroup's channels, one softplus each (the caller issues its first loads in front of the barrier)
+__device__ __forceinline__ void lr_rates(const LinrecK& k, int ch0, int channels, float* s_rate) {
+    if ((int)threadIdx.x < channels) {
         const int c = ch0 + (int)threadIdx.x;
         s_rate[threadIdx.x] = c < k.C ? k.scale * softplus_(k.decay[c % k.D]) : 0.f;
     }
     lds_barrier();
 }
 
-// S steps of one stream. `whole` (wave-uniform): every step is live and every channel there -- no predicates
+// S steps of one stream from `base` (the episode's first step, channel c0). `whole` (wave-uniform): every step is live and every channel
+// there. Otherwise a lane reads from where it may -- a step before the episode's end, V channels inside the row -- and puts right what it
+// got: no branches, one wait (B 3, T 5001, 997 channels of fp16: 73 against 99 us; the wave has a live step, so the episode has one). fp32,
+// whose registers are full, and rows of fewer than V channels branch instead.
 template <class T, int S>
-__device__ __forceinline__ void lr_load(Raw<T, LR_V> (&r)[S], const T* base, long sT, int t0, int Tb, int nv, bool whole, unsigned absent = 0u) {
-    const T* p = base + (long)t0 * sT;
+__device__ __forceinline__ void lr_load(Raw<T, LR_V> (&r)[S], const T* base, long sT, int t0, int Tb, int c0, int C, bool whole, unsigned absent = 0u) {
     if (whole) {
+        const T* p = base + (long)t0 * sT;
 #pragma unroll
         for (int s = 0; s < S; ++s) { r[s] = ld_raw<T, LR_V>(p, LR_V); p += sT; }
+    } else if (sizeof(T) == 2 && C >= LR_V) {
+        const int back = max(c0 - (C - LR_V), 0);
+        const T* p = base - back;
+#pragma unroll
+        for (int s = 0; s < S; ++s) r[s] = ld_raw<T, LR_V>(p + (long)min(t0 + s, Tb - 1) * sT, LR_V);
+        if (C % LR_V) {
+#pragma unroll
+            for (int s = 0; s < S; ++s) r[s] = raw_down<T, LR_V>(r[s], min(back, LR_V - 1));
+        }
+#pragma unroll
+        for (int s = 0; s < S; ++s)
+#pragma unroll
+            for (int w = 0; w < (int)(sizeof(r[s].w) / 4); ++w) r[s].w[w] = t0 + s < Tb ? r[s].w[w] : absent;
     } else {
 #pragma unroll
-        for (int s = 0; s < S; ++s) { r[s] = ld_raw<T, LR_V>(p, t0 + s < Tb ? nv : 0, absent); p += sT; }
+        for (int s = 0; s < S; ++s) r[s] = ld_raw<T, LR_V>(base + (long)(t0 + s) * sT, t0 + s < Tb ? C - c0 : 0, absent);
     }
 }
 // the reset flags of S steps: loaded with the data, looked at when the maps are built
@@ -105,39 +128,53 @@ __device__ __forceinline__ int lr_cuts(const uint8_t (&r)[S], int t0, int Tb) {
 
 // The maps of the n chunks in front (behind): chunk first + i * step is the i-th to apply. Each of the 16 time-threads composes a run of
 // them, the wave joins its four by shuffles; the waves' maps go to LDS (the caller's next barrier orders them).
-struct LrFront { float A[LR_WAVES][LR_CH], H[LR_WAVES][LR_CH]; int cut[LR_WAVES]; };
-__device__ __forceinline__ void lr_front(const LinrecK& k, LrFront& f, int b, int c0, int cl, int nv, int wave, int tw, int n, int first, int step) {
+template <int TC> struct LrFront { float A[LR_WAVES][TC * LR_V], H[LR_WAVES][TC * LR_V]; int cut[LR_WAVES]; };
+template <int TC>
+__device__ __forceinline__ void lr_front(const LinrecK& k, LrFront<TC>& f, int b, int c0, int cl, int nv, int wave, int tw, int n, int first, int step) {
+    constexpr int TW = 64 / TC, AT = 4;
     float A[LR_V], H[LR_V]; int cut = 0;
 #pragma unroll
     for (int i = 0; i < LR_V; ++i) { A[i] = 1.f; H[i] = 0.f; }
-    const int per = cdiv(n, LR_WAVES * LR_TW), i0 = (wave * LR_TW + tw) * per, i1 = min(i0 + per, n);
-    for (int j = i0; j < i1; ++j) {
-        const long o = ((long)b * k.nchunk + first + j * step) * k.C + c0;
-        float a[LR_V], h[LR_V];
+    const int per = cdiv(n, LR_WAVES * TW), i0 = (wave * TW + tw) * per, i1 = min(i0 + per, n);
+    for (int j = i0; j < i1; j += AT) {           // (AT chunks' loads at a time)
+        Raw<float> a[AT], h[AT];
 #pragma unroll
-        for (int i = 0; i < LR_V; ++i) { a[i] = i < nv ? k.sumA[o + i] : 1.f; h[i] = i < nv ? k.sumH[o + i] : 0.f; }
-        const bool c = nv > 0 && a[0] < 0.f;               // (a reset cuts every channel)
-        cut |= (int)c;
-#pragma unroll
-        for (int i = 0; i < LR_V; ++i) { H[i] = c ? h[i] : fmaf(a[i], H[i], h[i]); A[i] *= a[i]; }
-    }
-#pragma unroll
-    for (int d = 1; d < LR_TW; d *= 2) {
-        const int pc = __shfl_up(cut, d * LR_TC);
-#pragma unroll
-        for (int i = 0; i < LR_V; ++i) {
-            const float pA = __shfl_up(A[i], d * LR_TC), pH = __shfl_up(H[i], d * LR_TC);
-            if (tw >= d) { H[i] = cut ? H[i] : fmaf(A[i], pH, H[i]); A[i] *= pA; }
+        for (int q = 0; q < AT; ++q) {
+            const long o = ((long)b * k.nchunk + first + min(j + q, i1 - 1) * step) * k.C + c0;
+            a[q] = ld_raw<float>(k.sumA + o, nv); h[q] = ld_raw<float>(k.sumH + o, nv);
         }
-        if (tw >= d) cut |= pc;
+#pragma unroll
+        for (int q = 0; q < AT; ++q) {
+            const bool in = j + q < i1, c = in && nv > 0 && raw_get(a[q], 0) < 0.f;               // (a reset cuts every channel)
+            cut |= (int)c;
+#pragma unroll
+            for (int i = 0; i < LR_V; ++i) {
+                const float av = in ? raw_get(a[q], i) : 1.f, hv = in ? raw_get(h[q], i) : 0.f;
+                H[i] = c ? hv : fmaf(av, H[i], hv);
+                A[i] *= av;
+            }
+        }
     }
-    if (tw == LR_TW - 1) {
+    if constexpr (TW > 1) {
+#pragma unroll
+        for (int d = 1; d < TW; d *= 2) {
+            const int pc = __shfl_up(cut, d * TC);
+#pragma unroll
+            for (int i = 0; i < LR_V; ++i) {
+                const float pA = __shfl_up(A[i], d * TC), pH = __shfl_up(H[i], d * TC);
+                if (tw >= d) { H[i] = cut ? H[i] : fmaf(A[i], pH, H[i]); A[i] *= pA; }
+            }
+            if (tw >= d) cut |= pc;
+        }
+    }
+    if (tw == TW - 1) {
 #pragma unroll
         for (int i = 0; i < LR_V; ++i) { f.A[wave][cl + i] = A[i]; f.H[wave][cl + i] = H[i]; }
         if (cl == 0) f.cut[wave] = cut;
     }
 }
-__device__ __forceinline__ void lr_front_apply(const LrFront& f, int cl, float (&carry)[LR_V]) {
+template <int TC>
+__device__ __forceinline__ void lr_front_apply(const LrFront<TC>& f, int cl, float (&carry)[LR_V]) {
 #pragma unroll
     for (int w = 0; w < LR_WAVES; ++w) {
         const int c = f.cut[w];
@@ -146,21 +183,22 @@ __device__ __forceinline__ void lr_front_apply(const LrFront& f, int cl, float (
     }
 }
 
-// One workgroup per (episode, 64 channels, chunk of the time axis). FINAL: the outputs, starting from the carry of the chunks in front;
+// One workgroup per (episode, CH channels, chunk of the time axis). FINAL: the outputs, starting from the carry of the chunks in front;
 // else the chunk's whole map only. Steps past the episode's end are not loaded: their decay gate is -inf (a = 1, no input), the state
 // stays. A wave whose steps all lie there skips the arithmetic. The next tile's loads are in flight from the moment this tile's gates are
 // computed: over its scans, barrier and stores.
-template <class T, bool FINAL, bool RST>
+template <class T, int TC, bool FINAL, bool RST>
 __global__ void __launch_bounds__(256, sizeof(T) == 4 ? 4 : 3) linrec_fwd(const LinrecK k) {
-    constexpr int V = LR_V, TC = LR_TC, TW = LR_TW, S = LR_S_OF<T>, TT = LR_TT_OF<T>;
-    __shared__ float s_rate[LR_CH];
-    __shared__ float sA[2][LR_WAVES][LR_CH], sH[2][LR_WAVES][LR_CH];
+    typedef LrGeo<T, TC> G;
+    constexpr int V = LR_V, TW = G::TW, S = G::S, TT = G::TT, CH = G::CH;
+    __shared__ float s_rate[CH];
+    __shared__ float sA[2][LR_WAVES][CH], sH[2][LR_WAVES][CH];
     __shared__ int sCut[2][LR_WAVES];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
-    const int b = (int)(blockIdx.x / k.ncol), ch0 = (int)(blockIdx.x % k.ncol) * LR_CH, chunk = blockIdx.y;
+    const int b = (int)(blockIdx.x / k.ncol), ch0 = (int)(blockIdx.x % k.ncol) * CH, chunk = blockIdx.y;
     const int cl = (lane % TC) * V, c0 = ch0 + cl, nv = min(max(k.C - c0, 0), V);
     const int tw = lane / TC;
-    const bool all_ch = ch0 + LR_CH <= k.C;
+    const bool all_ch = ch0 + CH <= k.C;
     const int Tb = k.lengths ? min(max(k.lengths[b], 0), k.T) : k.T;
     const T* xb = (const T*)k.x + (long)b * k.x_sB + c0;
     const T* gab = (const T*)k.ga + (long)b * k.ga_sB + c0;
@@ -172,9 +210,9 @@ __global__ void __launch_bounds__(256, sizeof(T) == 4 ? 4 : 3) linrec_fwd(const 
         const int w0 = tile * TT + wave * (TW * S), t0 = w0 + tw * S;
         if (tile < tile1 && w0 < Tb) {
             const bool whole = all_ch && w0 + TW * S <= Tb;
-            lr_load(rga, gab, k.ga_sT, t0, Tb, nv, whole, NEG_INF_WORD<T>);
-            lr_load(rgi, gib, k.gi_sT, t0, Tb, nv, whole);
-            lr_load(rx, xb, k.x_sT, t0, Tb, nv, whole);
+            lr_load(rga, gab, k.ga_sT, t0, Tb, c0, k.C, whole, NEG_INF_WORD<T>);
+            lr_load(rgi, gib, k.gi_sT, t0, Tb, c0, k.C, whole);
+            lr_load(rx, xb, k.x_sT, t0, Tb, c0, k.C, whole);
             lr_load_cuts<RST, S>(rc, k, b, t0, Tb);
         }
     };
@@ -182,9 +220,9 @@ __global__ void __launch_bounds__(256, sizeof(T) == 4 ? 4 : 3) linrec_fwd(const 
     float carry[V];
 #pragma unroll
     for (int i = 0; i < V; ++i) carry[i] = FINAL && k.h0 && i < nv ? k.h0[(long)b * k.C + c0 + i] : 0.f;
-    __shared__ LrFront front;
+    __shared__ LrFront<TC> front;
     if (FINAL && chunk > 0) lr_front(k, front, b, c0, cl, nv, wave, tw, chunk, 0, 1);
-    lr_rates(k, ch0, s_rate);
+    lr_rates(k, ch0, CH, s_rate);
     if (FINAL && chunk > 0) lr_front_apply(front, cl, carry);
     float rate[V], top = 0.f;
 #pragma unroll
@@ -225,6 +263,7 @@ __global__ void __launch_bounds__(256, sizeof(T) == 4 ? 4 : 3) linrec_fwd(const 
                     A[i] *= a[s][i];
                 }
             // inclusive over the wave's time-threads, then exclusive
+            if constexpr (TW > 1) {
 #pragma unroll
             for (int d = 1; d < TW; d *= 2) {
                 const int pc = RST ? __shfl_up(cut, d * TC) : 0;
@@ -242,6 +281,7 @@ __global__ void __launch_bounds__(256, sizeof(T) == 4 ? 4 : 3) linrec_fwd(const 
                 eA[i] = tw ? pA : 1.f; eH[i] = tw ? pH : 0.f;
             }
             if (tw == 0) ecut = 0;
+            }
         }
         if (tw == TW - 1) {
 #pragma unroll
@@ -270,7 +310,7 @@ __global__ void __launch_bounds__(256, sizeof(T) == 4 ? 4 : 3) linrec_fwd(const 
         }
         if (FINAL && tw0 < k.T) {
             T* yp = (T*)k.y + (long)b * k.y_sB + (long)t0 * k.y_sT + c0;
-            if (any_live) {
+            if (TW > 1 && any_live) {
 #pragma unroll
                 for (int i = 0; i < V; ++i) h[i] = ecut ? eH[i] : fmaf(eA[i], h[i], eH[i]);
             }
@@ -303,17 +343,18 @@ __global__ void __launch_bounds__(256, sizeof(T) == 4 ? 4 : 3) linrec_fwd(const 
 }
 
 // the same cut of the time axis in reverse order
-template <class T, bool FINAL, bool RST>
+template <class T, int TC, bool FINAL, bool RST>
 __global__ void __launch_bounds__(256, sizeof(T) == 4 || !FINAL ? 3 : 2) linrec_bwd(const LinrecK k) {
-    constexpr int V = LR_V, TC = LR_TC, TW = LR_TW, S = LR_S_OF<T>, TT = LR_TT_OF<T>;
-    __shared__ float s_rate[LR_CH];
-    __shared__ float sA[2][LR_WAVES][LR_CH], sH[2][LR_WAVES][LR_CH], sR[2][LR_WAVES][LR_CH];
+    typedef LrGeo<T, TC> G;
+    constexpr int V = LR_V, TW = G::TW, S = G::S, TT = G::TT, CH = G::CH;
+    __shared__ float s_rate[CH];
+    __shared__ float sA[2][LR_WAVES][CH], sH[2][LR_WAVES][CH], sR[2][LR_WAVES][CH];
     __shared__ int sCut[2][LR_WAVES];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
-    const int b = (int)(blockIdx.x / k.ncol), ch0 = (int)(blockIdx.x % k.ncol) * LR_CH, chunk = blockIdx.y;
+    const int b = (int)(blockIdx.x / k.ncol), ch0 = (int)(blockIdx.x % k.ncol) * CH, chunk = blockIdx.y;
     const int cl = (lane % TC) * V, c0 = ch0 + cl, nv = min(max(k.C - c0, 0), V);
     const int tw = lane / TC;
-    const bool all_ch = ch0 + LR_CH <= k.C;
+    const bool all_ch = ch0 + CH <= k.C;
     const int Tb = k.lengths ? min(max(k.lengths[b], 0), k.T) : k.T;
     const T* xb = (const T*)k.x + (long)b * k.x_sB + c0;
     const T* gab = (const T*)k.ga + (long)b * k.ga_sB + c0;
@@ -327,11 +368,11 @@ __global__ void __launch_bounds__(256, sizeof(T) == 4 || !FINAL ? 3 : 2) linrec_
         const int w0 = tile * TT + wave * (TW * S), t0 = w0 + tw * S;
         if (tile >= tile0 && w0 < Tb) {
             const bool whole = all_ch && w0 + TW * S <= Tb;
-            lr_load(rga, gab, k.ga_sT, t0, Tb, nv, whole, NEG_INF_WORD<T>);
-            lr_load(rdy, dyb, k.dy_sT, t0, Tb, nv, whole);
+            lr_load(rga, gab, k.ga_sT, t0, Tb, c0, k.C, whole, NEG_INF_WORD<T>);
+            lr_load(rdy, dyb, k.dy_sT, t0, Tb, c0, k.C, whole);
             if (FINAL) {
-                lr_load(rgi, gib, k.gi_sT, t0, Tb, nv, whole);
-                lr_load(rx, xb, k.x_sT, t0, Tb, nv, whole);
+                lr_load(rgi, gib, k.gi_sT, t0, Tb, c0, k.C, whole);
+                lr_load(rx, xb, k.x_sT, t0, Tb, c0, k.C, whole);
                 const float* o = k.saved + ((long)b * k.ntile + tile) * k.C + c0;
 #pragma unroll
                 for (int i = 0; i < V; ++i) hin[i] = i < nv ? o[i] : 0.f;
@@ -346,10 +387,10 @@ __global__ void __launch_bounds__(256, sizeof(T) == 4 || !FINAL ? 3 : 2) linrec_
         carry[i] = FINAL && k.dh_last && i < nv ? k.dh_last[(long)b * k.C + c0 + i] : 0.f;
         cA[i] = 1.f; dl[i] = 0.f;
     }
-    __shared__ LrFront front;
+    __shared__ LrFront<TC> front;
     const int behind = k.nchunk - 1 - chunk;
     if (FINAL && behind > 0) lr_front(k, front, b, c0, cl, nv, wave, tw, behind, k.nchunk - 1, -1);
-    lr_rates(k, ch0, s_rate);
+    lr_rates(k, ch0, CH, s_rate);
     if (FINAL && behind > 0) lr_front_apply(front, cl, carry);
     float rate[V], top = 0.f;
 #pragma unroll
@@ -401,6 +442,7 @@ __global__ void __launch_bounds__(256, sizeof(T) == 4 || !FINAL ? 3 : 2) linrec_
             // forward: inclusive prefix of (A, H); backward: inclusive suffix of (B, R)
 #pragma unroll
             for (int i = 0; i < V; ++i) B[i] = A[i];
+            if constexpr (TW > 1) {
 #pragma unroll
             for (int d = 1; d < TW; d *= 2) {
                 const int pc = RST ? __shfl_up(fcut, d * TC) : 0, nc = RST ? __shfl_down(rcut, d * TC) : 0;
@@ -426,6 +468,7 @@ __global__ void __launch_bounds__(256, sizeof(T) == 4 || !FINAL ? 3 : 2) linrec_
                 }
                 if (tw == 0) ecut = 0;
                 if (tw == TW - 1) xcut = 0;
+            }
             }
         }
         if (tw == 0) {
@@ -463,10 +506,12 @@ __global__ void __launch_bounds__(256, sizeof(T) == 4 || !FINAL ? 3 : 2) linrec_
                         for (int i = 0; i < V; ++i) hin[i] = wc ? sH[p][w][cl + i] : fmaf(sA[p][w][cl + i], hin[i], sH[p][w][cl + i]);
                     }
                 }
+                if constexpr (TW > 1) {
 #pragma unroll
-                for (int i = 0; i < V; ++i) {
-                    hin[i] = ecut ? eH[i] : fmaf(eA[i], hin[i], eH[i]);
-                    c[i] = xcut ? xR[i] : fmaf(xA[i], c[i], xR[i]);
+                    for (int i = 0; i < V; ++i) {
+                        hin[i] = ecut ? eH[i] : fmaf(eA[i], hin[i], eH[i]);
+                        c[i] = xcut ? xR[i] : fmaf(xA[i], c[i], xR[i]);
+                    }
                 }
 #pragma unroll
                 for (int s = 0; s < S; ++s)
@@ -539,8 +584,8 @@ __global__ void __launch_bounds__(256, sizeof(T) == 4 || !FINAL ? 3 : 2) linrec_
         for (int i = 0; i < V; ++i) sA[0][wave][cl + i] = dl[i];
     }
     __syncthreads();
-    if (wave == 0 && ch0 + lane < k.C)
-        k.part[((long)b * k.nchunk + chunk) * k.C + ch0 + lane] = (sA[0][0][lane] + sA[0][1][lane]) + (sA[0][2][lane] + sA[0][3][lane]);
+    const int e = threadIdx.x;
+    if (e < CH && ch0 + e < k.C) k.part[((long)b * k.nchunk + chunk) * k.C + ch0 + e] = (sA[0][0][e] + sA[0][1][e]) + (sA[0][2][e] + sA[0][3][e]);
 }
 
 // One acting step: state rows are read, advanced and written back. Rows that name the same slot are consecutive steps of that state, in
@@ -630,8 +675,8 @@ __global__ void __launch_bounds__(1024) linrec_ddecay(const float* src, long R, 
 struct LrPlan { int ncol, ntile, nchunk, tiles_per_chunk; };
 static LrPlan lr_plan(const refil_linrec_desc& d, bool bwd) {
     LrPlan p;
-    p.ncol = cdiv(d.C, LR_CH);
-    p.ntile = cdiv(d.T, lr_tile(d.dtype));
+    p.ncol = cdiv(d.C, lr_tc(d.dtype, d.B, d.C) * LR_V);
+    p.ntile = cdiv(d.T, lr_tile(d.dtype, d.B, d.C));
     // Too few (episode, column) pairs to fill the card: the time axis is cut into chunks of whole tiles, at the price of reading the
     // inputs once more for the chunks' maps -- as many as the card holds at once (waves per SIMD by registers: launch bounds), so that
     // there is one round of workgroups and each starts once.
@@ -650,7 +695,7 @@ static int lr_check(const refil_linrec_desc& d, const char* who) {
     REFIL_CHECK(d.B >= 0 && d.T >= 0 && d.C >= 0 && d.D > 0, "%s: B %d, T %d, C %d must not be negative, D %d positive", who, d.B, d.T, d.C, d.D);
     REFIL_CHECK(d.C % d.D == 0, "%s: C %d must be a multiple of D %d", who, d.C, d.D);
     // (a launch holds fewer than 2^32 lanes)
-    REFIL_CHECK((long)d.B * cdiv(d.C, LR_CH) < (1L << 24) && d.T <= (1 << 30), "%s: B %d x C %d (64 channels a workgroup) or T %d too large", who, d.B, d.C, d.T);
+    REFIL_CHECK((long)d.B * cdiv(d.C, 64) < (1L << 24) && d.T <= (1 << 30), "%s: B %d x C %d (64 channels a workgroup) or T %d too large", who, d.B, d.C, d.T);
     REFIL_CHECK(d.scale > 0.f && d.scale < 1e30f, "%s: scale must be positive and finite", who);
     return 0;
 }
@@ -661,7 +706,7 @@ static LinrecK lr_args(const refil_linrec_desc& d, const LrPlan& p) {
     k.y = d.y; k.y_sB = d.y_sB; k.y_sT = d.y_sT; k.h_last = d.h_last; k.saved = d.saved;
     k.dy = d.dy; k.dy_sB = d.dy_sB; k.dy_sT = d.dy_sT; k.dh_last = d.dh_last; k.dx = d.dx; k.dga = d.dga; k.dgi = d.dgi; k.d_sB = d.d_sB; k.d_sT = d.d_sT;
     k.dh0 = d.dh0;
-    k.B = d.B; k.T = d.T; k.C = d.C; k.D = d.D; k.ncol = p.ncol; k.nchunk = p.nchunk; k.tiles_per_chunk = p.tiles_per_chunk; k.ntile = p.ntile;
+    k.B = d.B; k.T = d.T; k.C = d.C; k.D = d.D; k.ch = lr_tc(d.dtype, d.B, d.C) * LR_V; k.ncol = p.ncol; k.nchunk = p.nchunk; k.tiles_per_chunk = p.tiles_per_chunk; k.ntile = p.ntile;
     return k;
 }
 // workspace: [sumA][sumH] (more than one chunk), backward: [part]
@@ -675,6 +720,30 @@ static long lr_ws_floats(const refil_linrec_desc& d, const LrPlan& p, bool bwd) 
     return n;
 }
 
+template <class T, bool FINAL>
+static void lr_go_fwd(const LinrecK& k, dim3 grid, hipStream_t st) {
+    if constexpr (sizeof(T) == 2) {
+        if (k.ch == 256) {
+            if (k.reset) hipLaunchKernelGGL((linrec_fwd<T, 64, FINAL, true>), grid, dim3(256), 0, st, k);
+            else hipLaunchKernelGGL((linrec_fwd<T, 64, FINAL, false>), grid, dim3(256), 0, st, k);
+            return;
+        }
+    }
+    if (k.reset) hipLaunchKernelGGL((linrec_fwd<T, 16, FINAL, true>), grid, dim3(256), 0, st, k);
+    else hipLaunchKernelGGL((linrec_fwd<T, 16, FINAL, false>), grid, dim3(256), 0, st, k);
+}
+template <class T, bool FINAL>
+static void lr_go_bwd(const LinrecK& k, dim3 grid, hipStream_t st) {
+    if constexpr (sizeof(T) == 2) {
+        if (k.ch == 256) {
+            if (k.reset) hipLaunchKernelGGL((linrec_bwd<T, 64, FINAL, true>), grid, dim3(256), 0, st, k);
+            else hipLaunchKernelGGL((linrec_bwd<T, 64, FINAL, false>), grid, dim3(256), 0, st, k);
+            return;
+        }
+    }
+    if (k.reset) hipLaunchKernelGGL((linrec_bwd<T, 16, FINAL, true>), grid, dim3(256), 0, st, k);
+    else hipLaunchKernelGGL((linrec_bwd<T, 16, FINAL, false>), grid, dim3(256), 0, st, k);
+}
 template <class T>
 static int lr_forward(const refil_linrec_desc& d, hipStream_t st) {
     const LrPlan p = lr_plan(d, false);
@@ -685,13 +754,11 @@ static int lr_forward(const refil_linrec_desc& d, hipStream_t st) {
     const double n = (double)d.B * d.T * d.C;
     if (p.nchunk > 1) {
         ProfScope ps("linrec_fwd<summary>", 20 * n, 3 * n * sizeof(T), st);
-        if (k.reset) hipLaunchKernelGGL((linrec_fwd<T, false, true>), grid, dim3(256), 0, st, k);
-        else hipLaunchKernelGGL((linrec_fwd<T, false, false>), grid, dim3(256), 0, st, k);
+        lr_go_fwd<T, false>(k, grid, st);
         REFIL_LAUNCH_CHECK();
     }
     ProfScope ps("linrec_fwd", 25 * n, 4 * n * sizeof(T), st);
-    if (k.reset) hipLaunchKernelGGL((linrec_fwd<T, true, true>), grid, dim3(256), 0, st, k);
-    else hipLaunchKernelGGL((linrec_fwd<T, true, false>), grid, dim3(256), 0, st, k);
+    lr_go_fwd<T, true>(k, grid, st);
     REFIL_LAUNCH_CHECK();
     return 0;
 }
@@ -712,14 +779,12 @@ static int lr_backward(const refil_linrec_desc& d, hipStream_t st) {
     const double n = (double)d.B * d.T * d.C;
     if (p.nchunk > 1) {
         ProfScope ps("linrec_bwd<summary>", 20 * n, 2 * n * sizeof(T), st);
-        if (k.reset) hipLaunchKernelGGL((linrec_bwd<T, false, true>), grid, dim3(256), 0, st, k);
-        else hipLaunchKernelGGL((linrec_bwd<T, false, false>), grid, dim3(256), 0, st, k);
+        lr_go_bwd<T, false>(k, grid, st);
         REFIL_LAUNCH_CHECK();
     }
     {
         ProfScope ps("linrec_bwd", 55 * n, 7 * n * sizeof(T), st);
-        if (k.reset) hipLaunchKernelGGL((linrec_bwd<T, true, true>), grid, dim3(256), 0, st, k);
-        else hipLaunchKernelGGL((linrec_bwd<T, true, false>), grid, dim3(256), 0, st, k);
+        lr_go_bwd<T, true>(k, grid, st);
         REFIL_LAUNCH_CHECK();
     }
     return lr_ddecay(d, k.part, rows, st);
@@ -746,7 +811,7 @@ extern "C" size_t refil_linrec_workspace_bytes(const refil_linrec_desc* d, int32
 }
 extern "C" int64_t refil_linrec_saved_floats(const refil_linrec_desc* d) {
     if (!d || lr_check(*d, "refil_linrec_saved_floats")) return 0;
-    return (int64_t)d->B * cdiv(d->T, lr_tile(d->dtype)) * d->C;
+    return (int64_t)d->B * cdiv(d->T, lr_tile(d->dtype, d->B, d->C)) * d->C;
 }
 extern "C" int refil_linrec_forward(const refil_linrec_desc* d, void* stream) {
     REFIL_CHECK(d, "refil_linrec_forward: null desc");

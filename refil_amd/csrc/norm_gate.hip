@@ -81,7 +81,10 @@ __global__ void __launch_bounds__(TPR > 256 ? TPR : 256) norm_gate_kernel(const 
     __shared__ float s_red[64];
     const int col = threadIdx.x % TPR, grp = threadIdx.x / TPR;
     const float inv_d = 1.f / (float)k.D;
-    int turn = 0, nv[K];
+    // the ragged end of a row is read as the row's last VEC elements, moved down by `back`: one load, where VEC single ones would keep the
+    // wave waiting (rows of fewer than VEC elements do that, and the widest, whose registers are full)
+    const bool ragged = TPR < 1024 && k.D % VEC != 0 && k.D >= VEC;
+    int turn = 0, nv[K], back[K];
     float wp[KW][VEC], sc[KW][VEC], wq[KW][VEC];
     auto weights = [&](int j, float (&p)[VEC], float (&s)[VEC], float (&q)[VEC]) {
         const int c0 = (j * TPR + col) * VEC;
@@ -106,6 +109,7 @@ __global__ void __launch_bounds__(TPR > 256 ? TPR : 256) norm_gate_kernel(const 
 #pragma unroll
     for (int j = 0; j < K; ++j) {
         nv[j] = min(max(k.D - (j * TPR + col) * VEC, 0), VEC);
+        back[j] = ragged && nv[j] > 0 ? VEC - nv[j] : 0;
         if constexpr (WEIGHTS) weights(j, wp[j], sc[j], wq[j]);
     }
     float awp[BWD ? K : 1][VEC], asc[BWD ? K : 1][VEC], awq[BWD ? K : 1][VEC];
@@ -124,7 +128,7 @@ __global__ void __launch_bounds__(TPR > 256 ? TPR : 256) norm_gate_kernel(const 
     auto load = [&](long r, bool live) {
 #pragma unroll
         for (int j = 0; j < K; ++j) {
-            const int c0 = (j * TPR + col) * VEC, n = live ? nv[j] : 0;
+            const int c0 = (j * TPR + col) * VEC - back[j], n = live ? nv[j] + back[j] : 0;
             a.x[j] = ld_raw<T>((const T*)k.x + r * k.x_s + c0, n);
             a.o[j] = ld_raw<T>((const T*)k.o + r * k.o_s + c0, k.o ? n : 0);
             a.g[j] = ld_raw<T>((const T*)k.g + r * k.g_s + c0, k.g ? n : 0);
@@ -141,9 +145,16 @@ __global__ void __launch_bounds__(TPR > 256 ? TPR : 256) norm_gate_kernel(const 
         const bool in = r < k.N, live = live_next;
         if (it + 1 < rounds) live_next = alive(row_of(it + 1));
         if (!AHEAD) load(r, live);
-        const NgRow<T, K> c = a;
-        const NgGrad<T, BWD ? K : 1> d = b;
+        NgRow<T, K> c = a;
+        NgGrad<T, BWD ? K : 1> d = b;
         if (AHEAD && it + 1 < rounds) load(row_of(it + 1), live_next);
+        if (ragged) {
+#pragma unroll
+            for (int j = 0; j < K; ++j) {
+                c.x[j] = raw_down<T, VEC>(c.x[j], back[j]); c.o[j] = raw_down<T, VEC>(c.o[j], back[j]); c.g[j] = raw_down<T, VEC>(c.g[j], back[j]);
+                if constexpr (BWD) { d.dy[j] = raw_down<T, VEC>(d.dy[j], back[j]); d.dn[j] = raw_down<T, VEC>(d.dn[j], back[j]); }
+            }
+        }
         float irms_o = 0.f;
         if (k.o) {
             float q[1] = {0.f};

@@ -30,6 +30,22 @@ template <class T> inline constexpr unsigned NEG_INF_WORD = 0xFF800000u;
 template <> inline constexpr unsigned NEG_INF_WORD<bf16_t> = 0xFF80FF80u;
 template <> inline constexpr unsigned NEG_INF_WORD<f16_t> = 0xFC00FC00u;
 
+// V elements moved down by m (0 <= m < V), zeros coming in on top
+template <class T, int V>
+__device__ __forceinline__ Raw<T, V> raw_down(Raw<T, V> r, int m) {
+    constexpr int W = V * sizeof(T) / 4;
+    const int words = sizeof(T) == 4 ? m : m >> 1;
+#pragma unroll
+    for (int b = 1; b < W; b *= 2) {
+#pragma unroll
+        for (int i = 0; i < W; ++i) r.w[i] = (words & b) ? (i + b < W ? r.w[i + b] : 0u) : r.w[i];
+    }
+    if constexpr (sizeof(T) == 2) {
+#pragma unroll
+        for (int i = 0; i < W; ++i) r.w[i] = (m & 1) ? (r.w[i] >> 16) | (i + 1 < W ? r.w[i + 1] << 16 : 0u) : r.w[i];
+    }
+    return r;
+}
 // elements [p, p + n) of V; the others are `absent` (a bit pattern per word; n is 0, or V but for the ragged end of a row)
 template <class T, int V = VEC_OF<T>>
 __device__ __forceinline__ Raw<T, V> ld_raw(const T* p, int n, unsigned absent = 0u) {

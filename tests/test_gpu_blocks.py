@@ -136,7 +136,7 @@ def rec_check(args, kw, scale=8.0, dh_last=None, seed=99):
 
 
 @pytest.mark.parametrize("dtype", TYPES)
-@pytest.mark.parametrize("B,T,na,D", [(1, 1, 0, 1), (2, 3, 0, 64), (3, 65, 0, 7), (4, 81, 3, 24), (3, 128, 0, 65), (1, 200, 5, 33)])
+@pytest.mark.parametrize("B,T,na,D", [(1, 1, 0, 1), (2, 3, 0, 64), (3, 65, 0, 7), (4, 81, 3, 24), (3, 128, 0, 65), (1, 200, 5, 33), (2, 70, 0, 258), (3, 33, 0, 511), (1, 3, 0, 2)])
 def test_linrec_matches_the_definition(B, T, na, D, dtype):
     args, kw = rec_case(B, T, na, D, dtype, seed=100 + B * T + D)
     state = (B, na, D) if na else (B, D)
