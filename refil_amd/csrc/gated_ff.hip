@@ -43,7 +43,7 @@ __device__ __forceinline__ void gf_act_grad(int act, float v, float& f, float& d
     } else {
         const float s = fast_sigmoid(2.f * GF_A * (v + GF_B * v * v * v));
         f = v * s;
-        df = s + v * s * (1.f - s) * (2.f * GF_A) * (1.f + 3.f * GF_B * v * v);
+        df = s + v * s * (1.f - s) * (2.f * GF_A) * (1.f + 3.f * GF_B * fminf(v * v, 1e8f));      // (far out s (1 - s) is 0 and v^2 need not be Inf)
     }
 }
 
@@ -214,7 +214,7 @@ __global__ void __launch_bounds__(WM * WN * 64, WM * MT == 16 || sizeof(T) == 4 
         }
         auto stage = [&](int it, int buf) {
             const int k0 = it * BK;
-            const bool tail = k0 + BK > k.K;                  // (GF_K operands: chunks behind K are zeros of their own; wave-uniform)
+            const bool tail = k0 + BK > k.K;                  // (chunks behind K are zeros of their own; wave-uniform)
 #pragma unroll
             for (int i = 0; i < A_IT; ++i) {
                 const int e = (i * WAVES + wave) * 64 + lane, r = e / TA::CH;
@@ -229,6 +229,7 @@ __global__ void __launch_bounds__(WM * WN * 64, WM * MT == 16 || sizeof(T) == 4 
                 const int e = (i * WAVES + wave) * 64 + lane, r = e / TB::CH;
                 const T* p = LB == GF_K ? pb[i] + k0 : src + ob[i] + (long)min(kb + r, k.b_rows - 1) * k.ldb;
                 if (LB == GF_K && tail && k0 + ((e % TB::CH) ^ TB::swz(r)) * 8 >= k.K) p = (const T*)gf_zeros;
+                if (LB == GF_M && kb + BK > k.b_rows && kb + r >= k.b_rows) p = (const T*)gf_zeros;      // (times A's zeros: not another row's Inf)
                 gf_copy16(p, lb + buf * TB::BYTES + (i * WAVES + wave) * 1024);
             }
         };

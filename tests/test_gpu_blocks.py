@@ -584,6 +584,30 @@ def test_gated_ff_rows_do_not_mix():
     assert torch.isnan(dx[41]).all() and torch.isfinite(dx[keep]).all()
 
 
+@pytest.mark.parametrize("dtype", [BF16, F16])
+@pytest.mark.parametrize("N,F", [(130, 72), (70, 130)])
+def test_gated_ff_an_infinite_last_row_stays_where_it_is(N, F, dtype):
+    """the last row of a weight / of x is Inf, the tiles read whole 64-blocks of rows behind it: what it does not touch stays finite, and a
+    zero in front of it alone makes a NaN"""
+    D = 64
+    x, wg, wu = rnd(N, D, seed=1, dtype=dtype), rnd(F, D, seed=2, dtype=dtype, scale=0.1), rnd(F, D, seed=3, dtype=dtype, scale=0.1)
+    h, saved = blocks.gated_ff_forward(x, wg, wu, save=True)
+    dh = rnd(N, F, seed=4, dtype=dtype)
+    wi = wu.clone()
+    wi[-1, 5] = math.inf
+    dx = blocks.gated_ff_backward(dh, x, wg, wi, saved)[0]
+    clean = blocks.gated_ff_backward(dh, x, wg, wu, saved)[0]
+    others = torch.arange(D, device=DEV) != 5
+    assert torch.equal(dx[:, others], clean[:, others]) and torch.isinf(dx[:, 5]).all()
+    xi = x.clone()
+    xi[-1, 7] = -math.inf
+    _, dwg, dwu, _, _ = blocks.gated_ff_backward(dh, xi, wg, wu, saved)
+    _, cg, cu, _, _ = blocks.gated_ff_backward(dh, x, wg, wu, saved)
+    others = torch.arange(D, device=DEV) != 7
+    assert torch.equal(dwg[:, others], cg[:, others]) and torch.equal(dwu[:, others], cu[:, others])
+    assert torch.isinf(dwg[:, 7]).all() and torch.isinf(dwu[:, 7]).all()
+
+
 def test_gated_ff_autograd_and_differences():
     N, D, F = 5, 8, 6
     leaves = [t.requires_grad_(True) for t in (rnd(N, D, seed=1), rnd(F, D, seed=2), rnd(F, D, seed=3), rnd(F, seed=4), rnd(F, seed=5))]

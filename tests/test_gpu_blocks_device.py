@@ -106,18 +106,50 @@ def test_tensors_of_the_other_device_are_refused():
 
 
 def test_offsets_past_32_bits():
-    """a state pool and an activation whose last rows start past 2^32 elements' bytes: a row stride of 2^31 elements, four rows"""
+    """row and batch strides of 2^30 elements: the last rows start past 6 * 2^30 bytes"""
     n = 1 << 30
     pool = torch.empty(3 * n + 64, dtype=torch.bfloat16, device="cuda")
-    x = torch.as_strided(pool, (4, 2, 32), (n, 32, 1))                   # element offsets up to 3 * 2^30, byte offsets past 6 * 2^30
+    x = torch.as_strided(pool, (4, 2, 32), (n, 32, 1))
     g = torch.Generator(device="cuda").manual_seed(1)
     x.copy_(torch.randn(4, 2, 32, generator=g, device="cuda"))
     dense = x.contiguous()
     decay = torch.randn(32, generator=g, device="cuda") - 3
-    for a, b in zip(blocks.linrec_forward(x, x, x, decay, save=True), blocks.linrec_forward(dense, dense, dense, decay, save=True)):
-        assert torch.equal(a, b)
-    rows, drows = torch.as_strided(pool, (4, 32), (n, 1)), dense[:, 0].contiguous()
-    for a, b in zip(blocks.norm_gate_forward(rows, rows, rows), blocks.norm_gate_forward(drows, drows, drows)):
-        assert torch.equal(a, b)
+
+    def rec(t):
+        y, h, saved = blocks.linrec_forward(t, t, t, decay, save=True)
+        return [y, h, *blocks.linrec_backward(t, t, t, t, decay, saved), blocks.linrec_step(t[:, 0], t[:, 0], t[:, 0], decay, torch.zeros(4, 32, device="cuda"))]
+
+    def norm(t):
+        return [*blocks.norm_gate_forward(t, t, t), *blocks.norm_gate_backward(t, t, t, t, t)[:3]]
     w = torch.randn(40, 32, generator=g, device="cuda").to(torch.bfloat16)
-    assert torch.equal(blocks.gated_ff(rows, w, w), blocks.gated_ff(drows, w, w))
+
+    def ff(t):
+        h, saved = blocks.gated_ff_forward(t, w, w, save=True)
+        return [h, *blocks.gated_ff_backward(h, t, w, w, saved)[:3]]
+    for f, a, b in ((rec, x, dense), (norm, x[:, 0], dense[:, 0].contiguous()), (ff, x[:, 0], dense[:, 0].contiguous())):
+        assert all(torch.equal(p, q) for p, q in zip(f(a), f(b)))
+
+
+def test_more_than_two_to_the_31_elements():
+    """the last episode / rows of tensors of 2.2e9 elements against calls on them alone (other tile and chunk counts: to rounding)"""
+    B, T, D = 33, 8192, 8192
+    g = torch.Generator(device="cuda").manual_seed(2)
+    x = torch.empty(B, T, D, dtype=torch.bfloat16, device="cuda")
+    for b in range(B):
+        x[b] = torch.randn(T, D, generator=g, device="cuda")
+    decay = torch.randn(D, generator=g, device="cuda") - 5
+
+    def near(a, b):
+        torch.testing.assert_close(a, b, rtol=2 ** -7, atol=1e-3)        # (two roundings to bf16 apart at most)
+    y, h, _ = blocks.linrec_forward(x, x, x, decay)
+    y1, h1, _ = blocks.linrec_forward(x[-1:], x[-1:], x[-1:], decay)
+    near(y[-1], y1[0])
+    torch.testing.assert_close(h[-1], h1[0], rtol=1e-4, atol=1e-5)
+    rows = x.view(-1, D)
+    n = blocks.norm_gate_forward(rows, y.view(-1, D), want_y=False)[1]
+    near(n[-300:], blocks.norm_gate_forward(rows[-300:], y.view(-1, D)[-300:], want_y=False)[1])
+    del n, y
+    w = (torch.randn(D, 64, generator=g, device="cuda") * 0.1).to(torch.bfloat16)
+    narrow = rows[:, :64]
+    out = blocks.gated_ff(narrow, w, w)
+    near(out[-300:], blocks.gated_ff(narrow[-300:], w, w))
