@@ -251,24 +251,44 @@ __global__ void __launch_bounds__(WM * WN * 64, WM * MT == 16 || sizeof(T) == 4 
 #pragma unroll
             for (int q = 0; q < 8 / V; ++q) r[q] = ld_raw<T, V>(p + q * V, min(max(n - q * V, 0), V));
         };
+        // (whole tiles, wave-uniform: no predicates, so that the loads leave one behind the other)
         auto load = [&](int it) {
             const int k0 = it * BK;
+            const int ka = min(k.a_rows, k.K);
+            if (LA == GF_K ? m0 + BM <= k.M && k0 + BK <= k.K : m0 + BM <= k.M && k0 + BK <= ka) {
 #pragma unroll
-            for (int i = 0; i < A_IT; ++i) {
-                const int e = i * THREADS + (int)threadIdx.x, r = e / TA::CH, c = (e % TA::CH) * 8;
-                const int row = LA == GF_K ? m0 + r : k0 + r, col = LA == GF_K ? k0 + c : m0 + c;
-                const bool in = row < (LA == GF_K ? k.M : min(k.a_rows, k.K));
-                fetch(ra[i], (const T*)k.A + (long)(in ? row : 0) * k.lda + col, in ? (LA == GF_K ? k.K : k.M) - col : 0);
+                for (int i = 0; i < A_IT; ++i) {
+                    const int e = i * THREADS + (int)threadIdx.x, r = e / TA::CH, c = (e % TA::CH) * 8;
+                    fetch(ra[i], (const T*)k.A + (long)(LA == GF_K ? m0 + r : k0 + r) * k.lda + (LA == GF_K ? k0 + c : m0 + c), 8);
+                }
+            } else {
+#pragma unroll
+                for (int i = 0; i < A_IT; ++i) {
+                    const int e = i * THREADS + (int)threadIdx.x, r = e / TA::CH, c = (e % TA::CH) * 8;
+                    const int row = LA == GF_K ? m0 + r : k0 + r, col = LA == GF_K ? k0 + c : m0 + c;
+                    const bool in = row < (LA == GF_K ? k.M : ka);
+                    fetch(ra[i], (const T*)k.A + (long)(in ? row : 0) * k.lda + col, in ? (LA == GF_K ? k.K : k.M) - col : 0);
+                }
             }
             const T* src = (const T*)k.B0; int kb = k0;
             if (LB == GF_M && k0 >= k.ksplit) { src = (const T*)k.B1; kb -= k.ksplit; }
+            if (n0 + HALF <= k.N && (LB == GF_K ? k0 + BK <= k.K : kb + BK <= k.b_rows)) {
 #pragma unroll
-            for (int i = 0; i < B_IT; ++i) {
-                const int e = i * THREADS + (int)threadIdx.x, r = e / TB::CH, c = (e % TB::CH) * 8;
-                int row = kb + r; const int col = LB == GF_K ? k0 + c : n0 + c;
-                if (LB == GF_K) row = b_row(r, src);
-                const bool in = row < (LB == GF_K ? k.N : k.b_rows);
-                fetch(rb[i], src + (long)(in ? row : 0) * k.ldb + col, in ? (LB == GF_K ? k.K : k.N) - col : 0);
+                for (int i = 0; i < B_IT; ++i) {
+                    const int e = i * THREADS + (int)threadIdx.x, r = e / TB::CH, c = (e % TB::CH) * 8;
+                    int row = kb + r;
+                    if (LB == GF_K) row = b_row(r, src);
+                    fetch(rb[i], src + (long)row * k.ldb + (LB == GF_K ? k0 + c : n0 + c), 8);
+                }
+            } else {
+#pragma unroll
+                for (int i = 0; i < B_IT; ++i) {
+                    const int e = i * THREADS + (int)threadIdx.x, r = e / TB::CH, c = (e % TB::CH) * 8;
+                    int row = kb + r; const int col = LB == GF_K ? k0 + c : n0 + c;
+                    if (LB == GF_K) row = b_row(r, src);
+                    const bool in = row < (LB == GF_K ? k.N : k.b_rows);
+                    fetch(rb[i], src + (long)(in ? row : 0) * k.ldb + col, in ? (LB == GF_K ? k.K : k.N) - col : 0);
+                }
             }
         };
         auto put = [&](char* tile, int bytes, int slot, const Raw<T> (&r)[8 / V]) {
