@@ -100,11 +100,12 @@ __device__ __forceinline__ uint2 gf_read_tr(const char* p) {
 }
 
 // Geometry of one operand's LDS tile: ROWS rows of CH chunks of 16 bytes. Which chunk sits in which slot is permuted per row so that the
-// fragment reads meet no bank twice: GF_K rows (one chunk of 16 rows is read) slot = chunk ^ row bits; GF_M rows (32 bytes of eight rows
-// k, k + 1, .. k + 3, k + 8, .. are read) pairs of chunks ^ the row's bits 0, 1 and 3.
+// fragment reads meet no bank twice (the bank-conflict counter stays 0): GF_K rows (one chunk of 16 rows is read) slot = chunk ^ row bits, of
+// rows of four chunks minus row / 4, since a read takes rows 4 i from one half of the lanes with rows 4 i + 12 from the other; GF_M rows
+// (32 bytes of eight rows k, k + 1, .. k + 3, k + 8, .. are read) pairs of chunks ^ the row's bits 0, 1 and 3.
 template <int LAY, int DIM, int BK> struct GfTile {
     static constexpr int ROWS = LAY == GF_K ? DIM : BK, CH = (LAY == GF_K ? BK : DIM) / 8, BYTES = ROWS * CH * 16;
-    __device__ static int swz(int r) { return LAY == GF_K ? (CH == 8 ? (r & 7) : ((r >> 2) & 3)) : 2 * ((r & 3) | ((r >> 1) & 4)); }
+    __device__ static int swz(int r) { return LAY == GF_K ? (CH == 8 ? (r & 7) : (-(r >> 2) & 3)) : 2 * ((r & 3) | ((r >> 1) & 4)); }
     // fragment of the 16 m (n) behind 16 t, k = 32 kk + 8 (lane / 16) + 0..7
     __device__ static gf_u32x4 frag(const char* tile, int t, int kk, int lane) {
         const int g = lane >> 4, r = lane & 15;
@@ -583,13 +584,24 @@ static int gf_go(const GfGemm& k, hipStream_t st) {
     REFIL_LAUNCH_CHECK();
     return 0;
 }
+// Tiles of 32 MT rows instead of 128, where the last of the launch's rounds over the compute units is then so much fuller that fewer rows
+// pass in all: N 1537, D 520, F 1366 in fp16 21.2 against 24.3 us (forward, 374 tiles of 96 rows for 286), the backward of N 41472, D 128,
+// F 512 in fp32 218 against 222 us (dx, 648 tiles of 64 rows for 324).
+template <int MT>
+static bool gf_lower(const GfGemm& k, bool gated) {
+    const long cols = cdivl(k.N, gated ? 64 : 128);
+    return k.splits == 1 && cdivl(cdivl(k.M, 32 * MT) * cols, gf_cus()) * MT < cdivl(cdivl(k.M, 128) * cols, gf_cus()) * 4;
+}
 template <class T, int LA, int LB, bool GATED>
 static int gf_launch(GfGemm k, const GfPlan& p, hipStream_t st, const char* name, double flops, double bytes) {
     ProfScope ps(name, flops, bytes, st, nullptr, 0.0, sizeof(T) == 4 ? flops : 0.0);
     k.splits = p.splits;
     if constexpr (sizeof(T) == 2) {
         if (p.large) return gf_go<T, LA, LB, 2, 4, 8, 4, true, GATED>(k, st);
+        if constexpr (LA == GF_K) if (p.direct && gf_lower<3>(k, GATED)) return gf_go<T, LA, LB, 2, 2, 3, 4, true, GATED>(k, st);
         if (p.direct) return gf_go<T, LA, LB, 2, 2, 4, 4, true, GATED>(k, st);
+    } else if constexpr (LA == GF_K && !GATED) {
+        if (gf_lower<2>(k, GATED)) return gf_go<T, LA, LB, 2, 2, 2, 4, false, GATED>(k, st);
     }
     return gf_go<T, LA, LB, 2, 2, 4, 4, false, GATED>(k, st);
 }

@@ -554,6 +554,15 @@ def test_gated_ff_large_tiles(dtype):
     ff_check(x, wg, wu, rnd(F, seed=10, dtype=dtype), rnd(F, seed=11, dtype=dtype), "silu")
 
 
+@pytest.mark.parametrize("dtype", TYPES)
+def test_gated_ff_whole_rounds_of_tiles(dtype):
+    """rows and columns whose 128-row tiles fill the compute units evenly (the shorter tiles would not), forward and dx; and the ragged middle"""
+    k = 1 if DEV == "cuda" else 8
+    for N, D, F in ((1024 // k, 64, 1920 // k), (1024 // k, 3840 // k, 64), (1400 // k, 72, 1920 // k)):
+        x, wg, wu = rnd(N, D, seed=1, dtype=dtype), rnd(F, D, seed=2, dtype=dtype, scale=D ** -0.5), rnd(F, D, seed=3, dtype=dtype, scale=D ** -0.5)
+        ff_check(x, wg, wu, rnd(F, seed=4, dtype=dtype), rnd(F, seed=5, dtype=dtype), "silu")
+
+
 def test_gated_ff_shapes_and_strides():
     """agents' rows [B, T, na, D] cut out of wider rows, both weights in one fused matrix with padding, one bias alone, rows expanded over one"""
     D, F = 24, 20
