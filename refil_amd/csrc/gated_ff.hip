@@ -8,7 +8,9 @@
 //             is the row, the LDS tile keeps rows of k and ds_read_b64_tr_b16 hands the matrix core its columns -- nothing is transposed
 // fp32 operands are split exactly into three bf16 pieces on their way into LDS and a product runs as six bf16 products (lo hi, hi lo,
 // mid mid, mid hi, hi mid, hi hi), as the library's projection GEMMs do.
-// Up to 64 rows the weights' bytes are the cost and a second kernel reads them once, straight into matrix-core fragments.
+// Few rows, where the weights' bytes are the cost, and launches of few tiles have a second kernel that reads straight into matrix-core fragments.
+#include <type_traits>
+
 #include "kernels.h"
 #include "profile.h"
 #include "split.h"
@@ -248,47 +250,79 @@ __global__ void __launch_bounds__(WM * WN * 64, WM * MT == 16 || sizeof(T) == 4 
         char* const sa = gf_smem; char* const sb = gf_smem + P * TA::BYTES;
         Raw<T> ra[A_IT][8 / VEC_OF<T>], rb[B_IT][8 / VEC_OF<T>];
         constexpr int V = VEC_OF<T>;
-        auto fetch = [&](Raw<T> (&r)[8 / V], const T* p, int n) {
+        // Eight elements from column `col` of a row of `cols` on. WHOLE (wave-uniform): all there. At an edge a lane reads from where it may -- V
+        // columns inside the row, the last row that exists -- and puts right what it got, zeros behind the end (`mend`): no branches, so that the
+        // loads leave one behind the other and are waited for once. Rows of fewer than V columns go element by element.
+        enum { WHOLE, EDGE, FEW };
+        auto fetch = [&](auto way, Raw<T> (&r)[8 / V], const T* row, int col, int cols) {
 #pragma unroll
-            for (int q = 0; q < 8 / V; ++q) r[q] = ld_raw<T, V>(p + q * V, min(max(n - q * V, 0), V));
+            for (int q = 0; q < 8 / V; ++q) {
+                const int c = col + q * V;
+                if (way == WHOLE) r[q] = ld_raw<T, V>(row + c, V);
+                else if (way == EDGE) r[q] = ld_raw<T, V>(row + min(c, cols - V), V);
+                else r[q] = ld_raw<T, V>(row + (c < cols ? c : 0), c < cols ? cols - c : 0);
+            }
         };
-        // (whole tiles, wave-uniform: no predicates, so that the loads leave one behind the other)
+        auto mend = [&](Raw<T> (&r)[8 / V], int col, int cols, bool in) {
+#pragma unroll
+            for (int q = 0; q < 8 / V; ++q) {
+                const int back = cols >= V ? max(col + q * V - (cols - V), 0) : 0;
+                r[q] = raw_down<T, V>(r[q], min(back, V - 1));
+#pragma unroll
+                for (int w = 0; w < (int)(sizeof(r[q].w) / 4); ++w) r[q].w[w] = in && back < V ? r[q].w[w] : 0u;
+            }
+        };
+        auto load_a = [&](auto way, int k0) {
+            const int rows = LA == GF_K ? k.M : min(k.a_rows, k.K), cols = LA == GF_K ? k.K : k.M, r0 = LA == GF_K ? m0 : k0, c0 = LA == GF_K ? k0 : m0;
+#pragma unroll
+            for (int i = 0; i < A_IT; ++i) {
+                const int e = i * THREADS + (int)threadIdx.x, r = e / TA::CH, c = (e % TA::CH) * 8;
+                fetch(way, ra[i], (const T*)k.A + (long)(way == WHOLE ? r0 + r : min(r0 + r, rows - 1)) * k.lda, c0 + c, cols);
+            }
+        };
+        auto load_b = [&](auto way, const T* src, int kb) {
+            const int rows = LB == GF_K ? k.N : k.b_rows, cols = LB == GF_K ? k.K : k.N, c0 = LB == GF_K ? kb : n0;
+#pragma unroll
+            for (int i = 0; i < B_IT; ++i) {
+                const int e = i * THREADS + (int)threadIdx.x, r = e / TB::CH, c = (e % TB::CH) * 8;
+                int row = kb + r;
+                if (LB == GF_K) row = b_row(r, src);
+                fetch(way, rb[i], src + (long)(way == WHOLE ? row : min(row, rows - 1)) * k.ldb, c0 + c, cols);
+            }
+        };
         auto load = [&](int it) {
             const int k0 = it * BK;
-            const int ka = min(k.a_rows, k.K);
-            if (LA == GF_K ? m0 + BM <= k.M && k0 + BK <= k.K : m0 + BM <= k.M && k0 + BK <= ka) {
-#pragma unroll
-                for (int i = 0; i < A_IT; ++i) {
-                    const int e = i * THREADS + (int)threadIdx.x, r = e / TA::CH, c = (e % TA::CH) * 8;
-                    fetch(ra[i], (const T*)k.A + (long)(LA == GF_K ? m0 + r : k0 + r) * k.lda + (LA == GF_K ? k0 + c : m0 + c), 8);
-                }
-            } else {
-#pragma unroll
-                for (int i = 0; i < A_IT; ++i) {
-                    const int e = i * THREADS + (int)threadIdx.x, r = e / TA::CH, c = (e % TA::CH) * 8;
-                    const int row = LA == GF_K ? m0 + r : k0 + r, col = LA == GF_K ? k0 + c : m0 + c;
-                    const bool in = row < (LA == GF_K ? k.M : ka);
-                    fetch(ra[i], (const T*)k.A + (long)(in ? row : 0) * k.lda + col, in ? (LA == GF_K ? k.K : k.M) - col : 0);
-                }
-            }
+            typedef std::integral_constant<int, WHOLE> Whole;
+            typedef std::integral_constant<int, EDGE> Edge;
+            typedef std::integral_constant<int, FEW> Few;
+            if (m0 + BM <= k.M && k0 + BK <= (LA == GF_K ? k.K : min(k.a_rows, k.K))) load_a(Whole(), k0);
+            else if ((LA == GF_K ? k.K : k.M) >= V) load_a(Edge(), k0);
+            else load_a(Few(), k0);
             const T* src = (const T*)k.B0; int kb = k0;
             if (LB == GF_M && k0 >= k.ksplit) { src = (const T*)k.B1; kb -= k.ksplit; }
-            if (n0 + HALF <= k.N && (LB == GF_K ? k0 + BK <= k.K : kb + BK <= k.b_rows)) {
+            if (n0 + HALF <= k.N && kb + BK <= (LB == GF_K ? k.K : k.b_rows)) load_b(Whole(), src, kb);
+            else if ((LB == GF_K ? k.K : k.N) >= V) load_b(Edge(), src, kb);
+            else load_b(Few(), src, kb);
+        };
+        // (rows of m or n that are not there need no zeros: what they give is not stored)
+        auto fix = [&](int it) {
+            const int k0 = it * BK;
+            {
+                const int rows = min(k.a_rows, k.K), cols = LA == GF_K ? k.K : k.M, c0 = LA == GF_K ? k0 : m0;
+                if (c0 + (LA == GF_K ? BK : BM) > cols || (LA == GF_M && k0 + BK > rows)) {
 #pragma unroll
-                for (int i = 0; i < B_IT; ++i) {
-                    const int e = i * THREADS + (int)threadIdx.x, r = e / TB::CH, c = (e % TB::CH) * 8;
-                    int row = kb + r;
-                    if (LB == GF_K) row = b_row(r, src);
-                    fetch(rb[i], src + (long)row * k.ldb + (LB == GF_K ? k0 + c : n0 + c), 8);
+                    for (int i = 0; i < A_IT; ++i) {
+                        const int e = i * THREADS + (int)threadIdx.x, r = e / TA::CH, c = (e % TA::CH) * 8;
+                        mend(ra[i], c0 + c, cols, LA == GF_K || k0 + r < rows);
+                    }
                 }
-            } else {
+            }
+            const int kb = LB == GF_M && k0 >= k.ksplit ? k0 - k.ksplit : k0, cols = LB == GF_K ? k.K : k.N, c0 = LB == GF_K ? k0 : n0;
+            if (c0 + (LB == GF_K ? BK : BN) > cols || (LB == GF_M && kb + BK > k.b_rows)) {
 #pragma unroll
                 for (int i = 0; i < B_IT; ++i) {
                     const int e = i * THREADS + (int)threadIdx.x, r = e / TB::CH, c = (e % TB::CH) * 8;
-                    int row = kb + r; const int col = LB == GF_K ? k0 + c : n0 + c;
-                    if (LB == GF_K) row = b_row(r, src);
-                    const bool in = row < (LB == GF_K ? k.N : k.b_rows);
-                    fetch(rb[i], src + (long)(in ? row : 0) * k.ldb + col, in ? (LB == GF_K ? k.K : k.N) - col : 0);
+                    mend(rb[i], c0 + c, cols, LB == GF_K || kb + r < k.b_rows);
                 }
             }
         };
@@ -305,6 +339,7 @@ __global__ void __launch_bounds__(WM * WN * 64, WM * MT == 16 || sizeof(T) == 4 
         };
         if (it0 < it1) load(it0);
         for (int it = it0; it < it1; ++it) {
+            fix(it);
             lds_barrier();                  // the products of the tile before have been read
 #pragma unroll
             for (int i = 0; i < A_IT; ++i) {
@@ -351,9 +386,13 @@ __global__ void __launch_bounds__(WM * WN * 64, WM * MT == 16 || sizeof(T) == 4 
     }
 }
 
-// ---- few rows: every weight is read once, straight into fragments ----
-// A workgroup owns 16 columns of h, its eight waves share the reduction; a lane reads 16 neighbouring k (two matrix steps) of one weight
-// row, so that a row's reads are whole cache lines -- the order of k inside a product is free as long as both operands share it.
+// ---- few rows, or few tiles: straight into fragments ----
+// A workgroup owns 16 columns of h and 16 MT rows, its eight waves share the reduction; a lane reads 16 neighbouring k (two matrix steps)
+// of one weight row, so that a row's reads are whole cache lines -- the order of k inside a product is free as long as both operands share
+// it. Up to 64 rows every weight is read once: N 16, D 1024, F 4096 in bf16 5.6 us, 16.8 MB, bound by the launch and one round of latency
+// (fp32, N 3, D 3019, F 4313: 104 MB at 3.6 TB/s). With more rows the weights come again from the L2, but eight waves share what one
+// workgroup of the tiled kernel would walk alone: taken while that kernel would fill no more than a quarter of the compute units (N 200,
+// D 1000, F 1000 in fp32, 32 tiles: 17 against 63 us; N 245, D 257, F 3220, 102 tiles: 33 against 24).
 template <class T, int MT>
 __global__ void __launch_bounds__(512) gf_skinny(const GfGemm k) {
     typedef typename GfElem<T>::type E;
@@ -361,17 +400,18 @@ __global__ void __launch_bounds__(512) gf_skinny(const GfGemm k) {
     __shared__ float s_acc[8][2][MT][64][4];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6), r = lane & 15, g = lane >> 4;
     const int n0 = blockIdx.x * 16;
-    const bool in_n = n0 + r < k.N;
-    const T* pg = (const T*)k.B0 + (long)(in_n ? n0 + r : 0) * k.ldb;
-    const T* pu = (const T*)k.B1 + (long)(in_n ? n0 + r : 0) * k.ldb;
+    const int mb = blockIdx.y * 16 * MT;
+    const T* pg = (const T*)k.B0 + (long)min(n0 + r, k.N - 1) * k.ldb;
+    const T* pu = (const T*)k.B1 + (long)min(n0 + r, k.N - 1) * k.ldb;
     f32x4 acc[2][MT];
 #pragma unroll
     for (int z = 0; z < 2; ++z)
 #pragma unroll
         for (int i = 0; i < MT; ++i) acc[z][i] = f32x4{0.f, 0.f, 0.f, 0.f};
-    auto fetch = [&](Raw<T> (&o)[Q], const T* p, int k0, bool in) {
+    // (columns of h and rows of x that are not there read the last one: what they give is not stored)
+    auto fetch = [&](auto whole, Raw<T> (&o)[Q], const T* p, int k0) {
 #pragma unroll
-        for (int q = 0; q < Q; ++q) o[q] = ld_raw<T, V>(p + k0 + q * V, in ? min(max(k.K - k0 - q * V, 0), V) : 0);
+        for (int q = 0; q < Q; ++q) o[q] = ld_raw<T, V>(p + (whole || k0 + q * V < k.K ? k0 + q * V : 0), whole ? V : min(max(k.K - k0 - q * V, 0), V));
     };
     auto planes = [&](const Raw<T> (&o)[Q], int half, gf_u32x4 (&f)[P]) {
         if constexpr (P == 1) f[0] = gf_u32x4{o[half].w[0], o[half].w[1], o[half].w[2], o[half].w[3]};
@@ -387,13 +427,14 @@ __global__ void __launch_bounds__(512) gf_skinny(const GfGemm k) {
     for (int kb = wave * 64; kb < k.K; kb += 8 * 64) {
         const int k0 = kb + g * 16;
         Raw<T> wg[Q], wu[Q], x[MT][Q];
-        fetch(wg, pg, k0, in_n);
-        fetch(wu, pu, k0, in_n);
+        auto load = [&](auto whole) {
+            fetch(whole, wg, pg, k0);
+            fetch(whole, wu, pu, k0);
 #pragma unroll
-        for (int i = 0; i < MT; ++i) {
-            const int m = i * 16 + r;
-            fetch(x[i], (const T*)k.A + (long)min(m, k.M - 1) * k.lda, k0, m < k.M);
-        }
+            for (int i = 0; i < MT; ++i) fetch(whole, x[i], (const T*)k.A + (long)min(mb + i * 16 + r, k.M - 1) * k.lda, k0);
+        };
+        if (kb + 64 <= k.K) load(std::true_type());
+        else load(std::false_type());
 #pragma unroll
         for (int half = 0; half < 2; ++half) {
             gf_u32x4 fg[P], fu[P];
@@ -432,7 +473,7 @@ __global__ void __launch_bounds__(512) gf_skinny(const GfGemm k) {
                 for (int w = 0; w < 8; ++w) t += s_acc[w][z][wave][lane][q];
                 a[z][q] = t;
             }
-        const int m = wave * 16 + r, n = n0 + g * 4;
+        const int m = mb + wave * 16 + r, n = n0 + g * 4;
         if (m < k.M) gf_gated_out<T>(k, m, n, min(max(k.N - n, 0), 4), a[0], a[1]);
     }
 }
@@ -566,7 +607,7 @@ static GfPlan gf_plan(long M, long N, long K, int bk, bool direct) {
     p.large = direct && cdivl(M, 256) * cdivl(N, 256) >= gf_cus() / 2;
     const long b = p.large ? 256 : 128, tiles = cdivl(M, b) * cdivl(N, b), iters = cdivl(K, bk);
     long s = tiles >= gf_cus() ? 1 : 2L * gf_cus() / tiles;
-    if (s > iters / 8) s = iters / 8;
+    if (s > iters / 4) s = iters / 4;          // (the backward of N 339, D 260, F 294 in fp32: 33 us, 63 with eight blocks each; 1220, 310, 253 in bf16: 34 for 47)
     if (s > 64) s = 64;
     p.splits = s < 1 ? 1 : (int)s;
     return p;
@@ -635,9 +676,9 @@ static int gf_forward(const refil_gated_ff_desc& d, hipStream_t st) {
     k.C0 = d.h; k.ldc = d.h_stride; k.bias0 = d.b_gate; k.bias1 = d.b_up; k.act = d.act;
     k.save0 = d.saved; k.save1 = d.saved ? d.saved + d.N * d.F : nullptr;
     const double nf = (double)d.N * d.F, fl = 4 * nf * d.D, by = sizeof(T) * ((double)d.N * d.D + 2.0 * d.F * d.D + nf) + (d.saved ? 8 * nf : 0);
-    if (d.N <= 64) {
+    if (d.N <= 64 || cdivl(d.N, 128) * cdivl(d.F, 64) <= gf_cus() / 4) {
         ProfScope ps("gated_ff_few_rows", fl, by, st, nullptr, 0.0, sizeof(T) == 4 ? fl : 0.0);
-        const dim3 grid(cdiv(d.F, 16));
+        const dim3 grid(cdiv(d.F, 16), cdiv((int)d.N, 64));
         if (d.N <= 16) hipLaunchKernelGGL((gf_skinny<T, 1>), grid, dim3(512), 0, st, k);
         else if (d.N <= 32) hipLaunchKernelGGL((gf_skinny<T, 2>), grid, dim3(512), 0, st, k);
         else hipLaunchKernelGGL((gf_skinny<T, 4>), grid, dim3(512), 0, st, k);

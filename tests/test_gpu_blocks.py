@@ -556,9 +556,10 @@ def test_gated_ff_large_tiles(dtype):
 
 @pytest.mark.parametrize("dtype", TYPES)
 def test_gated_ff_whole_rounds_of_tiles(dtype):
-    """rows and columns whose 128-row tiles fill the compute units evenly (the shorter tiles would not), forward and dx; and the ragged middle"""
+    """rows and columns whose 128-row tiles fill the compute units evenly (the shorter tiles would not), forward and dx; the ragged middle; odd
+    widths, and rows shorter than a 16-byte load, in as many tiles"""
     k = 1 if DEV == "cuda" else 8
-    for N, D, F in ((1024 // k, 64, 1920 // k), (1024 // k, 3840 // k, 64), (1400 // k, 72, 1920 // k)):
+    for N, D, F in ((1024 // k, 64, 1920 // k), (1024 // k, 3840 // k, 64), (1400 // k, 72, 1920 // k), (700 // k, 37, 1000), (700 // k, 5, 1000), (700 // k, 3, 1001)):
         x, wg, wu = rnd(N, D, seed=1, dtype=dtype), rnd(F, D, seed=2, dtype=dtype, scale=D ** -0.5), rnd(F, D, seed=3, dtype=dtype, scale=D ** -0.5)
         ff_check(x, wg, wu, rnd(F, seed=4, dtype=dtype), rnd(F, seed=5, dtype=dtype), "silu")
 
