@@ -401,6 +401,9 @@ __global__ void __launch_bounds__(512) gf_skinny(const GfGemm k) {
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6), r = lane & 15, g = lane >> 4;
     const int n0 = blockIdx.x * 16;
     const int mb = blockIdx.y * 16 * MT;
+    // (16-bit rows that begin inside a word: 16-byte loads of them cost three times the aligned ones here, where a load's lanes lie in 16 rows --
+    // N 170, D 3317, F 791 in bf16 51 us, 25 by whole words, D 3320 17 -- but are the cheaper ones in the tiled kernel, whose lanes follow a row)
+    const bool odd_rows = (((size_t)k.A | (size_t)k.B0 | (size_t)k.B1 | (size_t)(k.lda * 2) | (size_t)(k.ldb * 2)) & 3) != 0;
     const T* pg = (const T*)k.B0 + (long)min(n0 + r, k.N - 1) * k.ldb;
     const T* pu = (const T*)k.B1 + (long)min(n0 + r, k.N - 1) * k.ldb;
     f32x4 acc[2][MT];
@@ -409,9 +412,25 @@ __global__ void __launch_bounds__(512) gf_skinny(const GfGemm k) {
 #pragma unroll
         for (int i = 0; i < MT; ++i) acc[z][i] = f32x4{0.f, 0.f, 0.f, 0.f};
     // (columns of h and rows of x that are not there read the last one: what they give is not stored)
-    auto fetch = [&](auto whole, Raw<T> (&o)[Q], const T* p, int k0) {
+    enum { WHOLE, ODD, RAGGED };
+    auto fetch = [&](auto way, Raw<T> (&o)[Q], const T* p, int k0) {
+        if constexpr (way == ODD) {
+            // Lanes whose 16 elements begin in the middle of a word read the words around them -- the element in front is the row before, or at
+            // the first row the storage's: an address that is no multiple of four is not its beginning -- and the last element by itself
+            typedef unsigned U4 __attribute__((ext_vector_type(4), aligned(4)));
+            p += k0;
+            const unsigned odd = ((unsigned)(size_t)p >> 1) & 1;
+            const U4 a = *reinterpret_cast<const U4*>(p - odd), b = *reinterpret_cast<const U4*>(p + 8 - odd);
+            const unsigned e[9] = {a[0], a[1], a[2], a[3], b[0], b[1], b[2], b[3], *reinterpret_cast<const unsigned short*>(p + 15)};
 #pragma unroll
-        for (int q = 0; q < Q; ++q) o[q] = ld_raw<T, V>(p + (whole || k0 + q * V < k.K ? k0 + q * V : 0), whole ? V : min(max(k.K - k0 - q * V, 0), V));
+            for (int i = 0; i < 8; ++i) o[i / 4].w[i % 4] = odd ? (e[i] >> 16) | (e[i + 1] << 16) : e[i];
+        } else {
+#pragma unroll
+            for (int q = 0; q < Q; ++q) {
+                const int c = k0 + q * V;
+                o[q] = ld_raw<T, V>(p + (way == WHOLE || c < k.K ? c : 0), way == WHOLE ? V : min(max(k.K - c, 0), V));
+            }
+        }
     };
     auto planes = [&](const Raw<T> (&o)[Q], int half, gf_u32x4 (&f)[P]) {
         if constexpr (P == 1) f[0] = gf_u32x4{o[half].w[0], o[half].w[1], o[half].w[2], o[half].w[3]};
@@ -427,14 +446,15 @@ __global__ void __launch_bounds__(512) gf_skinny(const GfGemm k) {
     for (int kb = wave * 64; kb < k.K; kb += 8 * 64) {
         const int k0 = kb + g * 16;
         Raw<T> wg[Q], wu[Q], x[MT][Q];
-        auto load = [&](auto whole) {
-            fetch(whole, wg, pg, k0);
-            fetch(whole, wu, pu, k0);
+        auto load = [&](auto way) {
+            fetch(way, wg, pg, k0);
+            fetch(way, wu, pu, k0);
 #pragma unroll
-            for (int i = 0; i < MT; ++i) fetch(whole, x[i], (const T*)k.A + (long)min(mb + i * 16 + r, k.M - 1) * k.lda, k0);
+            for (int i = 0; i < MT; ++i) fetch(way, x[i], (const T*)k.A + (long)min(mb + i * 16 + r, k.M - 1) * k.lda, k0);
         };
-        if (kb + 64 <= k.K) load(std::true_type());
-        else load(std::false_type());
+        if (kb + 64 > k.K) load(std::integral_constant<int, RAGGED>());
+        else if (sizeof(T) == 2 && odd_rows) { if constexpr (sizeof(T) == 2) load(std::integral_constant<int, ODD>()); }
+        else load(std::integral_constant<int, WHOLE>());
 #pragma unroll
         for (int half = 0; half < 2; ++half) {
             gf_u32x4 fg[P], fu[P];
