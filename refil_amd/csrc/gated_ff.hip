@@ -53,13 +53,14 @@ __device__ __forceinline__ void gf_act_grad(int act, float v, float& f, float& d
 // ---- the tiled product ----
 enum { GF_K = 0, GF_M = 1 };       // an operand's contiguous index: k (rows are m / n) or m / n (rows are k)
 
+__host__ __device__ inline long gf_ldp(int n) { return (n + 3) / 4 * 4; }      // (whole vectors of four: neither side of the partial sums has a ragged end)
 struct GfGemm {
     const void* A; long lda;
     const void* B0; const void* B1; long ldb;      // gated: B1 = the up projection; else rows of k at and behind ksplit come from B1
     int M, N, K;
     int a_rows, b_rows;                            // rows that exist of A, of each B (GF_M operands; GF_K: M, N)
     int ksplit;
-    int splits; float* partial;                    // splits > 1: fp32 partial sums [splits][M][N]
+    int splits; float* partial;                    // splits > 1: fp32 partial sums [splits][M][gf_ldp(N)]
     void* C0; void* C1; long ldc; int msplit, mlim;      // rows m < msplit: row m of C0; the others: row m - msplit of C1; rows at or behind mlim of either are padding
     const void* bias0; const void* bias1; float* save0; float* save1; int act;      // gated epilogue
 };
@@ -375,7 +376,7 @@ __global__ void __launch_bounds__(WM * WN * 64, WM * MT == 16 || sizeof(T) == 4 
                 float v[4];
 #pragma unroll
                 for (int r = 0; r < 4; ++r) v[r] = acc[i][j][r];
-                if (k.splits > 1) st_raw<float, 4>(k.partial + ((long)split * k.M + m) * k.N + n, raw_pack<float, 4>(v), c);
+                if (k.splits > 1) st_raw<float, 4>(k.partial + ((long)split * k.M + m) * gf_ldp(k.N) + n, raw_pack<float, 4>(v), c ? 4 : 0);
                 else {
                     const bool first = m < k.msplit;
                     const int row = first ? m : m - k.msplit;
@@ -558,18 +559,18 @@ struct GfFinish { GfGemm dx, dw; int dx_blocks, dw_blocks; const float* colsum; 
 template <class T>
 __device__ __forceinline__ void gf_reduce(const GfGemm& k, unsigned block, unsigned blocks) {
     const unsigned q = (unsigned)cdiv(k.N, 4), n = (unsigned)k.M * q;          // (fewer tiles than compute units: far below 2^32)
-    const long plane = (long)k.M * k.N;
+    const long plane = k.M * gf_ldp(k.N);
     for (unsigned e = block * 256 + threadIdx.x; e < n; e += blocks * 256) {
         const int m = (int)(e / q), c0 = (int)(e - (unsigned)m * q) * 4, c = min(k.N - c0, 4);
         const bool first = m < k.msplit;
         const int row = first ? m : m - k.msplit;
         if (row >= k.mlim) continue;
-        const float* p = k.partial + (long)m * k.N + c0;
+        const float* p = k.partial + m * gf_ldp(k.N) + c0;
         float s[4] = {0.f, 0.f, 0.f, 0.f};
         for (int z = 0; z < k.splits; z += 8) {
             Raw<float> v[8];
 #pragma unroll
-            for (int j = 0; j < 8; ++j) v[j] = ld_raw<float>(p + min(z + j, k.splits - 1) * plane, c);
+            for (int j = 0; j < 8; ++j) v[j] = ld_raw<float>(p + min(z + j, k.splits - 1) * plane, 4);
 #pragma unroll
             for (int j = 0; j < 8; ++j)
 #pragma unroll
@@ -682,8 +683,8 @@ static GfBwdWs gf_bwd_ws(const refil_gated_ff_desc& d, void* base) {
     w.colsum = (float*)take((size_t)w.row_blocks * 2 * d.F * 4);
     w.px = gf_plan(d.N, d.D, 2 * w.Fp, bk, direct);
     w.pw = gf_plan(2 * w.Fp, d.D, w.Np, bk, direct);
-    if (w.px.splits > 1) w.part_x = (float*)take((size_t)4 * w.px.splits * d.N * d.D);
-    if (w.pw.splits > 1) w.part_w = (float*)take((size_t)4 * w.pw.splits * 2 * w.Fp * d.D);
+    if (w.px.splits > 1) w.part_x = (float*)take((size_t)4 * w.px.splits * d.N * gf_ldp(d.D));
+    if (w.pw.splits > 1) w.part_w = (float*)take((size_t)4 * w.pw.splits * 2 * w.Fp * gf_ldp(d.D));
     w.bytes = n;
     return w;
 }
