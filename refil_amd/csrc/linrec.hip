@@ -5,15 +5,20 @@
 //
 // The gates do not read h, so a step is the affine map h -> A h + H and maps compose: (A2, H2) o (A1, H1) = (A2 A1, A2 H1 + H2). Time is
 // cut three times: a thread composes S consecutive steps, a wave its 64 / TC time-threads by shuffles, a workgroup its four waves through
-// LDS; the carry goes from 64-step tile to tile in registers. A reset cuts the chain: it travels beside the map as a flag instead of as
+// LDS; the carry goes from tile to tile (16 to 64 steps) in registers. A reset cuts the chain: it travels beside the map as a flag instead of as
 // A = 0, so that a NaN or Inf in front of it does not pass (0 * NaN).
 //
 // Backward: with g_t the whole gradient of h_t, g_t = dy_t + c_t and c_{t-1} = a_t g_t [no reset at t] -- the same maps A in reverse
 // order, R_t in H_t's place. h_{t-1} is computed again from the fp32 state that the forward keeps at every tile's start (one value per
-// 32 or 64 steps), not read from the rounded y: no 16-bit rounding enters the gradient, and 7 streams move where reading y would make 8.
+// 16 to 64 steps), not read from the rounded y: no 16-bit rounding enters the gradient, and 7 streams move where reading y would make 8.
 // The gate gradients come without a division by sqrt(1 - a^2):
 //   q_t = d loss / d log L_t = g_t (sigmoid(gi) x a^2 L / sqrt(1 - a^2) - a h_{t-1} L),   L / sqrt(1 - a^2) -> sqrt(L / 2) -> 0
 //   dga_t = q_t (1 - sigmoid(ga)),   ddecay = sum q_t sigmoid(decay) / softplus(decay)
+//
+// Bound by memory and by the latency of a tile (gates, shuffles, one barrier), which other waves of the compute unit hide. 96 ragged
+// episodes of 81 steps, 1024 channels in fp32: 31 + 48 us. Where sequences are too few to fill the card, time is cut into chunks, one round
+// of workgroups in all: a first launch makes the chunks' maps (3 streams read; backward 2), the second starts every chunk from the maps in
+// front of it. 4 sequences of 8192 steps, 1024 channels in bf16: 50 + 64 us forward (4.0 and 4.2 TB/s), 30 + 113 us backward.
 #include <type_traits>
 
 #include "kernels.h"

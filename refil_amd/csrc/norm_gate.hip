@@ -10,8 +10,13 @@
 //   f  = d s sigmoid(g),  e2 = f w_post:                        do = (e2 - oh mean(e2 oh)) / rms(o)
 //   dg = f oh w_post (1 - sigmoid(g)),  dw_post = sum f oh,  ds = sum d sigmoid(g) oh w_post,  dw_pre = sum dn yh
 // y is computed again from x, o and g (no more bytes than reading it, and unrounded); mean(e yh) and the sum of y^2 share one reduction.
-// The column sums stay in registers over a workgroup's rows, are joined in LDS, and a second launch adds the workgroups' partial rows in
-// a fixed order: no atomics, the same result every time.
+// The column sums stay in registers (the widest rows: in LDS) over a workgroup's rows, are joined in LDS, and a second launch adds the
+// workgroups' partial rows in a fixed order: no atomics, the same result every time.
+//
+// Bound by memory: N 16384, D 2048 in bf16 with a gate takes 64 us forward (5 streams, 5.2 TB/s) and 101 us backward (8 streams, 5.3 TB/s; a
+// large copy reaches 4.7 .. 4.9), N 41472, D 128 in fp32 with a fifth of its rows masked 17.7 + 31 us. Narrow rows share a workgroup so
+// that a wave's loads stay whole lines; the next row's loads leave in front of this row's sums, which is what keeps memory busy through the
+// barriers. Few rows (N 128, D 64: 3.8 us) are a launch and one round of latency.
 #include "kernels.h"
 #include "profile.h"
 #include "vecio.h"
@@ -66,6 +71,10 @@ __device__ __forceinline__ void row_sums(float (&v)[NS], float* s_red, int& turn
     }
 }
 
+// rows of 1024 threads: one workgroup fills a compute unit and its registers, so the column sums lie in LDS as far as it reaches (backward
+// of N 8000, D 8192 in bf16 249 us = 4.2 TB/s, 417 with them in registers; N 2707, D 4505 in fp32 146 and 190)
+template <class T> constexpr bool ng_col_lds(int tpr, int k, bool bwd) { return bwd && tpr == 1024 && 12 * tpr * k * VEC_OF<T> <= 128 * 1024; }
+
 template <class T, int K>
 struct NgRow { Raw<T> x[K], o[K], g[K]; };
 template <class T, int K>
@@ -112,12 +121,19 @@ __global__ void __launch_bounds__(TPR > 256 ? TPR : 256) norm_gate_kernel(const 
         back[j] = ragged && nv[j] > 0 ? VEC - nv[j] : 0;
         if constexpr (WEIGHTS) weights(j, wp[j], sc[j], wq[j]);
     }
-    float awp[BWD ? K : 1][VEC], asc[BWD ? K : 1][VEC], awq[BWD ? K : 1][VEC];
+    constexpr bool COL_LDS = ng_col_lds<T>(TPR, K, BWD);
+    constexpr int KA = BWD && !COL_LDS ? K : 1;
+    extern __shared__ __attribute__((aligned(16))) char ng_smem[];
+    f32x4* const s_acc = reinterpret_cast<f32x4*>(ng_smem) + threadIdx.x;       // [3][K][VEC / 4][TPR], a thread's own columns
+    float awp[KA][VEC], asc[KA][VEC], awq[KA][VEC];
     if (BWD) {
 #pragma unroll
-        for (int j = 0; j < K; ++j)
+        for (int j = 0; j < KA; ++j)
 #pragma unroll
             for (int i = 0; i < VEC; ++i) awp[j][i] = asc[j][i] = awq[j][i] = 0.f;
+        if constexpr (COL_LDS) {
+            for (int e = 0; e < 3 * K * VEC / 4; ++e) s_acc[e * TPR] = f32x4{0.f, 0.f, 0.f, 0.f};
+        }
     }
     NgRow<T, K> a;
     NgGrad<T, BWD ? K : 1> b;
@@ -221,11 +237,23 @@ __global__ void __launch_bounds__(TPR > 256 ? TPR : 256) norm_gate_kernel(const 
                     const float dd = raw_get(d.dy[j], i) + irms_y * (dn * wq[w][i] - yh * m);
                     const float oh = raw_get(c.o[j], i) * irms_o, dg = dd * sg[j][i], f = dg * sc[w][i];
                     // (masked rows were read as zeros: they add zeros)
-                    awq[j][i] = fmaf(dn, yh, awq[j][i]);
-                    awp[j][i] = fmaf(f, oh, awp[j][i]);
-                    asc[j][i] = fmaf(dg, oh * wp[w][i], asc[j][i]);
+                    const int ja = COL_LDS ? 0 : j;
+                    awq[ja][i] = fmaf(dn, yh, awq[ja][i]);
+                    awp[ja][i] = fmaf(f, oh, awp[ja][i]);
+                    asc[ja][i] = fmaf(dg, oh * wp[w][i], asc[ja][i]);
                     e2o[0] = fmaf(f * wp[w][i], oh, e2o[0]);
                     y[j][i] = dd;
+                }
+                if constexpr (COL_LDS) {
+#pragma unroll
+                    for (int h = 0; h < VEC / 4; ++h) {
+                        f32x4* const at = s_acc + (j * (VEC / 4) + h) * TPR;
+                        at[0] += f32x4{awp[0][4 * h], awp[0][4 * h + 1], awp[0][4 * h + 2], awp[0][4 * h + 3]};
+                        at[K * VEC / 4 * TPR] += f32x4{asc[0][4 * h], asc[0][4 * h + 1], asc[0][4 * h + 2], asc[0][4 * h + 3]};
+                        at[2 * K * VEC / 4 * TPR] += f32x4{awq[0][4 * h], awq[0][4 * h + 1], awq[0][4 * h + 2], awq[0][4 * h + 3]};
+                    }
+#pragma unroll
+                    for (int i = 0; i < VEC; ++i) awp[0][i] = asc[0][i] = awq[0][i] = 0.f;
                 }
             }
             float m2 = 0.f;
@@ -257,7 +285,17 @@ __global__ void __launch_bounds__(TPR > 256 ? TPR : 256) norm_gate_kernel(const 
 #pragma unroll
             for (int j = 0; j < K; ++j) {
                 const int c0 = (j * TPR + col) * VEC;
-                const float (&acc)[VEC] = q == 0 ? awp[j] : q == 1 ? asc[j] : awq[j];
+                if constexpr (COL_LDS) {
+#pragma unroll
+                    for (int h = 0; h < VEC / 4; ++h) {
+                        const f32x4 t = s_acc[((q * K + j) * (VEC / 4) + h) * TPR];
+                        const float v[4] = {t[0], t[1], t[2], t[3]};
+                        st_raw<float, 4>(dst + c0 + h * 4, raw_pack<float, 4>(v), min(max(nv[j] - h * 4, 0), 4));
+                    }
+                    continue;
+                }
+                const int ja = COL_LDS ? 0 : j;
+                const float (&acc)[VEC] = q == 0 ? awp[ja] : q == 1 ? asc[ja] : awq[ja];
                 if constexpr (GROUPS == 1) {
 #pragma unroll
                     for (int h = 0; h < VEC / 4; ++h) st_raw<float, 4>(dst + c0 + h * 4, raw_pack<float, 4>(acc + h * 4), min(max(nv[j] - h * 4, 0), 4));
@@ -308,30 +346,40 @@ __global__ void __launch_bounds__(1024) norm_gate_colsum(const float* part, int 
 }
 
 constexpr int NG_MAX_D = 16384;
-constexpr int NG_BLOCKS = 512;       // workgroups of a backward launch at most: each leaves three partial rows of D sums
+constexpr int NG_BLOCKS = 512;       // workgroups of a backward launch at most (rows of 1024 threads: half): each leaves three partial rows of D sums
 
+// (the threads of a row; of a row that ng_two halves, this many and half of them give the same launch)
 static int ng_tpr(int D, int vec) {
     int t = 8;
     while (t < 1024 && t * vec < D) t *= 2;
     return t;
 }
 static int ng_groups(int tpr) { return tpr >= 256 ? 1 : 256 / tpr; }
+// Rows of 513 .. 1024 vectors: 512 threads with two each, whose next row is in flight, against 1024 with one. N 3000, D 2500 in fp32 33 + 48 us
+// against 45 + 59 (forward, backward); N 8000, D 5000 in bf16 120 against 131 forward, but backward the registers do not reach.
+template <class T> constexpr bool ng_two(bool bwd) { return sizeof(T) == 4 || !bwd; }
 static long ng_blocks(const refil_norm_gate_desc& d, bool bwd) {
     const int tpr = ng_tpr(d.D, d.dtype == REFIL_F32 ? 4 : 8);
-    const long n = cdivl(d.N, ng_groups(tpr)), most = bwd ? NG_BLOCKS : 2048;
+    const long n = cdivl(d.N, ng_groups(tpr)), most = bwd ? (tpr == 1024 ? NG_BLOCKS / 2 : NG_BLOCKS) : 2048;
     return n < most ? n : most;
 }
 
 template <class T, int TPR, int K>
 static int ng_run(const NormGateK& k, bool bwd, long blocks, hipStream_t st) {
-    if (bwd) hipLaunchKernelGGL((norm_gate_kernel<T, TPR, K, true>), dim3(blocks), dim3(TPR > 256 ? TPR : 256), 0, st, k);
-    else hipLaunchKernelGGL((norm_gate_kernel<T, TPR, K, false>), dim3(blocks), dim3(TPR > 256 ? TPR : 256), 0, st, k);
+    const dim3 threads(TPR > 256 ? TPR : 256);
+    if (!bwd) hipLaunchKernelGGL((norm_gate_kernel<T, TPR, K, false>), dim3(blocks), threads, 0, st, k);
+    else if constexpr (TPR != 512 || K == 1 || ng_two<T>(true)) {
+        constexpr size_t LDS = ng_col_lds<T>(TPR, K, true) ? (size_t)12 * TPR * K * VEC_OF<T> : 0;
+        if (LDS) REFIL_HIP(hipFuncSetAttribute((const void*)norm_gate_kernel<T, TPR, K, true>, (hipFuncAttribute)hipFuncAttributeMaxDynamicSharedMemorySize, (int)LDS));
+        hipLaunchKernelGGL((norm_gate_kernel<T, TPR, K, true>), dim3(blocks), threads, LDS, st, k);
+    }
     REFIL_LAUNCH_CHECK();
     return 0;
 }
 template <class T>
 static int ng_pick(const NormGateK& k, bool bwd, long blocks, hipStream_t st) {
     constexpr int VEC = VEC_OF<T>;
+    if (k.D > 512 * VEC && k.D <= 1024 * VEC && ng_two<T>(bwd)) return ng_run<T, 512, 2>(k, bwd, blocks, st);
     switch (ng_tpr(k.D, VEC)) {
         case 8: return ng_run<T, 8, 1>(k, bwd, blocks, st);
         case 16: return ng_run<T, 16, 1>(k, bwd, blocks, st);
