@@ -430,6 +430,15 @@ def test_norm_gate_many_rows():
     norm_check(*(rnd(5003, 9, seed=i) for i in range(3)), *(1 + rnd(9, seed=5 + i, scale=0.2) for i in range(3)))
 
 
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("D", [2100, 4100, 6001])
+def test_norm_gate_wide_rows_in_several_rounds(D, dtype):
+    """a workgroup passes over several wide rows; some of them masked (a few rows on the emulator)"""
+    N = 700 if DEV == "cuda" else 3
+    x, o, g = (rnd(N, D, seed=s, dtype=dtype) for s in (1, 2, 3))
+    norm_check(x, o, g, 1 + 0.1 * rnd(D, seed=4), rnd(D, seed=5), 1 + 0.1 * rnd(D, seed=6), alpha=0.9, mask=(rnd(N, seed=7) > 0.8).to(torch.uint8))
+
+
 def test_norm_gate_zero_rows_and_gate_ends():
     """rows of zeros (the root is eps alone), gates at +-inf and at the type's lowest value"""
     N, D = 6, 16
@@ -580,6 +589,19 @@ def test_gated_ff_shapes_and_strides():
     h, saved = blocks.gated_ff_forward(e, wg, wu, save=True)
     dx, dwg, dwu, dbg, dbu = blocks.gated_ff_backward(h, e, wg, wu, saved, bias=True)
     assert h.shape == (0, F) and dx.shape == (0, D) and not dwg.any() and not dwu.any() and not dbg.any() and not dbu.any()
+
+
+@pytest.mark.parametrize("dtype", [BF16, F16])
+@pytest.mark.parametrize("N,D", [(5, 130), (40, 131), (70, 192)])
+def test_gated_ff_rows_that_begin_inside_words(N, D, dtype):
+    """16-bit rows at addresses that are no multiple of four: slices from an odd column on, odd and even strides, inputs alone and weights alone"""
+    F = 24
+    for off, pad in ((1, 0), (1, 2), (0, 1), (3, 3)):
+        x = rnd(N, off + D + pad, seed=1, dtype=dtype)[:, off:off + D]
+        both = rnd(2 * F, off + D + pad, seed=2, dtype=dtype, scale=0.2)[:, off:off + D]
+        ff_check(x, both[:F], both[F:], None, None, "silu")
+        ff_check(x, both[:F].contiguous(), both[F:].contiguous(), None, None, "gelu")
+        ff_check(x.contiguous(), both[:F], both[F:], None, None, "silu")
 
 
 def test_gated_ff_rows_do_not_mix():
