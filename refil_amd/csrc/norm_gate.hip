@@ -72,7 +72,7 @@ __device__ __forceinline__ void row_sums(float (&v)[NS], float* s_red, int& turn
 }
 
 // rows of 1024 threads: one workgroup fills a compute unit and its registers, so the column sums lie in LDS as far as it reaches (backward
-// of N 8000, D 8192 in bf16 249 us = 4.2 TB/s, 417 with them in registers; N 2707, D 4505 in fp32 146 and 190)
+// of N 8000, D 8192 in bf16 249 us = 4.2 TB/s, 417 with them in registers; N 2707, D 4505 in fp32 146 for 190)
 template <class T> constexpr bool ng_col_lds(int tpr, int k, bool bwd) { return bwd && tpr == 1024 && 12 * tpr * k * VEC_OF<T> <= 128 * 1024; }
 
 template <class T, int K>
@@ -82,7 +82,7 @@ struct NgGrad { Raw<T> dy[K], dn[K]; };
 
 // WEIGHTS: the weights stay in registers over the rows of the workgroup (else they are read again for every row: rows so wide that the
 // registers do not reach). AHEAD: the next row's loads are issued in front of this row's sums.
-template <class T, int TPR, int K, bool BWD>
+template <class T, int TPR, int K, bool BWD, bool ENDS>
 __global__ void __launch_bounds__(TPR > 256 ? TPR : 256) norm_gate_kernel(const NormGateK k) {
     constexpr int VEC = VEC_OF<T>, THREADS = TPR > 256 ? TPR : 256, GROUPS = THREADS / TPR;
     constexpr bool WEIGHTS = TPR < 1024, AHEAD = TPR < 1024;
@@ -91,8 +91,9 @@ __global__ void __launch_bounds__(TPR > 256 ? TPR : 256) norm_gate_kernel(const 
     const int col = threadIdx.x % TPR, grp = threadIdx.x / TPR;
     const float inv_d = 1.f / (float)k.D;
     // the ragged end of a row is read as the row's last VEC elements, moved down by `back`: one load, where VEC single ones would keep the
-    // wave waiting (rows of fewer than VEC elements do that, and the widest, whose registers are full)
-    const bool ragged = TPR < 1024 && k.D % VEC != 0 && k.D >= VEC;
+    // wave waiting (rows of fewer than VEC elements do that, and the widest, whose registers are full). ENDS: compiled in; rows of 1024
+    // threads have a kernel of their own for it (N 4000, D 5001 in bf16 148 us backward for 168, but D 8192 would pay 271 for 250)
+    const bool ragged = ENDS && k.D % VEC != 0 && k.D >= VEC;
     int turn = 0, nv[K], back[K];
     float wp[KW][VEC], sc[KW][VEC], wq[KW][VEC];
     auto weights = [&](int j, float (&p)[VEC], float (&s)[VEC], float (&q)[VEC]) {
@@ -364,21 +365,31 @@ static long ng_blocks(const refil_norm_gate_desc& d, bool bwd) {
     return n < most ? n : most;
 }
 
-template <class T, int TPR, int K>
-static int ng_run(const NormGateK& k, bool bwd, long blocks, hipStream_t st) {
+template <class T, int TPR, int K, bool ENDS>
+static int ng_go(const NormGateK& k, bool bwd, long blocks, hipStream_t st) {
     const dim3 threads(TPR > 256 ? TPR : 256);
-    if (!bwd) hipLaunchKernelGGL((norm_gate_kernel<T, TPR, K, false>), dim3(blocks), threads, 0, st, k);
-    else if constexpr (TPR != 512 || K == 1 || ng_two<T>(true)) {
+    // (rows of 513 .. 1024 vectors have one form in each direction: ng_two)
+    if (!bwd) {
+        if constexpr (TPR != 1024 || K > 1) hipLaunchKernelGGL((norm_gate_kernel<T, TPR, K, false, ENDS>), dim3(blocks), threads, 0, st, k);
+    } else if constexpr (TPR != 512 || K == 1 || ng_two<T>(true)) {
         constexpr size_t LDS = ng_col_lds<T>(TPR, K, true) ? (size_t)12 * TPR * K * VEC_OF<T> : 0;
-        if (LDS) REFIL_HIP(hipFuncSetAttribute((const void*)norm_gate_kernel<T, TPR, K, true>, (hipFuncAttribute)hipFuncAttributeMaxDynamicSharedMemorySize, (int)LDS));
-        hipLaunchKernelGGL((norm_gate_kernel<T, TPR, K, true>), dim3(blocks), threads, LDS, st, k);
+        if (LDS) REFIL_HIP(hipFuncSetAttribute((const void*)norm_gate_kernel<T, TPR, K, true, ENDS>, (hipFuncAttribute)hipFuncAttributeMaxDynamicSharedMemorySize, (int)LDS));
+        hipLaunchKernelGGL((norm_gate_kernel<T, TPR, K, true, ENDS>), dim3(blocks), threads, LDS, st, k);
     }
     REFIL_LAUNCH_CHECK();
     return 0;
 }
+template <class T, int TPR, int K>
+static int ng_run(const NormGateK& k, bool bwd, long blocks, hipStream_t st) {
+    if constexpr (TPR == 1024) {
+        if constexpr (K * VEC_OF<T> <= 8) { if (k.D % VEC_OF<T>) return ng_go<T, TPR, K, true>(k, bwd, blocks, st); }
+        return ng_go<T, TPR, K, false>(k, bwd, blocks, st);
+    } else return ng_go<T, TPR, K, true>(k, bwd, blocks, st);
+}
 template <class T>
 static int ng_pick(const NormGateK& k, bool bwd, long blocks, hipStream_t st) {
     constexpr int VEC = VEC_OF<T>;
+    static_assert(ng_two<T>(false), "the forward of 1024 vectors is the halved one");
     if (k.D > 512 * VEC && k.D <= 1024 * VEC && ng_two<T>(bwd)) return ng_run<T, 512, 2>(k, bwd, blocks, st);
     switch (ng_tpr(k.D, VEC)) {
         case 8: return ng_run<T, 8, 1>(k, bwd, blocks, st);
@@ -390,7 +401,7 @@ static int ng_pick(const NormGateK& k, bool bwd, long blocks, hipStream_t st) {
         case 512: return ng_run<T, 512, 1>(k, bwd, blocks, st);
         default: break;
     }
-    if (k.D <= 1024 * VEC) return ng_run<T, 1024, 1>(k, bwd, blocks, st);
+    if constexpr (!ng_two<T>(true)) { if (k.D <= 1024 * VEC) return ng_run<T, 1024, 1>(k, bwd, blocks, st); }
     if (k.D <= 2048 * VEC) return ng_run<T, 1024, 2>(k, bwd, blocks, st);
     if constexpr (VEC == 4) return ng_run<T, 1024, 4>(k, bwd, blocks, st);
     set_error("refil_norm_gate: D %d too large", k.D);
