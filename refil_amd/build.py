@@ -1,5 +1,6 @@
 """Builds librefil_hip.so (gfx950) in-tree with hipcc. No torch headers are involved: the library is a
 plain C-ABI shared object (include/refil_hip.h) loaded through ctypes by refil_amd/_lib.py."""
+import concurrent.futures
 import os
 import subprocess
 import sys
@@ -22,31 +23,60 @@ def _stale():
     return any(os.path.getmtime(d) > t for d in deps)
 
 
+def _jobs():
+    """compilers at a time: the processors this process may use, or MAX_JOBS if that is fewer"""
+    n = len(os.sched_getaffinity(0))
+    try:
+        n = min(n, int(os.environ.get("MAX_JOBS", n)))
+    except ValueError:
+        pass
+    return max(1, n)
+
+
+def _compile(todo):
+    """(source, object, command writing object + ".new") each, _jobs() at a time, large sources first; an object is replaced when its compile has ended
+    well. After a failure nothing new is started, and every failed compiler's output is printed."""
+    def one(job):
+        src, obj, cmd = job
+        r = subprocess.run(cmd, stdout=subprocess.PIPE, stderr=subprocess.STDOUT)
+        if r.returncode == 0:
+            os.replace(obj + ".new", obj)
+        return src, r
+
+    failed = []
+    with concurrent.futures.ThreadPoolExecutor(_jobs()) as pool:
+        waiting = [pool.submit(one, job) for job in sorted(todo, key=lambda job: -os.path.getsize(os.path.join(CSRC, job[0])))]
+        for f in concurrent.futures.as_completed(waiting):
+            if f.cancelled():
+                continue
+            src, r = f.result()
+            if r.returncode:
+                failed.append(src)
+                sys.stderr.write(f"--- {src}: {' '.join(r.args)}\n{r.stdout.decode(errors='replace')}")
+                for w in waiting:
+                    w.cancel()
+    if failed:
+        raise RuntimeError(f"hipcc failed on {', '.join(failed)}")
+
+
 def build(force=False, verbose=True):
     if not force and not _stale():
         return LIB
     hipcc = os.environ.get("HIPCC", "/opt/rocm/bin/hipcc")
-    objs = []
-    procs = []
     extra = os.environ.get("REFIL_EXTRA_FLAGS", "").split()
     obj_dir = os.path.join(HERE, "build", "extra") if extra else os.path.join(HERE, "build")     # (a variant's objects never mix with the library's)
     os.makedirs(obj_dir, exist_ok=True)
     headers = [os.path.join(CSRC, f) for f in os.listdir(CSRC) if f.endswith(".h")]
     headers += [os.path.join(HERE, "..", "include", "refil_hip.h"), os.path.abspath(__file__)]
+    objs, todo = [], []
     for src in SOURCES:
-        obj = os.path.join(obj_dir, src.replace(".hip", ".o"))
-        cmd = [hipcc, "--offload-arch=gfx950", "-O3", "-std=c++17", "-fPIC"] + NO_PACKED_FP32 + extra + ["-c", os.path.join(CSRC, src), "-o", obj]
+        path, obj = os.path.join(CSRC, src), os.path.join(obj_dir, src.replace(".hip", ".o"))
         objs.append(obj)
         # one source changed: one compile (an object newer than its source and every header is kept unless the build is forced)
-        if not force and not extra and os.path.exists(obj) and \
-                all(os.path.getmtime(d) <= os.path.getmtime(obj) for d in headers + [os.path.join(CSRC, src)]):
+        if not force and not extra and os.path.exists(obj) and all(os.path.getmtime(d) <= os.path.getmtime(obj) for d in headers + [path]):
             continue
-        procs.append((src, subprocess.Popen(cmd, stdout=subprocess.PIPE, stderr=subprocess.STDOUT)))
-    for src, p in procs:
-        out, _ = p.communicate()
-        if p.returncode != 0:
-            sys.stderr.write(out.decode())
-            raise RuntimeError(f"hipcc failed on {src}")
+        todo.append((src, obj, [hipcc, "--offload-arch=gfx950", "-O3", "-std=c++17", "-fPIC"] + NO_PACKED_FP32 + extra + ["-c", path, "-o", obj + ".new"]))
+    _compile(todo)
     # The dynamic symbol table holds the C ABI of include/refil_hip.h and nothing else: the launchers' C++ symbols and the kernel
     # handles stay local to the library (a linker version script: no object file is compiled differently for it).
     vs = os.path.join(HERE, "build", "exports.map")
