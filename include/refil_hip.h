@@ -550,7 +550,9 @@ int refil_norm_gate_backward(const refil_norm_gate_desc* desc, void* stream);
 /* Gated feed-forward block: h[N,F] = act(x w_gate^T + b_gate) * (x w_up^T + b_up), x [N,D], w_* [F,D] (both with w_stride), b_* [F] or NULL,
  * all of `dtype`; act: REFIL_ACT_SILU v sigmoid(v), REFIL_ACT_GELU the tanh form. saved: NULL, or 2 N F floats that the
  * backward needs (the two pre-activations). Backward: dh -> dx, dw_gate, dw_up [F,D] contiguous, db_* [F] or NULL; sums in fp32, rounded
- * once; in 16 bits the gradients of the two pre-activations are rounded to dtype in front of the products. fp32 products run as six bf16
+ * once; in 16 bits the gradients of the two pre-activations are rounded to dtype in front of the products, beside the rounding of the results
+ * (the error of dx and dw is 1.4 times that of one rounding); in fp16 under one power-of-two scale for all of them where they would leave the
+ * type's range, so that dh of 1e4 (loss scaling) or 1e-7 costs no more than dh of 1. fp32 products run as six bf16
  * matrix products of an exact three-way split (refil_set_tuning's "wres_split" = 6 arithmetic, with its operand range: an Inf gives NaN). */
 enum { REFIL_ACT_SILU = 0, REFIL_ACT_GELU = 1 };
 typedef struct refil_gated_ff_desc {

@@ -424,7 +424,8 @@ def gated_ff_forward(x, w_gate, w_up, b_gate=None, b_up=None, *, act="silu", sav
 
 
 def gated_ff_backward(dh, x, w_gate, w_up, saved, *, act="silu", bias=False):
-    """(dx, dw_gate, dw_up, db_gate, db_up) of gated_ff_forward(..., save=True); the bias gradients are None unless `bias`."""
+    """(dx, dw_gate, dw_up, db_gate, db_up) of gated_ff_forward(..., save=True); the bias gradients are None unless `bias`. In 16 bits the gradients
+    of the two pre-activations are rounded to the type once on the way to dx and the weight gradients, inside fp16's range whatever dh's."""
     who = "gated_ff_backward"
     d = _ff_desc(who, x, w_gate, w_up, act)
     L, F, D = _lib.lib(), d.F, d.D

@@ -68,6 +68,7 @@ struct GfGemm {
     int splits; float* partial;                    // splits > 1: fp32 partial sums [splits][M][gf_ldp(N)]
     void* C0; void* C1; long ldc; int msplit, mlim;      // rows m < msplit: row m of C0; the others: row m - msplit of C1; rows at or behind mlim of either are padding
     const void* bias0; const void* bias1; float* save0; float* save1; int act;      // gated epilogue
+    const float* unscale;                          // fp16 backward: A holds [dg | du] divided by *unscale, a power of two
 };
 
 template <class T>
@@ -364,6 +365,8 @@ __global__ void __launch_bounds__(WM * WN * 64, WM * MT == 16 || sizeof(T) == 4 
     }
 
     // lane: m = lane & 15, n = 4 (lane >> 4) + 0..3 of every tile
+    float unscale = 1.f;
+    if constexpr (__is_same(T, f16_t) && !GATED) unscale = *k.unscale;
 #pragma unroll
     for (int i = 0; i < MT; ++i) {
         const int m = m0 + (wm * MT + i) * 16 + (lane & 15);
@@ -380,7 +383,7 @@ __global__ void __launch_bounds__(WM * WN * 64, WM * MT == 16 || sizeof(T) == 4 
                 const int n = n0 + (wn * NT + j) * 16 + (lane >> 4) * 4, c = min(max(k.N - n, 0), 4);
                 float v[4];
 #pragma unroll
-                for (int r = 0; r < 4; ++r) v[r] = acc[i][j][r];
+                for (int r = 0; r < 4; ++r) v[r] = acc[i][j][r] * unscale;
                 if (k.splits > 1) st_raw<float, 4>(k.partial + ((long)split * k.M + m) * gf_ldp(k.N) + n, raw_pack<float, 4>(v), c ? 4 : 0);
                 else {
                     const bool first = m < k.msplit;
@@ -508,20 +511,23 @@ __global__ void __launch_bounds__(512) gf_skinny(const GfGemm k) {
 // [dg | du] of rows [0, rows_out) (rows behind N and columns behind F are zero: the products read whole 64-blocks of them), rounded to T:
 // in 16 bits half a step of each, which the products carry on as they carry x's and the weights'. A workgroup walks `per` rows of 32
 // vectors of columns (neighbouring workgroups: neighbouring columns, so that whole rows are in flight) and leaves one partial row of the bias sums, taken before the rounding.
+//
+// fp16: dg = dh u act' leaves the type's range where dh and the products' results lie in it, so [dg | du] is kept divided by a power of two
+// that the products' fp32 sums are multiplied with again (exactly). Almost always that is 1: the pass notes each workgroup's largest finite
+// magnitude, and a second launch (gf_regrad) writes everything again, scaled, only where the whole's largest is 61440 or more (Inf), or below 1
+// (subnormal numbers, steps of 2^-24, would be felt). One scale for all rows, because a weight gradient adds over them.
 struct GfGrad {
     const float* sg; const float* su; const void* dh; long dh_s; long N, rows_out; int F, Fp, act;
     void* out; long ldo; float* colsum; int per;      // colsum [row blocks][2 Fp] or NULL
+    float* top; float* unscale;                       // fp16: [workgroups of gf_grad], one number
 };
+// the workgroup's rows and columns: their [dg | du] times `scale`, their column sums and largest finite magnitude before it
 template <class T>
-__global__ void __launch_bounds__(256) gf_grad(const GfGrad k) {
+__device__ __forceinline__ void gf_grad_block(const GfGrad& k, int bx, int by, float scale, float (&bg)[VEC_OF<T>], float (&bu)[VEC_OF<T>], float& top) {
     constexpr int V = VEC_OF<T>, CT = 32, RT = 8;
-    __shared__ float s[RT][2][CT * V];
     const int ct = threadIdx.x % CT, rt = threadIdx.x / CT;
-    const int c0 = (blockIdx.x * CT + ct) * V, nv = min(max(k.F - c0, 0), V), np = min(max(k.Fp - c0, 0), V);
-    const long r0 = (long)blockIdx.y * k.per, r1 = min(r0 + k.per, k.rows_out);
-    float bg[V], bu[V];
-#pragma unroll
-    for (int i = 0; i < V; ++i) bg[i] = bu[i] = 0.f;
+    const int c0 = (bx * CT + ct) * V, nv = min(max(k.F - c0, 0), V), np = min(max(k.Fp - c0, 0), V);
+    const long r0 = (long)by * k.per, r1 = min(r0 + k.per, k.rows_out);
     for (long r = r0 + rt; r < r1; r += RT) {
         const int n = r < k.N ? nv : 0;
         const long o = r * k.F + c0;
@@ -541,10 +547,37 @@ __global__ void __launch_bounds__(256) gf_grad(const GfGrad k) {
             dg[i] = i < n ? d * raw_get(ru[i / 4], i % 4) * df : 0.f;
             du[i] = i < n ? d * f : 0.f;
             bg[i] += dg[i]; bu[i] += du[i];
+            if constexpr (__is_same(T, f16_t)) {
+                const float a = fabsf(dg[i]), b = fabsf(du[i]);
+                top = fmaxf(top, fmaxf(a < INFINITY ? a : 0.f, b < INFINITY ? b : 0.f));
+                dg[i] *= scale; du[i] *= scale;
+            }
         }
         T* p = (T*)k.out + r * k.ldo + c0;
         st_raw<T, V>(p, raw_pack<T, V>(dg), np);
         st_raw<T, V>(p + k.Fp, raw_pack<T, V>(du), np);
+    }
+}
+__device__ __forceinline__ float gf_block_max(float v, float (&s)[4]) {
+#pragma unroll
+    for (int d = 1; d < 64; d *= 2) v = fmaxf(v, __shfl_xor(v, d));
+    if ((threadIdx.x & 63) == 0) s[threadIdx.x >> 6] = v;
+    __syncthreads();
+    return fmaxf(fmaxf(s[0], s[1]), fmaxf(s[2], s[3]));
+}
+template <class T>
+__global__ void __launch_bounds__(256) gf_grad(const GfGrad k) {
+    constexpr int V = VEC_OF<T>, CT = 32, RT = 8;
+    __shared__ float s[RT][2][CT * V];
+    const int ct = threadIdx.x % CT, rt = threadIdx.x / CT;
+    float bg[V], bu[V], top = 0.f;
+#pragma unroll
+    for (int i = 0; i < V; ++i) bg[i] = bu[i] = 0.f;
+    gf_grad_block<T>(k, blockIdx.x, blockIdx.y, 1.f, bg, bu, top);
+    if constexpr (__is_same(T, f16_t)) {
+        __shared__ float s_top[4];
+        top = gf_block_max(top, s_top);
+        if (threadIdx.x == 0) k.top[(long)blockIdx.y * gridDim.x + blockIdx.x] = top;
     }
     if (!k.colsum) return;
 #pragma unroll
@@ -557,6 +590,23 @@ __global__ void __launch_bounds__(256) gf_grad(const GfGrad k) {
         for (int q = 0; q < RT; ++q) t += s[q][z][c];
         if (col < k.F) k.colsum[(long)blockIdx.y * 2 * k.F + z * k.F + col] = t;
     }
+}
+// every workgroup finds the largest magnitude of all (a maximum: the same in any order) and, if the scale is not 1, walks its share of gf_grad's blocks
+__global__ void __launch_bounds__(256) gf_regrad(const GfGrad k, int cols, int blocks) {
+    constexpr int V = VEC_OF<f16_t>;
+    __shared__ float s_top[4];
+    float top = 0.f;
+    for (int i = threadIdx.x; i < blocks; i += 256) top = fmaxf(top, k.top[i]);
+    top = gf_block_max(top, s_top);
+    float scale = 1.f;
+    if (top > 0.f && (top < 1.f || top >= 61440.f)) {
+        const int e = min(14 - ((int)(__float_as_uint(top) >> 23) - 127), 126);      // [2^14, 2^15) afterwards; far below 2^-112 nearer to 0
+        scale = __uint_as_float((unsigned)(127 + e) << 23);
+    }
+    if (blockIdx.x == 0 && threadIdx.x == 0) *k.unscale = 1.f / scale;               // (a power of two)
+    if (scale == 1.f) return;
+    float bg[V] = {}, bu[V] = {};
+    for (int b = blockIdx.x; b < blocks; b += gridDim.x) gf_grad_block<f16_t>(k, b % cols, b / cols, scale, bg, bu, top);
 }
 // The end of a backward in one launch: the sums of the split products (dx, then dw) in split order, a thread takes four columns of a row;
 // then the bias gradients, 64 columns a workgroup, their partial rows in order.
@@ -674,7 +724,7 @@ static int gf_launch(GfGemm k, const GfPlan& p, hipStream_t st, const char* name
 }
 
 static int gf_blocks(long n) { const long b = cdivl(n, 256); return (int)(b < 1 ? 1 : b > 8192 ? 8192 : b); }
-struct GfBwdWs { void* grad; float* colsum; float* part_x; float* part_w; long Fp, Np; GfPlan px, pw; int row_blocks, per; size_t bytes; };
+struct GfBwdWs { void* grad; float* colsum; float* top; float* unscale; int grad_cols; float* part_x; float* part_w; long Fp, Np; GfPlan px, pw; int row_blocks, per; size_t bytes; };
 static GfBwdWs gf_bwd_ws(const refil_gated_ff_desc& d, void* base) {
     char* const p = (char*)base; size_t n = 0;
     auto take = [&](size_t b) { char* r = p ? p + n : nullptr; n += (b + 255) / 256 * 256; return (void*)r; };
@@ -686,6 +736,11 @@ static GfBwdWs gf_bwd_ws(const refil_gated_ff_desc& d, void* base) {
     w.per = (int)(cdivl(cdivl(w.Np, 256), 8) * 8);          // at most 256 partial rows of bias sums, whole rounds of 8 rows
     w.row_blocks = (int)cdivl(w.Np, w.per);
     w.colsum = (float*)take((size_t)w.row_blocks * 2 * d.F * 4);
+    w.grad_cols = (int)cdivl(w.Fp, 32 * (d.dtype == REFIL_F32 ? 4 : 8));
+    if (d.dtype == REFIL_F16) {
+        w.top = (float*)take((size_t)w.grad_cols * w.row_blocks * 4);
+        w.unscale = (float*)take(4);
+    }
     w.px = gf_plan(d.N, d.D, 2 * w.Fp, bk, direct);
     w.pw = gf_plan(2 * w.Fp, d.D, w.Np, bk, direct);
     if (w.px.splits > 1) w.part_x = (float*)take((size_t)4 * w.px.splits * d.N * gf_ldp(d.D));
@@ -722,15 +777,22 @@ static int gf_backward(const refil_gated_ff_desc& d, hipStream_t st) {
     GfGrad g{};
     g.sg = d.saved; g.su = d.saved + d.N * d.F; g.dh = d.dh; g.dh_s = d.dh_stride; g.N = d.N; g.rows_out = w.Np; g.F = d.F; g.Fp = (int)w.Fp; g.act = d.act;
     g.out = w.grad; g.ldo = 2 * w.Fp; g.colsum = (d.db_gate || d.db_up) ? w.colsum : nullptr; g.per = w.per;
+    g.top = w.top; g.unscale = w.unscale;
     {
         ProfScope ps("gated_ff_grad", 20 * nf, nf * (8 + 3 * es), st);
-        hipLaunchKernelGGL((gf_grad<T>), dim3(cdiv(w.Fp, 32 * VEC_OF<T>), w.row_blocks), dim3(256), 0, st, g);
+        hipLaunchKernelGGL((gf_grad<T>), dim3(w.grad_cols, w.row_blocks), dim3(256), 0, st, g);
+        REFIL_LAUNCH_CHECK();
+    }
+    if constexpr (__is_same(T, f16_t)) {
+        const int blocks = w.grad_cols * w.row_blocks;
+        ProfScope ps("gated_ff_regrad", 0, 4.0 * blocks, st);
+        hipLaunchKernelGGL(gf_regrad, dim3(blocks < 1024 ? blocks : 1024), dim3(256), 0, st, g, w.grad_cols, blocks);
         REFIL_LAUNCH_CHECK();
     }
     GfGemm k{};
     k.A = w.grad; k.lda = 2 * w.Fp; k.B0 = d.w_gate; k.B1 = d.w_up; k.ldb = d.w_stride; k.ksplit = (int)w.Fp;
     k.M = (int)d.N; k.N = d.D; k.K = (int)(2 * w.Fp); k.a_rows = k.M; k.b_rows = d.F; k.C0 = d.dx; k.ldc = d.dx_stride; k.msplit = k.mlim = k.M;
-    k.splits = w.px.splits; k.partial = w.part_x;
+    k.splits = w.px.splits; k.partial = w.part_x; k.unscale = w.unscale;
     GfFinish f{};
     f.dx = k;
     const double fl = 4.0 * nf * d.D, by = es * (2 * nf + 2.0 * d.F * d.D + (double)d.N * d.D);

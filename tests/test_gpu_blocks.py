@@ -655,6 +655,105 @@ def test_gated_ff_autograd_and_differences():
         assert abs(got - want) <= 1e-5 * (leaf.grad.double().abs() * d.abs()).sum().item() + 1e-8, (i, got, want)
 
 
+def ff_ref16(x, wg, wu, bg, bu, act, dh):
+    """The backward of 16-bit inputs: values, error majorants and, for dx and the weight gradients, the variance of what the roundings do.
+
+    It starts from fp32 pre-activations. dg and du, the gradients of the two, are exact to fp32 errors Edg, Edu where the bias gradients sum them;
+    the products read them rounded to the type, off by half a step of the value, and in fp16 by half a subnormal step S / 2 = 2^-25 R more: R is 1
+    while the largest |dg|, |du| lies in [1, 61440), else the power of two that brings it into [2^14, 2^15). A rounding error is uniform in
+    +-half |v| at most, independent from element to element: its variance is at most (half |v|)^2 / 3."""
+    F, D = wg.shape
+    t = torch.finfo(x.dtype)
+    half = t.eps / 2
+    x2, wg2, wu2 = x.double().reshape(-1, D), wg.double(), wu.double()
+    z = torch.zeros(F, dtype=torch.float64, device=x.device)
+    b0, b1 = (z if b is None else b.double() for b in (bg, bu))
+    g, u = x2 @ wg2.t() + b0, x2 @ wu2.t() + b1
+    Eg, Eu = (D + 16) * U * (x2.abs() @ wg2.abs().t() + b0.abs()), (D + 16) * U * (x2.abs() @ wu2.abs().t() + b1.abs())
+    f, df = act_ref(act, g)
+    Ka = (3 * g.abs() + 0.3 * g.abs() ** 3 + 8) * U
+    d = dh.double().reshape(-1, F)
+    dg, du = d * u * df, d * f
+    Edg = d.abs() * ((u.abs() + Eu) * (1.2 * Eg + Ka * (1 + g.abs())) + Eu * df.abs()) + 4 * U * dg.abs()
+    Edu = d.abs() * (1.13 * Eg + Ka * f.abs()) + 4 * U * du.abs()
+    N = x2.shape[0]
+    k = (N + 16) * U
+    out = {"dbg": (dg.sum(0), (Edg + k * dg.abs()).sum(0)), "dbu": (du.sum(0), (Edu + k * du.abs()).sum(0))}
+    S = 0.0
+    if x.dtype == F16:
+        top = max(float(dg.abs().max()), float(du.abs().max()))
+        R = 1.0 if 1 <= top < 61440 else 2.0 ** (math.floor(math.log2(top)) - 14)
+        S = 2.0 ** -24 * R * (2 if abs(math.log2(top) - round(math.log2(top))) < 1e-5 else 1)       # (the fp32 value may sit on the other side of a power)
+    out["S"] = S
+    Rg, Ru = Edg + half * (dg.abs() + Edg) + S / 2, Edu + half * (du.abs() + Edu) + S / 2
+    vg, vu = (half * dg) ** 2 / 3 + S * S / 12, (half * du) ** 2 / 3 + S * S / 12
+    kx = (2 * F + 16) * U
+    dx = dg @ wg2 + du @ wu2
+    out["dx"] = (dx, Rg @ wg2.abs() + Ru @ wu2.abs() + kx * (dg.abs() @ wg2.abs() + du.abs() @ wu2.abs()))
+    var = {"dx": vg @ wg2 ** 2 + vu @ wu2 ** 2}
+    fp32 = {"dx": Edg @ wg2.abs() + Edu @ wu2.abs() + kx * (dg.abs() @ wg2.abs() + du.abs() @ wu2.abs())}
+    for name, v, E, R_, va in (("dwg", dg, Edg, Rg, vg), ("dwu", du, Edu, Ru, vu)):
+        out[name] = (v.t() @ x2, R_.t() @ x2.abs() + k * (v.abs().t() @ x2.abs()))
+        var[name] = va.t() @ x2 ** 2
+        fp32[name] = E.t() @ x2.abs() + k * (v.abs().t() @ x2.abs())
+    out["var"] = {n: var[n] + (half * out[n][0]) ** 2 / 3 + t.tiny ** 2 * t.eps ** 2 / 12 for n in var}        # (the last rounding, its subnormal step)
+    out["fp32"] = fp32
+    return out
+
+
+def close_or_inf(name, got, want, fp32_error):
+    """close(), and where the value itself lies outside the type: Inf of its sign. Rounding to nearest gives Inf from the largest number and half a
+    step on (fp16: 65520), so an Inf is right if the value may reach that, and a number is if it may stay below"""
+    t = torch.finfo(got.dtype)
+    edge = t.max * (1 + t.eps / 4)                  # (its last step is max eps / (2 - eps); half of it is max eps / 4 or a little more)
+    inf = torch.isinf(got)
+    assert (inf <= (want.abs() + fp32_error >= edge)).all() and (torch.sign(got) == torch.sign(want))[inf].all(), f"{name}: Inf where the value is in range"
+    assert (inf >= (want.abs() - fp32_error >= edge * (1 + t.eps))).all(), f"{name}: a number where the value is out of range"
+    close(name, torch.where(inf, 0, got), torch.where(inf, 0.0, want), torch.where(inf, 0.0, fp32_error))
+
+
+def ff_check16(x, wg, wu, bg, bu, act, dh):
+    """every gradient inside its majorant, and the errors of dx, dw_gate and dw_up no larger in the mean square than the roundings' variance (what
+    fp32 arithmetic may add comes off first; 1.1: thousands of elements, whose mean square strays by a few per cent)"""
+    _, saved = blocks.gated_ff_forward(x, wg, wu, bg, bu, act=act, save=True)
+    got = dict(zip(("dx", "dwg", "dwu", "dbg", "dbu"), blocks.gated_ff_backward(dh, x, wg, wu, saved, act=act, bias=bg is not None)))
+    ref = ff_ref16(x, wg, wu, bg, bu, act, dh)
+    for k, v in got.items():
+        if v is not None:
+            close_or_inf(k, v.reshape(ref[k][0].shape), *ref[k])
+    for k in ("dx", "dwg", "dwu"):
+        err = ((got[k].double().reshape(ref[k][0].shape) - ref[k][0]).abs() - ref["fp32"][k]).clamp_min(0)
+        fits = torch.isfinite(got[k].reshape(ref[k][0].shape))
+        ratio = ((err ** 2 / ref["var"][k])[fits]).mean().sqrt()
+        assert ratio <= 1.1, f"{k}: the mean square error is {float(ratio):.3g} of the roundings'"
+
+
+@pytest.mark.parametrize("act", ["silu", "gelu"])
+@pytest.mark.parametrize("N,D,F", [(128, 512, 64), (130, 512, 512), (70, 33, 131)])
+@pytest.mark.parametrize("scale", [1e4, 1.0, 1e-3, 3e-6, 1e-7])
+def test_gated_ff_half_gradients_over_the_types_range(scale, N, D, F, act):
+    """dh as loss scaling makes it, and down to subnormal numbers: the gradients of the pre-activations, which lie outside fp16 on the way, neither
+    overflow nor lose digits"""
+    x = rnd(N, D, seed=N + D, dtype=F16)
+    wg, wu = rnd(F, D, seed=1, dtype=F16, scale=D ** -0.5), rnd(F, D, seed=2, dtype=F16, scale=D ** -0.5)
+    ff_check16(x, wg, wu, rnd(F, seed=3, dtype=F16), rnd(F, seed=4, dtype=F16), act, rnd(N, F, seed=5, dtype=F16, scale=scale))
+
+
+def test_gated_ff_half_gradients_beside_infinities_and_zeros():
+    """an Inf in dh spoils its own row of dx, not the scale of the others; gradients that are all zero give zeros"""
+    N, D, F = 40, 64, 96
+    x, wg, wu = rnd(N, D, seed=1, dtype=F16), rnd(F, D, seed=2, dtype=F16, scale=0.1), rnd(F, D, seed=3, dtype=F16, scale=0.1)
+    _, saved = blocks.gated_ff_forward(x, wg, wu, save=True)
+    dh = rnd(N, F, seed=4, dtype=F16, scale=1e-6)
+    clean = blocks.gated_ff_backward(dh, x, wg, wu, saved)[0]
+    dh[7, 3] = math.inf
+    dx = blocks.gated_ff_backward(dh, x, wg, wu, saved)[0]
+    keep = torch.arange(N, device=DEV) != 7
+    assert not torch.isfinite(dx[7]).any() and torch.equal(dx[keep], clean[keep])
+    r = blocks.gated_ff_backward(torch.zeros_like(dh), x, wg, wu, saved, bias=True)
+    assert not any(t.any() for t in r)
+
+
 # ------------------------------------------------------------------------------------------------ together
 def block_pass(x, p, h0, lengths, row_mask, state=None):
     """norm -> recurrence -> norm, gate, residual -> gated feed-forward -> norm, gate, residual, as an agent would stack it; with `state` one
