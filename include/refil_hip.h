@@ -553,7 +553,8 @@ int refil_norm_gate_backward(const refil_norm_gate_desc* desc, void* stream);
  * once; in 16 bits the gradients of the two pre-activations are rounded to dtype in front of the products, beside the rounding of the results
  * (the error of dx and dw is 1.4 times that of one rounding); in fp16 under one power-of-two scale for all of them where they would leave the
  * type's range, so that dh of 1e4 (loss scaling) or 1e-7 costs no more than dh of 1. fp32 products run as six bf16
- * matrix products of an exact three-way split (refil_set_tuning's "wres_split" = 6 arithmetic, with its operand range: an Inf gives NaN). */
+ * matrix products of an exact three-way split (refil_set_tuning's "wres_split" = 6 arithmetic; an Inf gives NaN, the largest finite
+ * numbers are exact too, and an operand below 2^-110 keeps what lies above 2^-133 of it). */
 enum { REFIL_ACT_SILU = 0, REFIL_ACT_GELU = 1 };
 typedef struct refil_gated_ff_desc {
     const void* x; int64_t x_stride;

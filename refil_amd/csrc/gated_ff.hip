@@ -88,6 +88,30 @@ __device__ __forceinline__ void gf_gated_out(const GfGemm& k, int m, int n, int 
     }
 }
 
+// wr_split for operands of any finite size. A leading piece that rounds to Inf (the top 0.2 % of the fp32 range) is taken back to the largest bf16
+// number of its sign, 0x7F7F or 0xFF7F -- as 16-bit integers the smaller of the two, signed for the positive ones, unsigned for the negative ones --
+// and what is left over is below 2^120 and splits exactly.
+typedef short gf_s16x2 __attribute__((ext_vector_type(2)));
+typedef unsigned short gf_u16x2 __attribute__((ext_vector_type(2)));
+__device__ __forceinline__ void gf_split(float x, float y, unsigned& h, unsigned& m, unsigned& l) {
+    const gf_s16x2 p = __builtin_elementwise_min(__builtin_bit_cast(gf_s16x2, wr_pk(x, y)), gf_s16x2{0x7F7F, 0x7F7F});
+    h = __builtin_bit_cast(unsigned, __builtin_elementwise_min(__builtin_bit_cast(gf_u16x2, p), gf_u16x2{0xFF7F, 0xFF7F}));
+    x -= __uint_as_float(h << 16); y -= __uint_as_float(h & 0xFFFF0000u);
+    m = wr_pk(x, y);
+    x -= __uint_as_float(m << 16); y -= __uint_as_float(m & 0xFFFF0000u);
+    l = wr_pk(x, y);
+}
+// wr_split, and whether that was needed: `over` becomes Inf. One operation a pair instead of two, for the tiled product, whose vector units the
+// split keeps busy (N 4000, D 1024, F 2048: dx and dw 252 + 262 us with the minima in it, 241 + 246 without).
+__device__ __forceinline__ void gf_split_watched(float x, float y, unsigned& h, unsigned& m, unsigned& l, float& over) {
+    h = wr_pk(x, y);
+    x -= __uint_as_float(h << 16); y -= __uint_as_float(h & 0xFFFF0000u);
+    over = fmaxf(over, fmaxf(fabsf(x), fabsf(y)));
+    m = wr_pk(x, y);
+    x -= __uint_as_float(m << 16); y -= __uint_as_float(m & 0xFFFF0000u);
+    l = wr_pk(x, y);
+}
+
 template <class T> constexpr int GF_P = sizeof(T) == 4 ? 3 : 1;        // 16-bit planes of an operand
 template <class T> constexpr int GF_BK = sizeof(T) == 4 ? 32 : 64;
 template <class T> struct GfElem { typedef T type; };
@@ -333,12 +357,17 @@ __global__ void __launch_bounds__(WM * WN * 64, WM * MT == 16 || sizeof(T) == 4 
                 }
             }
         };
-        auto put = [&](char* tile, int bytes, int slot, const Raw<T> (&r)[8 / V]) {
+        float over;
+        auto put = [&](auto any_size, char* tile, int bytes, int slot, const Raw<T> (&r)[8 / V]) {
             if constexpr (P == 1) *reinterpret_cast<gf_u32x4*>(tile + slot * 16) = gf_u32x4{r[0].w[0], r[0].w[1], r[0].w[2], r[0].w[3]};
             else {
                 unsigned h[4], m[4], l[4];
 #pragma unroll
-                for (int q = 0; q < 4; ++q) wr_split(raw_get(r[q / 2], 2 * (q & 1)), raw_get(r[q / 2], 2 * (q & 1) + 1), h[q], m[q], l[q]);
+                for (int q = 0; q < 4; ++q) {
+                    const float v0 = raw_get(r[q / 2], 2 * (q & 1)), v1 = raw_get(r[q / 2], 2 * (q & 1) + 1);
+                    if constexpr (decltype(any_size)::value) gf_split(v0, v1, h[q], m[q], l[q]);
+                    else gf_split_watched(v0, v1, h[q], m[q], l[q], over);
+                }
                 *reinterpret_cast<gf_u32x4*>(tile + slot * 16) = gf_u32x4{h[0], h[1], h[2], h[3]};
                 *reinterpret_cast<gf_u32x4*>(tile + bytes + slot * 16) = gf_u32x4{m[0], m[1], m[2], m[3]};
                 *reinterpret_cast<gf_u32x4*>(tile + 2 * bytes + slot * 16) = gf_u32x4{l[0], l[1], l[2], l[3]};
@@ -348,16 +377,21 @@ __global__ void __launch_bounds__(WM * WN * 64, WM * MT == 16 || sizeof(T) == 4 
         for (int it = it0; it < it1; ++it) {
             fix(it);
             lds_barrier();                  // the products of the tile before have been read
+            auto put_all = [&](auto any_size) {
 #pragma unroll
-            for (int i = 0; i < A_IT; ++i) {
-                const int e = i * THREADS + (int)threadIdx.x, r = e / TA::CH;
-                put(sa, TA::BYTES, r * TA::CH + ((e % TA::CH) ^ TA::swz(r)), ra[i]);
-            }
+                for (int i = 0; i < A_IT; ++i) {
+                    const int e = i * THREADS + (int)threadIdx.x, r = e / TA::CH;
+                    put(any_size, sa, TA::BYTES, r * TA::CH + ((e % TA::CH) ^ TA::swz(r)), ra[i]);
+                }
 #pragma unroll
-            for (int i = 0; i < B_IT; ++i) {
-                const int e = i * THREADS + (int)threadIdx.x, r = e / TB::CH;
-                put(sb, TB::BYTES, r * TB::CH + ((e % TB::CH) ^ TB::swz(r)), rb[i]);
-            }
+                for (int i = 0; i < B_IT; ++i) {
+                    const int e = i * THREADS + (int)threadIdx.x, r = e / TB::CH;
+                    put(any_size, sb, TB::BYTES, r * TB::CH + ((e % TB::CH) ^ TB::swz(r)), rb[i]);
+                }
+            };
+            over = 0.f;
+            put_all(std::false_type());
+            if constexpr (P == 3) { if (__any(over == INFINITY)) put_all(std::true_type()); }      // (a lane writes its own slots again)
             lds_barrier();
             if (it + 1 < it1) load(it + 1);
             products(sa, sb);
@@ -447,7 +481,7 @@ __global__ void __launch_bounds__(512) gf_skinny(const GfGemm k) {
 #pragma unroll
             for (int q = 0; q < 4; ++q) {
                 unsigned h, m, l;
-                wr_split(raw_get(o[half * 2 + q / 2], 2 * (q & 1)), raw_get(o[half * 2 + q / 2], 2 * (q & 1) + 1), h, m, l);
+                gf_split(raw_get(o[half * 2 + q / 2], 2 * (q & 1)), raw_get(o[half * 2 + q / 2], 2 * (q & 1) + 1), h, m, l);
                 f[0][q] = h; f[P / 2][q] = m; f[P - 1][q] = l;
             }
         }

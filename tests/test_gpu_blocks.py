@@ -754,6 +754,34 @@ def test_gated_ff_half_gradients_beside_infinities_and_zeros():
     assert not any(t.any() for t in r)
 
 
+@pytest.mark.parametrize("N,D,F", [(3, 32, 20), (65, 32, 40), (1100, 40, 900), (130, 33, 31)])
+def test_gated_ff_largest_fp32_numbers(N, D, F):
+    """operands up to the largest fp32 number, whose leading 16-bit piece must not round to Inf: x in front of small weights (few rows, fragments, tiles),
+    then weights and x in the backward's products. (1e-30: all three pieces of a weight are normal numbers)"""
+    if DEV == "cpu":
+        N, F = min(N, 260), min(F, 200)
+    top = torch.finfo(F32).max
+    x, wg, wu = rnd(N, D, seed=1), rnd(F, D, seed=2, scale=1e-30), rnd(F, D, seed=3, scale=1e-39 ** 0.5)
+    x[:, ::3], x[0], x[-1, 1::3] = top, -3.4e38, 3.3962e38
+    h, saved = blocks.gated_ff_forward(x, wg, wu, save=True)
+    assert torch.isfinite(h).all()
+    close("h", h, *ff_ref(x, wg, wu, None, None, "silu")["h"])
+    # dw: x as large against small gradients; dx: weights as large against them
+    a, b = rnd(F, D, seed=4), rnd(F, D, seed=5)
+    saved = torch.stack([rnd(N, F, seed=6), rnd(N, F, seed=7)])
+    dh = rnd(N, F, seed=8, scale=1e-6)
+    g, u = saved[0].double(), saved[1].double()
+    f, df = act_ref("silu", g)
+    dg, du = dh.double() * u * df, dh.double() * f
+    E = (3 * g.abs() + 16) * U * (1 + g.abs()) * dh.double().abs() * (1 + u.abs())
+    a[:, ::4], b[1] = top, -top
+    dx, dwg, dwu, _, _ = blocks.gated_ff_backward(dh, x, a, b, saved)
+    A, B, X = a.double(), b.double(), x.double()
+    close("dx", dx, dg @ A + du @ B, E @ (A.abs() + B.abs()) + (2 * F + 16) * U * (dg.abs() @ A.abs() + du.abs() @ B.abs()))
+    for name, got, v in (("dwg", dwg, dg), ("dwu", dwu, du)):
+        close(name, got, v.t() @ X, E.t() @ X.abs() + (N + 16) * U * (v.abs().t() @ X.abs()))
+
+
 # ------------------------------------------------------------------------------------------------ together
 def block_pass(x, p, h0, lengths, row_mask, state=None):
     """norm -> recurrence -> norm, gate, residual -> gated feed-forward -> norm, gate, residual, as an agent would stack it; with `state` one
