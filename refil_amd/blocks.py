@@ -19,6 +19,7 @@ import ctypes as C
 from collections import namedtuple
 
 import torch
+from torch.autograd import forward_ad as _forward_ad
 
 from . import _lib
 from ._lib import GatedFfDesc, LinrecDesc, LinrecStepDesc, NormGateDesc, check
@@ -111,7 +112,16 @@ def _workspace(nbytes, x):
     return x.new_empty(nbytes, dtype=torch.uint8) if nbytes else None
 
 
-def _grad(*tensors):
+def _no_tangent(who, *tensors):
+    if _forward_ad._current_level >= 0:
+        for t in tensors:
+            if t is not None and _forward_ad.unpack_dual(t).tangent is not None:
+                raise NotImplementedError(f"{who}: an input carries a forward-mode tangent; forward-mode derivatives are not supported")
+
+
+def _grad(who, *tensors):
+    """whether autograd has to record this call (a tangent would be dropped: refused)"""
+    _no_tangent(who, *tensors)
     return torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors)
 
 
@@ -206,6 +216,7 @@ def linrec_step(x, decay_gate, input_gate, decay, state, *, scale=8.0, slots=Non
     the same shape. slots [B] int32: the state row of each x row (None: row b is state b); a slot outside [0, n) marks a padded row (y = 0),
     rows that name one slot are consecutive steps of it in row order. No gradient."""
     who = "linrec_step"
+    _no_tangent(who, x, decay_gate, input_gate, decay, state, state_out)
     code = _first(x, who)
     if x.dim() not in (2, 3):
         raise ValueError(f"{who}: x has shape {tuple(x.shape)}, expected [B, D] or [B, n_agents, D]")
@@ -265,7 +276,7 @@ class _LinearRecurrence(torch.autograd.Function):
 
 def linear_recurrence(x, decay_gate, input_gate, decay, *, scale=8.0, h0=None, reset=None, lengths=None):
     """(y, h_last) of linrec_forward, differentiable in x, decay_gate, input_gate, decay and h0."""
-    if not _grad(x, decay_gate, input_gate, decay, h0):
+    if not _grad("linear_recurrence", x, decay_gate, input_gate, decay, h0):
         return linrec_forward(x, decay_gate, input_gate, decay, scale=scale, h0=h0, reset=reset, lengths=lengths)[:2]
     return _LinearRecurrence.apply(x, decay_gate, input_gate, decay, h0, reset, lengths, scale)
 
@@ -374,7 +385,7 @@ class _NormGate(torch.autograd.Function):
 
 def norm_gate_residual(x, o=None, gate=None, *, post_weight=None, res_scale=None, pre_weight=None, alpha=1.0, eps=1e-6, row_mask=None):
     """(y, n) of norm_gate_forward, differentiable in the tensors and the weights. Without o: (None, N(alpha x; pre_weight))."""
-    if not _grad(x, o, gate, post_weight, res_scale, pre_weight):
+    if not _grad("norm_gate_residual", x, o, gate, post_weight, res_scale, pre_weight):
         return norm_gate_forward(x, o, gate, post_weight=post_weight, res_scale=res_scale, pre_weight=pre_weight, alpha=alpha, eps=eps, row_mask=row_mask,
                                  want_y=o is not None)
     return _NormGate.apply(x, o, gate, post_weight, res_scale, pre_weight, alpha, eps, row_mask)
@@ -464,6 +475,6 @@ class _GatedFf(torch.autograd.Function):
 
 def gated_ff(x, w_gate, w_up, b_gate=None, b_up=None, *, act="silu"):
     """h of gated_ff_forward, differentiable in x, the weights and the biases."""
-    if not _grad(x, w_gate, w_up, b_gate, b_up):
+    if not _grad("gated_ff", x, w_gate, w_up, b_gate, b_up):
         return gated_ff_forward(x, w_gate, w_up, b_gate, b_up, act=act)[0]
     return _GatedFf.apply(x, w_gate, w_up, b_gate, b_up, act)

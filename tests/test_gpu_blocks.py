@@ -853,3 +853,25 @@ def test_the_block_as_a_whole_trains_and_acts():
             steps.append(block_pass(x[:, t], p, None, None, mask[:, t], state=state)[0])
         acted = torch.stack(steps, 1)
         assert (acted - full).abs().max() <= 3e-5 * full.abs().max() and (state - hT).abs().max() <= 3e-5 * hT.abs().max()
+
+
+def test_forward_mode_derivatives_are_refused():
+    """a tangent on any differentiable input raises, whether or not the input also requires a gradient; values without one pass, at any level"""
+    fw = torch.autograd.forward_ad
+    B, T, D, F = 2, 3, 8, 5
+    seq, decay, h0, w = [rnd(B, T, D, seed=i) for i in range(3)], rnd(D, seed=3), rnd(B, D, seed=4), 1 + 0.1 * rnd(D, seed=5)
+    wg, wu, b = rnd(F, D, seed=6), rnd(F, D, seed=7), rnd(F, seed=8)
+    calls = [(lambda x, ga, gi, d, h: blocks.linear_recurrence(x, ga, gi, d, h0=h), [*seq, decay, h0]),
+             (lambda x, o, g, a, c, e: blocks.norm_gate_residual(x, o, g, post_weight=a, res_scale=c, pre_weight=e), [*seq, w, w, w]),
+             (lambda *a: blocks.gated_ff(*a), [seq[0], wg, wu, b, b]),
+             (lambda x, ga, gi, d: blocks.linrec_step(x, ga, gi, d, h0.clone()), [seq[0][:, 0], seq[1][:, 0], seq[2][:, 0], decay])]
+    for f, args in calls:
+        for i in range(len(args)):
+            for needs_grad in (False, True):
+                with fw.dual_level(), torch.set_grad_enabled(needs_grad):
+                    primal = args[i].clone().requires_grad_(needs_grad)
+                    a = list(args)
+                    a[i] = fw.make_dual(primal, torch.ones_like(primal))
+                    with pytest.raises(RuntimeError, match="forward-mode"):
+                        f(*a)
+                    f(*args)
