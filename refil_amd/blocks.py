@@ -214,9 +214,11 @@ def linrec_backward(dy, x, decay_gate, input_gate, decay, saved, *, scale=8.0, h
 def linrec_step(x, decay_gate, input_gate, decay, state, *, scale=8.0, slots=None, state_out=None):
     """One step for the rows of x [B, D] / [B, n_agents, D]; returns y. state [n, ..., D] fp32, dense, is advanced in place, or into state_out of
     the same shape. slots [B] int32: the state row of each x row (None: row b is state b); a slot outside [0, n) marks a padded row (y = 0),
-    rows that name one slot are consecutive steps of it in row order. No gradient."""
+    rows that name one slot are consecutive steps of it in row order. No gradient: inputs that require one are refused outside torch.no_grad()."""
     who = "linrec_step"
-    _no_tangent(who, x, decay_gate, input_gate, decay, state, state_out)
+    if _grad(who, x, decay_gate, input_gate, decay, state, state_out):
+        raise RuntimeError(f"{who}: an input requires a gradient, which an acting step does not have: call it under torch.no_grad(), or train through "
+                           "linear_recurrence")
     code = _first(x, who)
     if x.dim() not in (2, 3):
         raise ValueError(f"{who}: x has shape {tuple(x.shape)}, expected [B, D] or [B, n_agents, D]")
@@ -251,6 +253,8 @@ def linrec_step(x, decay_gate, input_gate, decay, state, *, scale=8.0, slots=Non
     d = LinrecStepDesc(x.data_ptr(), x.stride(0), decay_gate.data_ptr(), decay_gate.stride(0), input_gate.data_ptr(), input_gate.stride(0), decay.data_ptr(),
                        a, b, _p(slots), y.data_ptr(), width, B, width, D, state.shape[0], code, scale)
     _launch(_lib.lib().refil_linrec_step, d, x.device, who)
+    if not out.is_inference():
+        torch.autograd.graph.increment_version(out)         # (written behind torch's back: a graph that kept it has to notice)
     return y
 
 

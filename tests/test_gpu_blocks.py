@@ -875,3 +875,40 @@ def test_forward_mode_derivatives_are_refused():
                     with pytest.raises(RuntimeError, match="forward-mode"):
                         f(*a)
                     f(*args)
+
+
+def test_linrec_step_tells_torch_that_the_state_changed():
+    """a graph that kept the state notices the step; state_out counts, a state that is only read does not; inference tensors have no counter"""
+    B, D = 3, 8
+    x, ga, gi, decay, state = rnd(B, D, seed=1), rnd(B, D, seed=2), rnd(B, D, seed=3), rnd(D, seed=4), rnd(B, D, seed=5)
+    leaf = rnd(B, D, seed=6).requires_grad_(True)
+    loss = (leaf * state).sum()
+    before = state._version
+    blocks.linrec_step(x, ga, gi, decay, state)
+    assert state._version > before
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        loss.backward()
+    out = torch.empty_like(state)
+    counts = state._version, out._version
+    blocks.linrec_step(x, ga, gi, decay, state, state_out=out)
+    assert state._version == counts[0] and out._version > counts[1]
+    with torch.inference_mode():
+        s = state.clone()
+        y = blocks.linrec_step(x, ga, gi, decay, s)
+    assert torch.equal(s, out) and not y.requires_grad
+
+
+def test_linrec_step_refuses_inputs_that_require_a_gradient():
+    """it has no backward: under no_grad parameters pass, elsewhere the call raises before anything is written"""
+    B, D = 3, 8
+    args = [rnd(B, D, seed=1), rnd(B, D, seed=2), rnd(B, D, seed=3), rnd(D, seed=4), rnd(B, D, seed=5)]
+    for i in range(5):
+        a = list(args)
+        a[i] = args[i].clone().requires_grad_(True)
+        keep = a[4].detach().clone()
+        with pytest.raises(RuntimeError, match="linrec_step: .*no_grad"):
+            blocks.linrec_step(*a)
+        assert torch.equal(a[4], keep)
+        with torch.no_grad():
+            y = blocks.linrec_step(*a)
+        assert not y.requires_grad and not torch.equal(a[4], keep)
