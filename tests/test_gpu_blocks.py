@@ -912,3 +912,27 @@ def test_linrec_step_refuses_inputs_that_require_a_gradient():
         with torch.no_grad():
             y = blocks.linrec_step(*a)
         assert not y.requires_grad and not torch.equal(a[4], keep)
+
+
+def rec_plan(args, kw, backward):
+    """(tiles of the time axis, chunks they are dealt to) of a call, from what it asks for: one state a tile and row is saved, two maps a chunk and row"""
+    from refil_amd import _lib
+    d = blocks._linrec_desc("rec_plan", *args, 8.0, kw["h0"], kw["reset"], kw["lengths"])
+    row = d.B * d.C
+    tiles = _lib.lib().refil_linrec_saved_floats(d) // row
+    ws = _lib.lib().refil_linrec_workspace_bytes(d, backward) // 4
+    sums = ws if not backward else ws - row                          # one chunk: no maps; the backward keeps a partial decay gradient a chunk
+    return tiles, 1 if sums == 0 else ws // (3 * row if backward else 2 * row)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("ragged", [True, False])
+@pytest.mark.parametrize("B,T,D,chunks", [(200, 200, 3, "several"), (1100, 100, 4, "one"), (100, 200, 130, "several"), (40, 260, 300, "several"), (700, 150, 5, "any")])
+def test_linrec_workgroups_that_walk_several_tiles(B, T, D, chunks, ragged, dtype):
+    """the carry from tile to tile, the LDS halves in turn, loads into the next (backward: the previous) tile, chunks' maps over several tiles: the plan
+    that a shape is here for is asserted"""
+    args, kw = rec_case(B, T, 0, D, dtype, seed=B + T + D, ragged=ragged, decay_shift=-5.0)
+    for backward in (0, 1):
+        tiles, n = rec_plan(args, kw, backward)
+        assert tiles > n and (n == 1 if chunks == "one" else n > 1 if chunks == "several" else True), (backward, tiles, n)
+    rec_check(args, kw, dh_last=rnd(B, D, seed=9))
