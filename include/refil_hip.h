@@ -469,8 +469,8 @@ int refil_gru_backward(const refil_gru_desc* desc, void* stream);
  * gate, residual. No counterpart in the reference (its one recurrence is the GRUCell of entity_rnn_agent.py:49-55). Element types of
  * the activations and the feed-forward weights: fp32, bf16 or fp16 (`dtype`); parameters of the recurrence and the norms, hidden
  * states and their gradients are fp32. All strides count ELEMENTS, the innermost dimension is contiguous, no alignment beyond the
- * element's is needed. Workspaces are scratch of one call: no content is kept, two calls in flight need two of them. Inputs and outputs
- * of one call must not overlap (except state / state_out of refil_linrec_step, which may be the same buffer). */
+ * element's is needed. Workspaces begin on 16 bytes and are scratch of one call: no content is kept, two calls in flight need two of them.
+ * Inputs and outputs of one call must not overlap (except state / state_out of refil_linrec_step, which may be the same buffer). */
 enum { REFIL_F32 = 0, REFIL_BF16 = 1, REFIL_F16 = 2 };
 
 /* Gated linear recurrence over [B, T, C], channel c with decay[c % D] (agents: C = n_agents * D):

@@ -880,6 +880,7 @@ extern "C" int refil_gated_ff_backward(const refil_gated_ff_desc* d, void* strea
                 "refil_gated_ff_backward: x, w_gate, w_up, saved, dh, dx, dw_gate and dw_up are required");
     const size_t need = refil_gated_ff_workspace_bytes(d, 1);
     REFIL_CHECK(d->workspace && d->workspace_bytes >= need, "refil_gated_ff_backward: workspace of %zu bytes, %zu needed", d->workspace_bytes, need);
+    REFIL_CHECK((uintptr_t)d->workspace % 16 == 0, "refil_gated_ff_backward: workspace must begin on 16 bytes");      // (gf_copy16 reads it)
     hipStream_t st = (hipStream_t)stream;
     return d->dtype == REFIL_F32 ? gf_backward<float>(*d, st) : d->dtype == REFIL_BF16 ? gf_backward<bf16_t>(*d, st) : gf_backward<f16_t>(*d, st);
 }

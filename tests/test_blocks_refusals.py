@@ -148,3 +148,18 @@ def test_sizing_queries_answer_zero_for_bad_descriptors():
     assert L.refil_linrec_saved_floats(C.byref(_lib.LinrecDesc(B=2, T=65, C=4, D=4, scale=1.0))) >= 2 * 2 * 4
     assert L.refil_norm_gate_workspace_bytes(C.byref(_lib.NormGateDesc(N=1, D=0, eps=1.0))) == 0
     assert L.refil_gated_ff_workspace_bytes(C.byref(_lib.GatedFfDesc(N=1, D=4, F=0)), 0) == 0
+
+
+def test_gated_ff_workspace_begins_on_16_bytes():
+    """its copies to LDS take 16 bytes at a time; the call before the one that is refused gets past this check, to the size's"""
+    L = _lib.lib()
+    buf = (C.c_float * 64)()
+    p = C.addressof(buf)
+    d = _lib.GatedFfDesc(x=p, w_gate=p, w_up=p, x_stride=8, w_stride=8, N=2, D=8, F=8, dtype=_lib.BF16, saved=p, dh=p, dh_stride=8, dx=p, dx_stride=8, dw_gate=p, dw_up=p)
+    need = L.refil_gated_ff_workspace_bytes(C.byref(d), 1)
+    base = (p + 63) // 64 * 64
+    d.workspace, d.workspace_bytes = base, need - 1
+    assert L.refil_gated_ff_backward(C.byref(d), None) != 0 and f"workspace of {need - 1} bytes" in _err()
+    for off in (1, 4, 8):
+        d.workspace, d.workspace_bytes = base + off, need
+        assert L.refil_gated_ff_backward(C.byref(d), None) != 0 and "workspace must begin on 16 bytes" in _err()
