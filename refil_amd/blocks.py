@@ -112,17 +112,17 @@ def _workspace(nbytes, x):
     return x.new_empty(nbytes, dtype=torch.uint8) if nbytes else None
 
 
-def _no_tangent(who, *tensors):
+def _grad(who, *tensors):
+    """whether autograd has to record this call. A forward-mode tangent, which a call without a recorded gradient would drop, is refused"""
     if _forward_ad._current_level >= 0:
         for t in tensors:
             if t is not None and _forward_ad.unpack_dual(t).tangent is not None:
                 raise NotImplementedError(f"{who}: an input carries a forward-mode tangent; forward-mode derivatives are not supported")
-
-
-def _grad(who, *tensors):
-    """whether autograd has to record this call (a tangent would be dropped: refused)"""
-    _no_tangent(who, *tensors)
-    return torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors)
+    if torch.is_grad_enabled():
+        for t in tensors:
+            if t is not None and t.requires_grad:
+                return True
+    return False
 
 
 def _no_capture(who):
