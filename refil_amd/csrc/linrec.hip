@@ -46,9 +46,12 @@ constexpr int LR_V = 4, LR_WAVES = 4;
 template <class T, int TC> struct LrGeo {
     static constexpr int CH = TC * LR_V, TW = 64 / TC, S = sizeof(T) == 4 ? 2 : 4, TT = LR_WAVES * TW * S;
 };
-// Which: B 4, T 8192, C 1024 bf16 took 98 + 133 us (forward, backward) with 64 lanes and 105 + 143 with 16; fp32 does not gain (78 + 116
-// against 78 + 120 us at T 4096), and many short episodes lose (96 of 81 steps: 45 against 31 us): few 16-bit sequences, wide rows.
-static int lr_tc(int dtype, int B, int C) { return dtype != REFIL_F32 && C > 128 && (long)B * cdiv(C, 64) <= 512 ? 64 : 16; }
+// Which: 64 lanes where 16 would have their time axis cut anyway (lr_plan: two chunks or more fit while (episode, 64 channels) pairs are at most
+// half of 768), so that the cheaper tile wins; beyond, 16 lanes pass once over the data. bf16, forward + backward at 33.5 million elements, 64 against
+// 16 lanes: 64 pairs (B 4, T 8192, C 1024) 100 + 133 against 102 + 141 us, 128 pairs 96 + 129 / 101 + 143, 256 pairs 96 + 130 / 97 + 143, 384 pairs
+// (36.9 million) 109 + 155 / 116 + 162; 512 pairs 96 + 130 / 63 + 118, 1024 pairs 93 + 130 / 67 + 127. fp32 does not gain (78 + 116 against
+// 78 + 120 us at B 4, T 4096, C 1024).
+static int lr_tc(int dtype, int B, int C) { return dtype != REFIL_F32 && C > 128 && (long)B * cdiv(C, 64) <= 384 ? 64 : 16; }
 static int lr_tile(int dtype, int B, int C) {
     return dtype == REFIL_F32 ? LrGeo<float, 16>::TT : lr_tc(dtype, B, C) == 64 ? LrGeo<bf16_t, 64>::TT : LrGeo<bf16_t, 16>::TT;
 }
@@ -684,7 +687,7 @@ static LrPlan lr_plan(const refil_linrec_desc& d, bool bwd) {
     p.ntile = cdiv(d.T, lr_tile(d.dtype, d.B, d.C));
     // Too few (episode, column) pairs to fill the card: the time axis is cut into chunks of whole tiles, at the price of reading the
     // inputs once more for the chunks' maps -- as many as the card holds at once (waves per SIMD by registers: launch bounds), so that
-    // there is one round of workgroups and each starts once.
+    // there is one round of workgroups and each starts once. (256 compute units of four SIMDs.)
     const bool wide = d.dtype == REFIL_F32;
     const long pairs = (long)d.B * p.ncol, hold = 256L * (bwd ? (wide ? 3 : 2) : (wide ? 4 : 3));
     long n = pairs > 0 ? hold / pairs : 1;
