@@ -3,17 +3,18 @@
 // Every product is C[m][n] = sum_k A(m, k) B(n, k) on v_mfma_f32_16x16x32 (fp32 accumulate), tiles staged through LDS:
 //   forward   A = x, B = rows of Wg and Wu interleaved so that one wave holds both projections of a column: bias, activation and product
 //             happen in its registers; h (and for training the two pre-activations, fp32) is all that is written
-//   backward  one elementwise pass turns the saved pre-activations and dh into [dg | du] (rounded to the type once) and the bias sums;
+//   backward  one elementwise pass turns the saved pre-activations and dh into [dg | du] (rounded to the type once; fp16: kept in range by a
+//             power of two) and the bias sums;
 //             dx = [dg | du] [Wg ; Wu] and [dWg ; dWu] = [dg | du]^T x read the operands as they lie in memory: where the reduction index
 //             is the row, the LDS tile keeps rows of k and ds_read_b64_tr_b16 hands the matrix core its columns -- nothing is transposed
 // fp32 operands are split exactly into three bf16 pieces on their way into LDS and a product runs as six bf16 products (lo hi, hi lo,
 // mid mid, mid hi, hi mid, hi hi), as the library's projection GEMMs do.
 // Few rows, where the weights' bytes are the cost, and launches of few tiles have a second kernel that reads straight into matrix-core fragments.
 //
-// Bound by the matrix cores. N 8192, D 2048, F 8192 in bf16: forward with the pre-activations kept 575 .. 600 us (550 GFLOP, 0.92 .. 0.96
-// PFLOP/s under 671 MB of writes), dx 463 .. 490 us (1.12 .. 1.19 PFLOP/s), dw 511 .. 530, the elementwise pass 193 us (940 MB, 4.9 TB/s); a
-// large library product reaches 1.33 PFLOP/s here. N 41472, D 128, F 512 in fp32: 119 us forward, 227 backward, 32.6 GFLOP in all = 94
-// TFLOP/s of fp32 work (the fp32 instruction's library product: 154 at 8192^3), a quarter of it the elementwise pass.
+// Bound by the matrix cores. N 8192, D 2048, F 8192 in bf16: forward with the pre-activations kept 579 us (550 GFLOP, 0.95 PFLOP/s under 671 MB
+// of writes), dx 440 us (1.25 PFLOP/s), dw 469 (1.17), the elementwise pass 189 us (940 MB, 5.0 TB/s); a large library product reaches 1.33
+// PFLOP/s here. (At the card's steady clock: the first dozen passes take up to 15 % longer.) N 41472, D 128, F 512 in fp32: 122 us forward, 237
+// backward, 32.6 GFLOP in all = 91 TFLOP/s of fp32 work (the fp32 instruction's library product: 154 at 8192^3), a fifth of it the elementwise pass.
 #include <type_traits>
 
 #include "kernels.h"

@@ -16,9 +16,9 @@
 //   dga_t = q_t (1 - sigmoid(ga)),   ddecay = sum q_t sigmoid(decay) / softplus(decay)
 //
 // Bound by memory and by the latency of a tile (gates, shuffles, one barrier), which other waves of the compute unit hide. 96 ragged
-// episodes of 81 steps, 1024 channels in fp32: 31 + 48 us. Where sequences are too few to fill the card, time is cut into chunks, one round
+// episodes of 81 steps, 1024 channels in fp32: 30 + 45 us. Where sequences are too few to fill the card, time is cut into chunks, one round
 // of workgroups in all: a first launch makes the chunks' maps (3 streams read; backward 2), the second starts every chunk from the maps in
-// front of it. 4 sequences of 8192 steps, 1024 channels in bf16: 50 + 64 us forward (4.0 and 4.2 TB/s), 30 + 113 us backward.
+// front of it. 4 sequences of 8192 steps, 1024 channels in bf16: 42 + 58 us forward, 28 + 101 us backward (maps and outputs; 4.6 .. 4.9 TB/s).
 #include <type_traits>
 
 #include "kernels.h"

@@ -13,10 +13,10 @@
 // The column sums stay in registers (the widest rows: in LDS) over a workgroup's rows, are joined in LDS, and a second launch adds the
 // workgroups' partial rows in a fixed order: no atomics, the same result every time.
 //
-// Bound by memory: N 16384, D 2048 in bf16 with a gate takes 64 us forward (5 streams, 5.2 TB/s) and 101 us backward (8 streams, 5.3 TB/s; a
-// large copy reaches 4.7 .. 4.9), N 41472, D 128 in fp32 with a fifth of its rows masked 17.7 + 31 us. Narrow rows share a workgroup so
+// Bound by memory: N 16384, D 2048 in bf16 with a gate takes 64 us forward (5 streams, 5.2 TB/s) and 102 us backward (8 streams, 5.3 TB/s; a
+// large copy reaches 4.7 .. 4.9), N 41472, D 128 in fp32 with a fifth of its rows masked 17.5 + 29 us. Narrow rows share a workgroup so
 // that a wave's loads stay whole lines; the next row's loads leave in front of this row's sums, which is what keeps memory busy through the
-// barriers. Few rows (N 128, D 64: 3.8 us) are a launch and one round of latency.
+// barriers. Few rows (N 128, D 64: 3.7 us) are a launch and one round of latency.
 #include "kernels.h"
 #include "profile.h"
 #include "vecio.h"
